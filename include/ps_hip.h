@@ -523,6 +523,93 @@ uint64_t ps_hip_seq_weight_bytes_per_token(const ps_hip_seq *m);
  * expert that has matrices -- identity experts take neither).  A few tokens run the mat-vec. */
 int ps_hip_seq_bench_kernel(ps_hip_seq *m, int which, int T, int reps, double *us_per_launch, double *bytes, double *flops);
 
+/* ------------------------------------------------------------------ a serving step of many sequences
+ * Operators over device memory that the caller holds, for steps that serve several sequences at once: attention over their caches (ps_hip_cache_*), sampling from their logits
+ * (ps_hip_sample) and low-rank adapters beside a shared projection (ps_hip_adapters_*).  Everything that changes from step to step -- lengths, counts, trees, settings, ids -- is read from
+ * DEVICE arrays by the kernels, and scratch memory is the caller's (its size from the *_workspace function beside the call; 16-byte aligned; nothing is kept in it between calls), so that calls
+ * on the ctx stream can be captured into a graph and replayed.  Two calls that may run at the same time (graphs, contexts) need a workspace each.  All calls only enqueue.  Buffers
+ * lie on the ctx's device; memory last written on another stream is the caller's to order.  No two buffers of a call overlap unless it says so.  A refused call enqueues nothing. */
+
+/* The keys and values of one attention layer for n_seqs sequences: number e of kv head g in slot j of sequence s is k[s * seq_stride + j * slot_stride + g * head_stride + e], the same for v; slots
+ * of one layer may lie between those of others.  Rows are 16-byte aligned (pointers, and strides times the size of a number); dim is a multiple of 8, 8 to 128.  The slots 0 .. n_kv[s] - 1 are
+ * held, in any order: attention does not depend on it, positions are part of the keys. */
+typedef struct {
+    int32_t dtype; /* PS_F32, PS_F16, PS_BF16 */
+    int32_t n_seqs, n_ctx /* slots */, kv_heads, dim, _pad;
+    void *k, *v;
+    int64_t seq_stride, slot_stride, head_stride;
+    int32_t *n_kv;  /* [n_seqs]; a number below 0 is taken as 0, above n_ctx as n_ctx */
+    int32_t *pos;   /* [n_seqs][kv_heads][n_ctx] position of the token in a slot, or NULL (ps_hip_cache_evict needs it) */
+    float *weight;  /* [n_seqs][kv_heads][n_ctx] attention weight that a slot has accumulated, or NULL */
+} ps_kv_cache;
+
+/* Attention of the newest tokens: token t < count[s] of sequence s goes into slot n_kv[s] + t (written here where k_new / v_new are given; they are there already where both are NULL; n_kv is not
+ * changed: a step may be repeated) and attends to the slots before n_kv[s] and to the new tokens u with tree[s][t][u] != 0, or u <= t where tree is NULL.  Query head h reads kv head
+ * h / (heads / kv_heads).  out = soft-max(scale * q . k) . v, zero for a token that sees nothing; sums, maxima and soft-max in fp32, the numbers that multiply the values in 16 bits for 16-bit
+ * caches (two of them for few rows).  weight_out (NULL: not wanted; may be cache->weight): a slot's soft-max weights, summed over all tokens of the call and the query heads of its kv head, added
+ * to cache->weight (NULL: to nothing) for the slots before n_kv[s] and set for the new ones; other slots are left as they were.  Tokens that do not fit behind n_kv[s] are left out,
+ * as if count[s] were smaller; rows of out behind count[s] are left as they were.  A number that a token does not see does not reach its result, whatever it is. */
+typedef struct {
+    int32_t heads, n_new; /* query heads; rows per sequence of q, out, k_new, v_new, tree (n_new x n_new bytes), pos_new */
+    float scale;
+    int32_t _pad;
+    const void *q;  /* number e of head h of token t: q[s * q_seq_stride + t * q_row_stride + h * dim + e]; the cache's type; rows 16-byte aligned */
+    void *out;      /* the same with out_*_stride; not q */
+    const void *k_new, *v_new; /* [s * new_seq_stride + t * new_row_stride + g * dim + e], both or neither */
+    int64_t q_seq_stride, q_row_stride, out_seq_stride, out_row_stride, new_seq_stride, new_row_stride; /* 0: rows one behind the other */
+    const int32_t *count;   /* [n_seqs], or NULL: n_new each */
+    const int32_t *pos_new; /* [n_seqs][n_new] written to cache->pos for every kv head, or NULL */
+    const uint8_t *tree;
+    float *weight_out;
+} ps_cache_attn_params;
+size_t ps_hip_cache_attn_workspace(ps_hip_ctx *ctx, const ps_kv_cache *cache, const ps_cache_attn_params *p);
+int ps_hip_cache_attn(ps_hip_ctx *ctx, const ps_kv_cache *cache, const ps_cache_attn_params *p, void *workspace, size_t workspace_bytes);
+/* Takes new tokens into the cache: n_kv[s] += count[s].  take (NULL: the first count[s] tokens): [n_seqs][n_take] ascending indices of the tokens that stay, an accepted path of a tree -- token take[s][i]
+ * moves to slot n_kv[s] + i first, keys, values, cache->pos and cache->weight where they are given.  An index that is not above the one before it, or lies behind the last slot, ends a
+ * sequence's list; count[s] is bounded by n_take and by the slots that are left. */
+int ps_hip_cache_advance(ps_hip_ctx *ctx, const ps_kv_cache *cache, const int32_t *count, const int32_t *take, int n_take);
+
+/* Eviction: of a sequence that holds more than `keep` slots, every kv head keeps its own `keep`: those whose position is below `first` or above its largest position less `recent`, then those of the
+ * largest accumulated weight (equal ones: the lower slot; NaN is below every number).  recent + first <= keep.  The kept slots at `keep` and behind, in ascending order, move to the places below
+ * `keep` of the evicted ones, in ascending order: keys, values, position, weight.  Then n_kv[s] = keep.  Other sequences, and slots from `keep` on, are left as they were.
+ * weight_out / pos_out / n_kv_out: where the new weights, positions and lengths go instead of the cache's arrays (the slots that are held afterwards), or NULL; a repeated call with all three
+ * gives the same result. */
+typedef struct {
+    int32_t keep, recent, first, _pad;
+    float *weight_out;
+    int32_t *pos_out, *n_kv_out;
+} ps_cache_evict_params;
+size_t ps_hip_cache_evict_workspace(ps_hip_ctx *ctx, const ps_kv_cache *cache, const ps_cache_evict_params *p);
+int ps_hip_cache_evict(ps_hip_ctx *ctx, const ps_kv_cache *cache, const ps_cache_evict_params *p, void *workspace, size_t workspace_bytes);
+
+/* Sampling, the stages of the host's sampler chain in its order (top-k, temperature, soft-max, top-p, draw) with min-p beside top-p and the random number given: the candidates of a row of logits are
+ * taken from the largest to the smallest, equal ones by index; NaN and minus infinity are none.  With w = exp((logit - largest) / temperature): the first top_k (<= 0: all); of those the shortest
+ * beginning whose w add up to top_p of theirs (>= 1 or NaN: all; at least one); of those the ones with w >= min_p (<= 0 or NaN: all; the largest always stays); then the first whose w, added up to
+ * and with it, exceed u times the sum of the ones left (u < 0 or NaN: 0; u >= 1: the last).  A temperature that is not above 0 takes the first candidate.  A row without candidates gives id -1 and
+ * probability 0.  Weights are computed in 64 bits and added as whole multiples of 2^-44 or less of the largest one, so that no order of work changes a result; a weight below e^-40 of the
+ * largest is 0.  NULL arrays: temperature 1, no filter; u is required. */
+typedef struct {
+    const float *temperature; /* device [rows] each */
+    const int32_t *top_k;
+    const float *top_p, *min_p, *u;
+} ps_sample_params;
+size_t ps_hip_sample_workspace(ps_hip_ctx *ctx, int64_t n, int64_t rows);
+/* logits: [rows][n] of dtype PS_F32, PS_F16 or PS_BF16, rows `stride` numbers apart; ids int32 [rows]; prob [rows] the taken token's share of the candidates left, or NULL (device) */
+int ps_hip_sample(ps_hip_ctx *ctx, int dtype, const void *logits, int64_t n, int64_t rows, int64_t stride, const ps_sample_params *p, int32_t *ids, float *prob, void *workspace,
+                  size_t workspace_bytes);
+
+/* Low-rank adapters of one dense matrix [N, K] (ps_hip_dense_*): slot a holds down [rank, K], up [N, rank] and a scale, and token t with ids[t] = a gets out[t] = base[t] + scale * up (down x[t]);
+ * tokens whose id is no loaded slot get out = base.  Matrices are bfloat16, every product of them exact and every sum fp32 (x in fp32 is taken whole).  base: the shared projection's output, may be out; NULL: zeros. */
+typedef struct ps_adapters ps_adapters;
+int ps_hip_adapters_create(ps_hip_ctx *ctx, int64_t N, int64_t K, int n_slots, int max_rank, ps_adapters **out);
+/* host_down [rank][K], host_up [N][rank] bfloat16 bit patterns; rank 0 empties the slot.  Waits for the stream: what was enqueued before sees the old adapter, what follows the new one. */
+int ps_hip_adapters_load(ps_hip_ctx *ctx, ps_adapters *a, int slot, const uint16_t *host_down, const uint16_t *host_up, int rank, float scale);
+void ps_hip_adapters_free(ps_hip_ctx *ctx, ps_adapters *a);
+size_t ps_hip_adapters_workspace(const ps_adapters *a, int T);
+/* x [T][ldx] of x_dtype (PS_F32, PS_BF16), base and out [T][ldo] fp32, ids int32 [T] (device) */
+int ps_hip_adapters_apply(ps_hip_ctx *ctx, const ps_adapters *a, int x_dtype, const void *x, int64_t ldx, int T, const int32_t *ids, const float *base, float *out, int64_t ldo, void *workspace,
+                          size_t workspace_bytes);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,505 @@
+// Attention of the newest tokens of many sequences over their caches (ps_hip_cache_attn), with the attention weight every slot receives, and taking an accepted path (ps_hip_cache_advance).
+//   O = softmax(scale Q K^T + mask) V per kv head; its rows are the new tokens times the query heads that share the head (row t R + r: token t, query head r of R), its keys the held slots and the
+//   new tokens.  Weight of a slot = the sum over rows of its soft-max weights.
+//   cache_attn_kernel     16 RT rows of one kv head against a part of its keys; the waves of a work-group share the part (blocks of 32 keys in turn), join in LDS, and leave sum, maximum and
+//                         unnormed result of the part -- or the result itself where there is one part.  New rows go into the cache on the way.
+//   cache_join_kernel     the parts of a row together; a row's log-sum of weights is left for
+//   cache_weight_kernel   64 keys against all rows once more: the soft-max weights from the scores and the log-sums, summed over rows in a fixed order
+// S^T = K Q^T, so that a lane has one row and maximum and sum run over its own registers and two lane moves; the second product O^T = V^T P^T takes its 32 keys in any order that both operands
+// share, so a lane's weights are its piece of the operand as they are.  16-bit values pass through LDS, a wave's own stretch, and come back transposed (ds_read_b64_tr_b16: 4 keys x 16 numbers).
+// Lengths are read on the device; a part is ceil(length / parts) keys, so that a fixed grid serves any length.
+#include "ps_serve.h"
+
+#include <algorithm>
+#include <cmath>
+
+namespace {
+typedef __bf16 b8 __attribute__((ext_vector_type(8)));
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+typedef short s4 __attribute__((ext_vector_type(4)));
+struct F16 { static constexpr int SIZE = 2; };
+struct BF16 { static constexpr int SIZE = 2; };
+struct F32 { static constexpr int SIZE = 4; };
+
+struct ca_args {
+    char *k, *v, *out;
+    const char *q, *k_new, *v_new;
+    long long seq, slot, head, q_seq, q_row, o_seq, o_row, new_seq, new_row; // strides in bytes
+    int n_seqs, n_ctx, G, dim, R, T;
+    float sc2; // scale * log2(e): scores are held in units of log 2
+    const int32_t *n_kv, *count, *pos_new;
+    int32_t *pos;
+    const uint8_t *tree;
+    const float *weight;
+    float *weight_out;
+    float *part; // [seq][kv head][16 rows][part]: 16 x dim results, 16 maxima, 16 sums
+    float *lse;  // [seq][kv head][T R] log2 of the sum of weights (+inf: no weights)
+    int parts, tiles; // tiles of 16 rows
+};
+struct ca_lens { int n0, cnt, len; };
+__device__ __forceinline__ ca_lens lens_of(const ca_args &a, int s) {
+    ca_lens l;
+    l.n0 = min(max(a.n_kv[s], 0), a.n_ctx);
+    l.cnt = min(max(a.count ? a.count[s] : a.T, 0), min(a.T, a.n_ctx - l.n0));
+    l.len = l.n0 + l.cnt;
+    return l;
+}
+__device__ __forceinline__ int chunk_of(int len, int parts) { return max(128, ((len + parts - 1) / parts + 127) / 128 * 128); }
+__device__ __forceinline__ bool sees(const ca_args &a, int s, int t, int u) { return a.tree ? a.tree[((long long)s * a.T + t) * a.T + u] != 0 : u <= t; }
+
+template <class E> __device__ __forceinline__ pv_f4 mfma(const pv_u4 &x, const pv_u4 &y, const pv_f4 &c);
+template <> __device__ __forceinline__ pv_f4 mfma<BF16>(const pv_u4 &x, const pv_u4 &y, const pv_f4 &c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8, x), __builtin_bit_cast(b8, y), c, 0, 0, 0);
+}
+template <> __device__ __forceinline__ pv_f4 mfma<F16>(const pv_u4 &x, const pv_u4 &y, const pv_f4 &c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, x), __builtin_bit_cast(h8, y), c, 0, 0, 0);
+}
+// two numbers to 16 bits, to nearest even, and what that leaves
+template <class E> __device__ __forceinline__ unsigned round2(float a, float b) {
+    if constexpr (sizeof(E) && __is_same(E, BF16)) return __builtin_bit_cast(unsigned, __builtin_convertvector((pv_f2){a, b}, b2));
+    else return __builtin_bit_cast(unsigned, __builtin_convertvector((pv_f2){a, b}, h2));
+}
+template <class E> __device__ __forceinline__ pv_f2 wide2(unsigned u) {
+    if constexpr (__is_same(E, BF16)) return (pv_f2){__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u)};
+    else { const h2 h = __builtin_bit_cast(h2, u); return (pv_f2){(float)h[0], (float)h[1]}; }
+}
+template <class E> __device__ __forceinline__ bool odd16(unsigned u) { // infinities or NaN among two 16-bit numbers
+    constexpr unsigned m = __is_same(E, BF16) ? 0x7f80u : 0x7c00u;
+    return (u & m) == m || (u >> 16 & m) == m;
+}
+// the infinities and NaN of two 16-bit numbers alone, or the others alone
+template <class E> __device__ __forceinline__ unsigned without_odd(unsigned u) {
+    constexpr unsigned m = __is_same(E, BF16) ? 0x7f80u : 0x7c00u;
+    return ((u & m) == m ? 0u : u & 0xffffu) | ((u >> 16 & m) == m ? 0u : u & 0xffff0000u);
+}
+__device__ __forceinline__ bool odd32(float v) { return (__float_as_uint(v) & 0x7f800000u) == 0x7f800000u; }
+template <class E> __device__ __forceinline__ float number(const char *p) {
+    if constexpr (E::SIZE == 4) return *(const float *)p;
+    else return wide2<E>(*(const unsigned short *)p)[0];
+}
+
+// The frames of operands.  16-bit: a lane's piece of 16 x 32 numbers is 8 numbers of one row, of k step s 32 s + 8 (l / 16) ..; fp32: four steps' numbers at once, 16 s + 4 (l / 16) ..
+template <class E, int DP> constexpr int STEPS = E::SIZE == 2 ? DP / 32 : DP / 16;
+template <class E, int DP> using frame = pv_u4[STEPS<E, DP>];
+template <class E, int DP>
+__device__ __forceinline__ void get_row(frame<E, DP> &f, const char *row, int q, int dim) { // zeros behind dim
+#pragma unroll
+    for (int s = 0; s < STEPS<E, DP>; s++) {
+        const int e = E::SIZE == 2 ? 32 * s + 8 * q : 16 * s + 4 * q;
+        f[s] = *(const pv_u4 *)(row + (e < dim ? e * E::SIZE : 0));
+        if (e >= dim) f[s] = (pv_u4){0, 0, 0, 0};
+    }
+}
+template <class E, int DP>
+__device__ __forceinline__ pv_f4 dot(const frame<E, DP> &k, const frame<E, DP> &q) {
+    pv_f4 c = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int s = 0; s < STEPS<E, DP>; s++) {
+        if constexpr (E::SIZE == 2) c = mfma<E>(k[s], q[s], c);
+        else {
+#pragma unroll
+            for (int e = 0; e < 4; e++) c = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(k[s][e]), __uint_as_float(q[s][e]), c, 0, 0, 0);
+        }
+    }
+    return c;
+}
+
+constexpr int VPAD = 8; // numbers behind a value row in LDS
+
+template <class E, int DP, int RT>
+__global__ __launch_bounds__(256) void cache_attn_kernel(const ca_args a) {
+    constexpr int NS = STEPS<E, DP>, ND = DP / 16, OP = DP + 4, VR = DP + VPAD;
+    constexpr int VBYTES = E::SIZE == 2 ? 4 * 32 * VR * 2 : 0, OBYTES = 4 * 16 * OP * 4;
+    __shared__ __attribute__((aligned(16))) char lds[VBYTES > OBYTES ? VBYTES : OBYTES];
+    __shared__ float lm[4][16], ll[4][16];
+    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, c = lane & 15, q4 = lane >> 4;
+    const int blocks = (a.tiles + RT - 1) / RT;
+    int id = blockIdx.x;
+    const int rb = id % blocks; id /= blocks;
+    const int split = id % a.parts; id /= a.parts;
+    const int g = id % a.G, s = id / a.G;
+    const ca_lens L = lens_of(a, s);
+    const int chunk = chunk_of(L.len, a.parts), k0 = split * chunk, k1 = min(L.len, k0 + chunk);
+    if (L.cnt == 0 || (k0 >= L.len && split > 0) || rb * RT * 16 >= L.cnt * a.R) return;
+    const char *kb_ = a.k + s * a.seq + g * a.head, *vb_ = a.v + s * a.seq + g * a.head;
+    const char *kn = a.k_new ? a.k_new + s * a.new_seq + (long long)g * a.dim * E::SIZE : nullptr, *vn = a.k_new ? a.v_new + s * a.new_seq + (long long)g * a.dim * E::SIZE : nullptr;
+    auto row_at = [&](const char *held, const char *fresh, int j) { return fresh && j >= L.n0 ? fresh + (j - L.n0) * a.new_row : held + j * a.slot; };
+
+    pv_u4 qf[RT][NS];
+    int tok[RT];
+    pv_f4 o[RT][ND];
+    float m[RT], l[RT];
+#pragma unroll
+    for (int r = 0; r < RT; r++) {
+        const int row = min((rb * RT + r) * 16 + c, L.cnt * a.R - 1); // rows behind the last repeat it
+        tok[r] = row / a.R;
+        get_row<E, DP>(qf[r], a.q + s * a.q_seq + tok[r] * a.q_row + (long long)(g * a.R + row % a.R) * a.dim * E::SIZE, q4, a.dim);
+        m[r] = -INFINITY;
+        l[r] = 0.f;
+#pragma unroll
+        for (int d = 0; d < ND; d++) o[r][d] = (pv_f4){0.f, 0.f, 0.f, 0.f};
+    }
+    bool odd = false; // a new token's values hold infinities or NaN: they stay out of the products and join those rows that see them
+    unsigned short *vl = (unsigned short *)lds + wave * 32 * VR;
+
+    // a block's operands: keys of two tiles of 16; values as rows (16-bit) or as they are multiplied (fp32: keys 4 (l / 16) + i, numbers 64 x + 4 c ..)
+    constexpr int LPR = DP / 8, RPI = 64 / LPR, VI = E::SIZE == 2 ? 32 / RPI : 8 * (DP / 64);
+    pv_u4 kf[2][NS], vf[VI];
+    const int vr = lane / LPR, vc = lane % LPR * 8;
+    auto fetch = [&](int kb) {
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+            const int j = min(kb + 16 * u + c, k1 - 1);
+            get_row<E, DP>(kf[u], row_at(kb_, kn, j), q4, a.dim);
+        }
+#pragma unroll
+        for (int i = 0; i < VI; i++) {
+            const int r = E::SIZE == 2 ? i * RPI + vr : 16 * (i / (4 * (DP / 64))) + 4 * q4 + i / (DP / 64) % 4, e = E::SIZE == 2 ? vc : 64 * (i % (DP / 64)) + 4 * c;
+            const int j = kb + r;
+            vf[i] = *(const pv_u4 *)(row_at(vb_, vn, min(j, k1 - 1)) + (e < a.dim ? e * E::SIZE : 0));
+            if (j >= k1 || e >= a.dim) vf[i] = (pv_u4){0, 0, 0, 0};
+        }
+    };
+    if (k0 + wave * 32 < k1) fetch(k0 + wave * 32);
+    for (int kb = k0 + wave * 32; kb < k1; kb += 128) {
+        if (kb + 32 > L.n0) { // new tokens among the keys
+            if (kn && rb == 0) {
+#pragma unroll
+                for (int u = 0; u < 2; u++) {
+                    const int j = kb + 16 * u + c;
+                    if (j >= L.n0 && j < k1) {
+#pragma unroll
+                        for (int st = 0; st < NS; st++) {
+                            const int e = E::SIZE == 2 ? 32 * st + 8 * q4 : 16 * st + 4 * q4;
+                            if (e < a.dim) *(pv_u4 *)(a.k + s * a.seq + g * a.head + j * a.slot + e * E::SIZE) = kf[u][st];
+                        }
+                        if (q4 == 0 && a.pos_new && a.pos) a.pos[((long long)s * a.G + g) * a.n_ctx + j] = a.pos_new[(long long)s * a.T + j - L.n0];
+                    }
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < VI; i++) {
+                const int r = E::SIZE == 2 ? i * RPI + vr : 16 * (i / (4 * (DP / 64))) + 4 * q4 + i / (DP / 64) % 4, e = E::SIZE == 2 ? vc : 64 * (i % (DP / 64)) + 4 * c;
+                const int j = kb + r;
+                if (j < L.n0 || j >= k1 || e >= a.dim) continue;
+                if (vn && rb == 0) *(pv_u4 *)(a.v + s * a.seq + g * a.head + j * a.slot + e * E::SIZE) = vf[i];
+#pragma unroll
+                for (int x = 0; x < 4; x++) {
+                    if constexpr (E::SIZE == 2) {
+                        if (odd16<E>(vf[i][x])) { odd = true; vf[i][x] = without_odd<E>(vf[i][x]); }
+                    } else if (odd32(__uint_as_float(vf[i][x]))) { odd = true; vf[i][x] = 0u; }
+                }
+            }
+        }
+        pv_u4 vk[VI];
+        if constexpr (E::SIZE == 2) {
+#pragma unroll
+            for (int i = 0; i < VI; i++) *(pv_u4 *)(vl + (i * RPI + vr) * VR + vc) = vf[i];
+        } else {
+#pragma unroll
+            for (int i = 0; i < VI; i++) vk[i] = vf[i];
+        }
+        pv_f4 z[RT][2];
+#pragma unroll
+        for (int r = 0; r < RT; r++)
+#pragma unroll
+            for (int u = 0; u < 2; u++) z[r][u] = dot<E, DP>(kf[u], qf[r]);
+        if (kb + 128 < k1) fetch(kb + 128);
+        const bool edge = kb + 32 > min(L.n0, k1);
+#pragma unroll
+        for (int r = 0; r < RT; r++) {
+            float top = -INFINITY;
+#pragma unroll
+            for (int u = 0; u < 2; u++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    float v = z[r][u][i] * a.sc2;
+                    if (edge) {
+                        const int j = kb + 16 * u + 4 * q4 + i;
+                        if (j >= k1 || (j >= L.n0 && !sees(a, s, tok[r], j - L.n0))) v = -INFINITY;
+                    }
+                    z[r][u][i] = v;
+                    top = fmaxf(top, v);
+                }
+            top = fmaxf(top, __shfl_xor(top, 16, 64));
+            top = fmaxf(top, __shfl_xor(top, 32, 64));
+            const float mn = fmaxf(m[r], top), ms = mn == -INFINITY ? 0.f : mn, al = __builtin_amdgcn_exp2f(m[r] - ms);
+            float p[8], sum = 0.f;
+#pragma unroll
+            for (int u = 0; u < 2; u++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    p[4 * u + i] = __builtin_amdgcn_exp2f(z[r][u][i] - ms);
+                    sum += p[4 * u + i];
+                }
+            m[r] = mn;
+            l[r] = fmaf(l[r], al, sum);
+#pragma unroll
+            for (int d = 0; d < ND; d++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) o[r][d][i] *= al;
+            if constexpr (E::SIZE == 2) {
+                // the weights as two 16-bit numbers each: what the second product rounds off is 2^-17 (bf16; fp16 2^-23) of a weight, not the 2^-9 that would stand beside the result's own
+                // rounding; these products are not what bounds a pass over the cache
+                pv_u4 hi, lo;
+#pragma unroll
+                for (int x = 0; x < 4; x++) {
+                    hi[x] = round2<E>(p[2 * x], p[2 * x + 1]);
+                    const pv_f2 w = wide2<E>(hi[x]);
+                    lo[x] = round2<E>(p[2 * x] - w[0], p[2 * x + 1] - w[1]);
+                }
+                const unsigned short *base = vl + (4 * q4 + (c >> 2)) * VR + 4 * (c & 3);
+#pragma unroll
+                for (int d = 0; d < ND; d++) {
+                    typedef __attribute__((address_space(3))) s4 lds_s4;
+                    const s4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)(base + 16 * d)), y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)(base + 16 * VR + 16 * d));
+                    pv_u4 vt;
+                    const pv_u2 xx = __builtin_bit_cast(pv_u2, x), yy = __builtin_bit_cast(pv_u2, y);
+                    vt[0] = xx[0]; vt[1] = xx[1]; vt[2] = yy[0]; vt[3] = yy[1];
+                    o[r][d] = mfma<E>(vt, hi, o[r][d]);
+                    o[r][d] = mfma<E>(vt, lo, o[r][d]);
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < VI; i++) {
+                    const int x = i % (DP / 64);
+#pragma unroll
+                    for (int e = 0; e < 4; e++) o[r][4 * x + e] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(vk[i][e]), p[i / (DP / 64)], o[r][4 * x + e], 0, 0, 0);
+                }
+            }
+        }
+    }
+    // the four waves together
+    float *ol = (float *)lds;
+    odd = __syncthreads_or(odd);
+#pragma unroll
+    for (int r = 0; r < RT; r++) {
+        if (r) __syncthreads();
+        l[r] += __shfl_xor(l[r], 16, 64);
+        l[r] += __shfl_xor(l[r], 32, 64);
+        if (q4 == 0) { lm[wave][c] = m[r]; ll[wave][c] = l[r]; }
+        float *mine = ol + (wave * 16 + c) * OP;
+        if constexpr (E::SIZE == 2) {
+#pragma unroll
+            for (int d = 0; d < ND; d++) *(pv_f4 *)(mine + 16 * d + 4 * q4) = o[r][d];
+        } else {
+#pragma unroll
+            for (int x = 0; x < DP / 64; x++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) *(pv_f4 *)(mine + 64 * x + 16 * q4 + 4 * i) = (pv_f4){o[r][4 * x][i], o[r][4 * x + 1][i], o[r][4 * x + 2][i], o[r][4 * x + 3][i]};
+        }
+        __syncthreads();
+        const int tile = rb * RT + r, rr = tid >> 4, row = tile * 16 + rr;
+        if (row >= L.cnt * a.R) continue;
+        float top = fmaxf(fmaxf(lm[0][rr], lm[1][rr]), fmaxf(lm[2][rr], lm[3][rr])), f[4], sum = 0.f;
+        const float ms = top == -INFINITY ? 0.f : top;
+#pragma unroll
+        for (int w = 0; w < 4; w++) { f[w] = __builtin_amdgcn_exp2f(lm[w][rr] - ms); sum = fmaf(ll[w][rr], f[w], sum); }
+        const int t = row / a.R, hd = g * a.R + row % a.R;
+        float *part = a.part + ((((long long)s * a.G + g) * a.tiles + tile) * a.parts + split) * (16 * (a.dim + 2));
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+        for (int e = (tid & 15) * 4; e < a.dim; e += 64) {
+            pv_f4 v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int w = 0; w < 4; w++) {
+                const pv_f4 x = *(const pv_f4 *)(ol + (w * 16 + rr) * OP + e);
+#pragma unroll
+                for (int i = 0; i < 4; i++) v[i] = fmaf(x[i], f[w], v[i]);
+            }
+            if (odd)
+                for (int j = max(k0, L.n0); j < k1; j++) {
+                    if (!sees(a, s, t, j - L.n0)) continue;
+                    const char *src = row_at(vb_, vn, j) + e * E::SIZE;
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const float x = number<E>(src + i * E::SIZE);
+                        if (odd32(x)) v[i] += x;
+                    }
+                }
+            if (a.parts > 1) *(pv_f4 *)(part + rr * a.dim + e) = v;
+            else {
+                char *dst = a.out + s * a.o_seq + t * a.o_row + ((long long)hd * a.dim + e) * E::SIZE;
+                if constexpr (E::SIZE == 2) *(pv_u2 *)dst = (pv_u2){round2<E>(v[0] * inv, v[1] * inv), round2<E>(v[2] * inv, v[3] * inv)};
+                else *(pv_f4 *)dst = (pv_f4){v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv};
+            }
+        }
+        if ((tid & 15) == 0) {
+            if (a.parts > 1) { part[16 * a.dim + rr] = top; part[16 * a.dim + 16 + rr] = sum; }
+            else a.lse[((long long)s * a.G + g) * a.T * a.R + row] = sum == 0.f ? INFINITY : ms + log2f(sum);
+        }
+    }
+}
+
+// a row's parts: 16 lanes a row, 16 rows a work-group
+template <class E>
+__global__ __launch_bounds__(256) void cache_join_kernel(const ca_args a) {
+    int id = blockIdx.x;
+    const int tile = id % a.tiles; id /= a.tiles;
+    const int g = id % a.G, s = id / a.G, rr = threadIdx.x >> 4, row = tile * 16 + rr;
+    const ca_lens L = lens_of(a, s);
+    if (row >= L.cnt * a.R) return;
+    const int chunk = chunk_of(L.len, a.parts), n = (L.len + chunk - 1) / chunk, t = row / a.R, hd = g * a.R + row % a.R;
+    const long long step = 16 * (a.dim + 2);
+    const float *part = a.part + (((long long)s * a.G + g) * a.tiles + tile) * a.parts * step;
+    float top = -INFINITY, sum = 0.f;
+    for (int i = 0; i < n; i++) top = fmaxf(top, part[i * step + 16 * a.dim + rr]);
+    const float ms = top == -INFINITY ? 0.f : top;
+    for (int i = 0; i < n; i++) sum = fmaf(part[i * step + 16 * a.dim + 16 + rr], __builtin_amdgcn_exp2f(part[i * step + 16 * a.dim + rr] - ms), sum);
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    for (int e = (threadIdx.x & 15) * 4; e < a.dim; e += 64) {
+        pv_f4 v = {0.f, 0.f, 0.f, 0.f};
+        for (int i = 0; i < n; i++) {
+            const float f = __builtin_amdgcn_exp2f(part[i * step + 16 * a.dim + rr] - ms);
+            const pv_f4 x = *(const pv_f4 *)(part + i * step + rr * a.dim + e);
+#pragma unroll
+            for (int y = 0; y < 4; y++) v[y] = fmaf(x[y], f, v[y]);
+        }
+        char *dst = a.out + s * a.o_seq + t * a.o_row + ((long long)hd * a.dim + e) * E::SIZE;
+        if constexpr (E::SIZE == 2) *(pv_u2 *)dst = (pv_u2){round2<E>(v[0] * inv, v[1] * inv), round2<E>(v[2] * inv, v[3] * inv)};
+        else *(pv_f4 *)dst = (pv_f4){v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv};
+    }
+    if ((threadIdx.x & 15) == 0) a.lse[((long long)s * a.G + g) * a.T * a.R + row] = sum == 0.f ? INFINITY : ms + log2f(sum);
+}
+
+// 64 keys of a kv head; the waves take the 16-row tiles in turn (SHARE), or 64 keys each where there is one tile or two
+template <class E, int DP, bool SHARE>
+__global__ __launch_bounds__(256) void cache_weight_kernel(const ca_args a) {
+    constexpr int NS = STEPS<E, DP>, KEYS = SHARE ? 64 : 256;
+    __shared__ float red[4][64];
+    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, c = lane & 15, q4 = lane >> 4;
+    const int blocks = (a.n_ctx + KEYS - 1) / KEYS;
+    int id = blockIdx.x;
+    const int b = id % blocks; id /= blocks;
+    const int g = id % a.G, s = id / a.G;
+    const ca_lens L = lens_of(a, s);
+    if (b * KEYS >= L.len) return;
+    const int kb = b * KEYS + (SHARE ? 0 : wave * 64);
+    const float *w_in = a.weight ? a.weight + ((long long)s * a.G + g) * a.n_ctx : nullptr;
+    float *w_out = a.weight_out + ((long long)s * a.G + g) * a.n_ctx;
+    pv_u4 kf[4][NS];
+    float w[4][4] = {};
+    if (kb < L.len) {
+#pragma unroll
+        for (int u = 0; u < 4; u++) get_row<E, DP>(kf[u], a.k + s * a.seq + g * a.head + min(kb + 16 * u + c, L.len - 1) * a.slot, q4, a.dim);
+        const int rows = L.cnt * a.R;
+        const float *lse = a.lse + ((long long)s * a.G + g) * a.T * a.R;
+        for (int tile = SHARE ? wave : 0; tile * 16 < rows; tile += SHARE ? 4 : 1) {
+            const int row = min(tile * 16 + c, rows - 1), t = row / a.R;
+            if (!a.tree && min(tile * 16 + 15, rows - 1) / a.R < kb - L.n0) continue; // all these tokens come before these keys
+            pv_u4 qf[NS];
+            get_row<E, DP>(qf, a.q + s * a.q_seq + t * a.q_row + (long long)(g * a.R + row % a.R) * a.dim * E::SIZE, q4, a.dim);
+            const float ls = tile * 16 + c < rows ? lse[row] : INFINITY;
+#pragma unroll
+            for (int u = 0; u < 4; u++) {
+                const pv_f4 z = dot<E, DP>(kf[u], qf);
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const int j = kb + 16 * u + 4 * q4 + i;
+                    const float p = ls == INFINITY ? 0.f : __builtin_amdgcn_exp2f(fmaf(z[i], a.sc2, -ls));
+                    if (kb + 64 <= L.n0 || (j < L.len && (j < L.n0 || sees(a, s, t, j - L.n0)))) w[u][i] += p;
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < 4; u++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+#pragma unroll
+            for (int x = 1; x < 16; x <<= 1) w[u][i] += __shfl_xor(w[u][i], x, 64);
+            if (c == 0) red[wave][16 * u + 4 * q4 + i] = w[u][i];
+        }
+    __syncthreads();
+    const int j = SHARE ? kb + lane : b * KEYS + tid;
+    if (j >= L.len || (SHARE && wave)) return;
+    const float sum = SHARE ? (red[0][lane] + red[1][lane]) + (red[2][lane] + red[3][lane]) : red[wave][lane];
+    w_out[j] = j < L.n0 && w_in ? w_in[j] + sum : sum;
+}
+
+// an accepted path: a work-group per kv head and sequence, token after token (a row moves down, or stays)
+__global__ __launch_bounds__(256) void cache_take_kernel(char *k, char *v, long long seq, long long slot, long long head, int n_ctx, int row_bytes, const int32_t *n_kv, const int32_t *count, const int32_t *take,
+                                                         int n_take, int32_t *pos, float *weight) {
+    const int g = blockIdx.x, s = blockIdx.y, n0 = min(max(n_kv[s], 0), n_ctx), cnt = min(max(count[s], 0), min(n_take, n_ctx - n0));
+    char *kr = k + s * seq + g * head, *vr = v + s * seq + g * head;
+    const long long at = ((long long)s * gridDim.x + g) * n_ctx;
+    int last = -1;
+    for (int i = 0; i < cnt; i++) {
+        const int t = take[(long long)s * n_take + i];
+        if (t <= last || t >= n_ctx - n0) return;
+        last = t;
+        if (t == i) continue;
+        const int from = n0 + t, to = n0 + i; // to < from: no later row reads `to`
+        for (int x = threadIdx.x * 16; x < 2 * row_bytes; x += 4096) {
+            char *r = x < row_bytes ? kr + x : vr + (x - row_bytes);
+            *(pv_u4 *)(r + to * slot) = *(const pv_u4 *)(r + from * slot);
+        }
+        if (threadIdx.x == 0) {
+            if (pos) pos[at + to] = pos[at + from];
+            if (weight) weight[at + to] = weight[at + from];
+        }
+    }
+}
+__global__ __launch_bounds__(256) void cache_count_kernel(int32_t *n_kv, const int32_t *count, const int32_t *take, int n_take, int n_seqs, int n_ctx) {
+    const int s = blockIdx.x * 256 + threadIdx.x;
+    if (s >= n_seqs) return;
+    const int n0 = min(max(n_kv[s], 0), n_ctx);
+    int cnt = min(max(count[s], 0), n_ctx - n0);
+    if (take) {
+        cnt = min(cnt, n_take);
+        int last = -1, i = 0;
+        for (; i < cnt; i++) {
+            const int t = take[(long long)s * n_take + i];
+            if (t <= last || t >= n_ctx - n0) break;
+            last = t;
+        }
+        cnt = i;
+    }
+    n_kv[s] = n0 + cnt;
+}
+
+template <class E, int DP>
+void launch_attn(const ca_args &a, hipStream_t st) {
+    const long long heads = (long long)a.n_seqs * a.G;
+    // two tiles of rows a wave where there are two: its keys are read once for both
+    if (a.tiles > 1) hipLaunchKernelGGL((cache_attn_kernel<E, DP, 2>), dim3((unsigned)(heads * a.parts * ((a.tiles + 1) / 2))), dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((cache_attn_kernel<E, DP, 1>), dim3((unsigned)(heads * a.parts)), dim3(256), 0, st, a);
+    if (a.parts > 1) hipLaunchKernelGGL((cache_join_kernel<E>), dim3((unsigned)(heads * a.tiles)), dim3(256), 0, st, a);
+    if (!a.weight_out) return;
+    if (a.tiles > 2) hipLaunchKernelGGL((cache_weight_kernel<E, DP, true>), dim3((unsigned)(heads * ((a.n_ctx + 63) / 64))), dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((cache_weight_kernel<E, DP, false>), dim3((unsigned)(heads * ((a.n_ctx + 255) / 256))), dim3(256), 0, st, a);
+}
+} // namespace
+
+size_t psv_attn_space(int n_cu, const ps_kv_cache &c, const ps_cache_attn_params &p, void *base, bool launch, hipStream_t st) {
+    const int R = p.heads / c.kv_heads, size = c.dtype == PS_F32 ? 4 : 2;
+    const long long heads = (long long)c.n_seqs * c.kv_heads, rows = (long long)p.n_new * R;
+    ca_args a{};
+    a.tiles = (int)((rows + 15) / 16);
+    const long long groups = heads * ((a.tiles + 1) / 2);
+    a.parts = (int)std::min<long long>({std::max<long long>((3 * n_cu + groups - 1) / groups, (c.n_ctx + 1023) / 1024), (c.n_ctx + 127) / 128, 64});
+    ps_carve ws{(char *)base};
+    a.lse = ws.take<float>((size_t)(heads * rows));
+    if (a.parts > 1) a.part = ws.take<float>((size_t)(heads * a.tiles * a.parts * 16 * (c.dim + 2)));
+    if (!launch) return ws.at;
+    a.k = (char *)c.k; a.v = (char *)c.v; a.out = (char *)p.out; a.q = (const char *)p.q; a.k_new = (const char *)p.k_new; a.v_new = (const char *)p.v_new;
+    a.seq = c.seq_stride * size; a.slot = c.slot_stride * size; a.head = c.head_stride * size;
+    a.q_seq = p.q_seq_stride * size; a.q_row = p.q_row_stride * size; a.o_seq = p.out_seq_stride * size; a.o_row = p.out_row_stride * size;
+    a.new_seq = p.new_seq_stride * size; a.new_row = p.new_row_stride * size;
+    a.n_seqs = c.n_seqs; a.n_ctx = c.n_ctx; a.G = c.kv_heads; a.dim = c.dim; a.R = R; a.T = p.n_new;
+    a.sc2 = p.scale * 1.44269504088896340736f;
+    a.n_kv = c.n_kv; a.count = p.count; a.pos_new = p.pos_new; a.pos = c.pos; a.tree = p.tree; a.weight = c.weight; a.weight_out = p.weight_out;
+    if (c.dtype == PS_F32) c.dim > 64 ? launch_attn<F32, 128>(a, st) : launch_attn<F32, 64>(a, st);
+    else if (c.dtype == PS_F16) c.dim > 64 ? launch_attn<F16, 128>(a, st) : launch_attn<F16, 64>(a, st);
+    else c.dim > 64 ? launch_attn<BF16, 128>(a, st) : launch_attn<BF16, 64>(a, st);
+    return ws.at;
+}
+
+void psv_advance(hipStream_t st, const ps_kv_cache &c, const int32_t *count, const int32_t *take, int n_take) {
+    const int size = c.dtype == PS_F32 ? 4 : 2;
+    if (take)
+        hipLaunchKernelGGL(cache_take_kernel, dim3((unsigned)c.kv_heads, (unsigned)c.n_seqs), dim3(256), 0, st, (char *)c.k, (char *)c.v, c.seq_stride * size, c.slot_stride * size, c.head_stride * size, c.n_ctx,
+                           c.dim * size, c.n_kv, count, take, n_take, c.pos, c.weight);
+    hipLaunchKernelGGL(cache_count_kernel, dim3((unsigned)((c.n_seqs + 255) / 256)), dim3(256), 0, st, c.n_kv, count, take, n_take, c.n_seqs, c.n_ctx);
+}

@@ -18,7 +18,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("PS_HIP_LIB") or os.path.join(HERE, "lib", "libps_hip.so")  # PS_HIP_LIB: an A/B build (tools/ab_build.py)
 SEQ_LIB_PATH = os.path.join(HERE, "lib", "libps_hip_seq.so")  # the context + the layer-list models only (powerserve_amd/build.py build_seq)
 
-F32, F16, Q4_0, Q8_0, Q4_K, Q5_K, Q6_K, Q8_K, I32 = 0, 1, 2, 8, 12, 13, 14, 15, 26
+F32, F16, Q4_0, Q8_0, Q4_K, Q5_K, Q6_K, Q8_K, I32, BF16 = 0, 1, 2, 8, 12, 13, 14, 15, 26, 30
 DENSE_BF16, DENSE_F32, DENSE_F32_LINES = 0, 1, 2  # enum ps_dense_form
 ATTN_TIMEOUT = 3  # PS_HIP_ATTN_TIMEOUT (include/ps_hip.h)
 QUANT = (Q4_0, Q8_0, Q4_K, Q5_K, Q6_K)
@@ -38,6 +38,8 @@ EXPORTS = [
     "ps_hip_dense_upload", "ps_hip_dense_free", "ps_hip_dense_matmul", "ps_hip_dense_f32_form", "ps_hip_dense_form", "ps_hip_seq_create", "ps_hip_seq_create_sized", "ps_hip_seq_launch_rows", "ps_hip_seq_destroy", "ps_hip_seq_acquire", "ps_hip_seq_release",
     "ps_hip_seq_position", "ps_hip_seq_slot_bytes", "ps_hip_seq_layer_runs", "ps_hip_seq_forward", "ps_hip_seq_decode_greedy", "ps_hip_seq_debug_layers", "ps_hip_seq_set_mode",
     "ps_hip_seq_weight_bytes_per_token", "ps_hip_seq_bench_kernel",
+    "ps_hip_cache_attn_workspace", "ps_hip_cache_attn", "ps_hip_cache_advance", "ps_hip_cache_evict_workspace", "ps_hip_cache_evict", "ps_hip_sample_workspace", "ps_hip_sample",
+    "ps_hip_adapters_create", "ps_hip_adapters_load", "ps_hip_adapters_free", "ps_hip_adapters_workspace", "ps_hip_adapters_apply",
 ]
 # the part of EXPORTS that lib/libps_hip_seq.so has (everything else belongs to the quantized path)
 SEQ_EXPORTS = [n for n in EXPORTS if n.startswith(("ps_hip_dense_", "ps_hip_seq_"))] + [
@@ -119,6 +121,29 @@ class SeqDesc(C.Structure):
                 [("side_embed", C.c_void_p), ("final_norm_bias", C.c_void_p)])
 
 
+class KVCache(C.Structure):
+    """ps_kv_cache (include/ps_hip.h)"""
+    _fields_ = ([(n, C.c_int32) for n in ("dtype", "n_seqs", "n_ctx", "kv_heads", "dim", "_pad")] + [("k", C.c_void_p), ("v", C.c_void_p)] +
+                [(n, C.c_int64) for n in ("seq_stride", "slot_stride", "head_stride")] + [(n, C.c_void_p) for n in ("n_kv", "pos", "weight")])
+
+
+class CacheAttnParams(C.Structure):
+    """ps_cache_attn_params (include/ps_hip.h)"""
+    _fields_ = ([("heads", C.c_int32), ("n_new", C.c_int32), ("scale", C.c_float), ("_pad", C.c_int32)] + [(n, C.c_void_p) for n in ("q", "out", "k_new", "v_new")] +
+                [(n, C.c_int64) for n in ("q_seq_stride", "q_row_stride", "out_seq_stride", "out_row_stride", "new_seq_stride", "new_row_stride")] +
+                [(n, C.c_void_p) for n in ("count", "pos_new", "tree", "weight_out")])
+
+
+class CacheEvictParams(C.Structure):
+    """ps_cache_evict_params (include/ps_hip.h)"""
+    _fields_ = [(n, C.c_int32) for n in ("keep", "recent", "first", "_pad")] + [(n, C.c_void_p) for n in ("weight_out", "pos_out", "n_kv_out")]
+
+
+class SampleParams(C.Structure):
+    """ps_sample_params (include/ps_hip.h)"""
+    _fields_ = [(n, C.c_void_p) for n in ("temperature", "top_k", "top_p", "min_p", "u")]
+
+
 _LIB = None
 
 
@@ -179,6 +204,12 @@ def lib(seq_only_ok: bool = False) -> C.CDLL:
         "ps_hip_seq_slot_bytes": (sz, [vp]), "ps_hip_seq_layer_runs": (i32, [vp]), "ps_hip_seq_forward": (i32, [vp, i32, vp, i32, vp, i32, vp, vp]),
         "ps_hip_seq_decode_greedy": (i32, [vp, i32, i32, i32, vp]), "ps_hip_seq_debug_layers": (i32, [vp, vp]), "ps_hip_seq_set_mode": (i32, [vp, i32]),
         "ps_hip_seq_weight_bytes_per_token": (C.c_uint64, [vp]),
+        "ps_hip_cache_attn_workspace": (sz, [vp, C.POINTER(KVCache), C.POINTER(CacheAttnParams)]), "ps_hip_cache_attn": (i32, [vp, C.POINTER(KVCache), C.POINTER(CacheAttnParams), vp, sz]),
+        "ps_hip_cache_advance": (i32, [vp, C.POINTER(KVCache), vp, vp, i32]),
+        "ps_hip_cache_evict_workspace": (sz, [vp, C.POINTER(KVCache), C.POINTER(CacheEvictParams)]), "ps_hip_cache_evict": (i32, [vp, C.POINTER(KVCache), C.POINTER(CacheEvictParams), vp, sz]),
+        "ps_hip_sample_workspace": (sz, [vp, i64, i64]), "ps_hip_sample": (i32, [vp, i32, vp, i64, i64, i64, C.POINTER(SampleParams), vp, vp, vp, sz]),
+        "ps_hip_adapters_create": (i32, [vp, i64, i64, i32, i32, C.POINTER(vp)]), "ps_hip_adapters_load": (i32, [vp, vp, i32, vp, vp, i32, C.c_float]), "ps_hip_adapters_free": (None, [vp, vp]),
+        "ps_hip_adapters_workspace": (sz, [vp, i32]), "ps_hip_adapters_apply": (i32, [vp, vp, i32, vp, i64, i32, vp, vp, vp, i64, vp, sz]),
         "ps_hip_seq_bench_kernel": (i32, [vp, i32, i32, i32, C.POINTER(C.c_double), C.POINTER(C.c_double), C.POINTER(C.c_double)]),
     }
     for name, (res, args) in sig.items():
@@ -196,6 +227,33 @@ class PSHipError(RuntimeError):
 
 def _ptr(a: np.ndarray):
     return a.ctypes.data_as(C.c_void_p)
+
+
+def _dev(a):
+    """Device address of a DevArray, of anything with a data_ptr(), or as given (None: none)."""
+    if a is None or isinstance(a, int):
+        return a
+    return a.ptr if hasattr(a, "ptr") else a.data_ptr()
+
+
+def kv_cache(dtype: int, k, v, n_kv, n_seqs: int, n_ctx: int, kv_heads: int, dim: int, pos=None, weight=None, strides=None) -> KVCache:
+    """The caches of one attention layer (ps_kv_cache): by default numbers of [n_seqs][n_ctx][kv_heads][dim], or strides = (sequence, slot, head).  The buffers stay the caller's."""
+    s = strides or (n_ctx * kv_heads * dim, kv_heads * dim, dim)
+    return KVCache(dtype, n_seqs, n_ctx, kv_heads, dim, 0, _dev(k), _dev(v), *s, _dev(n_kv), _dev(pos), _dev(weight))
+
+
+def cache_attn_args(q, out, heads: int, n_new: int, scale: float, k_new=None, v_new=None, count=None, pos_new=None, tree=None, weight_out=None, strides=(0, 0, 0, 0, 0, 0)) -> CacheAttnParams:
+    """What Ctx.cache_attn takes beside the caches (ps_cache_attn_params): made once for a step's buffers, passed every step."""
+    return CacheAttnParams(heads, n_new, scale, 0, _dev(q), _dev(out), _dev(k_new), _dev(v_new), *strides, _dev(count), _dev(pos_new), _dev(tree), _dev(weight_out))
+
+
+def cache_evict_args(keep: int, recent: int = 0, first: int = 0, weight_out=None, pos_out=None, n_kv_out=None) -> CacheEvictParams:
+    return CacheEvictParams(keep, recent, first, 0, _dev(weight_out), _dev(pos_out), _dev(n_kv_out))
+
+
+def sample_params(u, temperature=None, top_k=None, top_p=None, min_p=None) -> SampleParams:
+    """Settings of a batch of requests, one number a row each (device arrays; None: off)."""
+    return SampleParams(_dev(temperature), _dev(top_k), _dev(top_p), _dev(min_p), _dev(u))
 
 
 class Ctx:
@@ -258,6 +316,32 @@ class Ctx:
         self.check(self.L.ps_hip_event_elapsed_ms(self.h, a, b, C.byref(ms)))
         return ms.value
 
+    # ---- a serving step of many sequences (include/ps_hip.h; device buffers: addresses, DevArrays, or anything with a data_ptr())
+    def cache_attn_workspace(self, cache: KVCache, args: CacheAttnParams) -> int:
+        return self.L.ps_hip_cache_attn_workspace(self.h, cache, args)
+
+    def cache_attn(self, cache: KVCache, args: CacheAttnParams, space, space_bytes: int):
+        """The newest tokens into the caches and their attention (ps_hip_cache_attn)."""
+        self.check(self.L.ps_hip_cache_attn(self.h, cache, args, _dev(space), space_bytes))
+
+    def cache_advance(self, cache: KVCache, count, take=None, n_take: int = 0):
+        """New tokens, or the accepted path of a tree, become part of the caches (ps_hip_cache_advance)."""
+        self.check(self.L.ps_hip_cache_advance(self.h, cache, _dev(count), _dev(take), n_take))
+
+    def cache_evict_workspace(self, cache: KVCache, args: CacheEvictParams) -> int:
+        return self.L.ps_hip_cache_evict_workspace(self.h, cache, args)
+
+    def cache_evict(self, cache: KVCache, args: CacheEvictParams, space, space_bytes: int):
+        """Down to args.keep slots a sequence by accumulated attention weight (ps_hip_cache_evict)."""
+        self.check(self.L.ps_hip_cache_evict(self.h, cache, args, _dev(space), space_bytes))
+
+    def sample_workspace(self, n: int, rows: int) -> int:
+        return self.L.ps_hip_sample_workspace(self.h, n, rows)
+
+    def sample(self, logits, n: int, rows: int, params: SampleParams, ids, prob=None, dtype: int = F32, stride: int | None = None, space=None, space_bytes: int = 0):
+        """A token per row of logits (ps_hip_sample)."""
+        self.check(self.L.ps_hip_sample(self.h, dtype, _dev(logits), n, rows, n if stride is None else stride, params, _dev(ids), _dev(prob), _dev(space), space_bytes))
+
     # ---- weights
     def upload_weight(self, dtype: int, blocks: np.ndarray, K: int, N: int) -> "Weight":
         blocks = np.ascontiguousarray(blocks)
@@ -313,6 +397,39 @@ class Weight:
     def free(self):
         if self.h:
             self.ctx.L.ps_hip_weight_free(self.ctx.h, self.h)
+            self.h = None
+
+
+class Adapters:
+    """Low-rank adapters of one dense matrix [N, K] (ps_hip_adapters_*): n_slots of them, of up to max_rank."""
+
+    def __init__(self, ctx: Ctx, N: int, K: int, n_slots: int, max_rank: int):
+        self.ctx, self.N, self.K = ctx, N, K
+        self.h = None
+        h = C.c_void_p()
+        ctx.check(ctx.L.ps_hip_adapters_create(ctx.h, N, K, n_slots, max_rank, C.byref(h)))
+        self.h = h
+
+    def load(self, slot: int, down: np.ndarray | None, up: np.ndarray | None, scale: float = 1.0):
+        """down [rank, K], up [N, rank]: bfloat16 bit patterns (16-bit integers); None, None empties the slot."""
+        if down is None and up is None:
+            return self.ctx.check(self.ctx.L.ps_hip_adapters_load(self.ctx.h, self.h, slot, None, None, 0, 0.0))
+        down, up = np.ascontiguousarray(down), np.ascontiguousarray(up)
+        if down.dtype.itemsize != 2 or up.dtype.itemsize != 2 or down.ndim != 2 or up.shape != (self.N, down.shape[0]) or down.shape[1] != self.K:
+            raise PSHipError(f"adapters: down {down.shape} {down.dtype} and up {up.shape} {up.dtype} are not bfloat16 matrices [rank, {self.K}] and [{self.N}, rank]")
+        self.ctx.check(self.ctx.L.ps_hip_adapters_load(self.ctx.h, self.h, slot, _ptr(down), _ptr(up), down.shape[0], scale))
+
+    def workspace(self, T: int) -> int:
+        return self.ctx.L.ps_hip_adapters_workspace(self.h, T)
+
+    def apply(self, x, T: int, ids, out, base=None, dtype: int = F32, ldx: int | None = None, ldo: int | None = None, space=None, space_bytes: int = 0):
+        """out[t] = base[t] + scale * up (down x[t]) with the adapter ids[t] (ps_hip_adapters_apply)."""
+        self.ctx.check(self.ctx.L.ps_hip_adapters_apply(self.ctx.h, self.h, dtype, _dev(x), self.K if ldx is None else ldx, T, _dev(ids), _dev(base), _dev(out), self.N if ldo is None else ldo, _dev(space),
+                                                        space_bytes))
+
+    def close(self):
+        if self.h:
+            self.ctx.L.ps_hip_adapters_free(self.ctx.h, self.h)
             self.h = None
 
 
