@@ -586,8 +586,8 @@ int ps_hip_cache_evict(ps_hip_ctx *ctx, const ps_kv_cache *cache, const ps_cache
  * taken from the largest to the smallest, equal ones by index; NaN and minus infinity are none.  With w = exp((logit - largest) / temperature): the first top_k (<= 0: all); of those the shortest
  * beginning whose w add up to top_p of theirs (>= 1 or NaN: all; at least one); of those the ones with w >= min_p (<= 0 or NaN: all; the largest always stays); then the first whose w, added up to
  * and with it, exceed u times the sum of the ones left (u < 0 or NaN: 0; u >= 1: the last).  A temperature that is not above 0 takes the first candidate.  A row without candidates gives id -1 and
- * probability 0.  Weights are computed in 64 bits and added as whole multiples of 2^-44 or less of the largest one, so that no order of work changes a result; a weight below e^-40 of the
- * largest is 0.  NULL arrays: temperature 1, no filter; u is required. */
+ * probability 0.  A weight is within 2^-27 of itself, and weights are added as whole multiples of 2^-38 (2^-45 for vocabularies of up to 2^17) or less of the largest one, so that no order of work
+ * changes a result; one below e^-40 of the largest is 0.  NULL arrays: temperature 1, no filter; u is required. */
 typedef struct {
     const float *temperature; /* device [rows] each */
     const int32_t *top_k;

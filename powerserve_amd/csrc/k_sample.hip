@@ -1,13 +1,17 @@
 // Sampling (ps_hip_sample): top-k, temperature, top-p, min-p and a draw from a given number, a row of logits each.
 //   Every stage takes a beginning of the candidates in descending order, so that none of them needs the order itself, only places in it: the place where a count (top-k), a sum of weights
-//   (top-p, the draw) or a weight (min-p) is reached.  Candidates are counted and their weights added in bins of equal width of z = (largest - logit) / temperature, 1/32 wide up to z = 40 and
-//   one for the rest (weight 0); a place's bin follows from sums over bins, and only that bin's candidates are collected and sorted.  A bin with more of them than LDS takes
-//   (equal logits, a high temperature) is walked digit by digit of the logit instead.
-//   Weights e^-z are computed in 64 bits -- e^-(bin / 32) from a table times a polynomial of what is left, below 1/32 -- and added as whole multiples of 2^-scale of the largest one: any
-//   order of work gives the same sums, and they are within 2^-44 or so of the true ones, where 32-bit sums would move one draw in some thousands to a neighbour.
-//   sample_top_kernel    the largest logit of a part of a row; clears the bins
-//   sample_bins_kernel   counts and weights of a part, in LDS, added to the row's bins
-//   sample_pick_kernel   the stages; with few parts of a row (many rows) it makes the bins itself
+//   (top-p, the draw) or a weight (min-p) is reached.
+//   First pass: the largest logit of each of 1024 groups of a row.  The k-th largest of those is a bound that at least k candidates reach (any k up to 1024), and few more than that do.
+//   Second pass: the candidates at or above the bound -- the k-th for a count, else the 1014th, some 5000 of a large vocabulary -- go into a list, the head; where no count makes the others
+//   irrelevant, all are counted and their weights added in bins of equal width of z = (largest - logit) / temperature, 1/32 wide up to z = 40 and one for the rest (weight 0).
+//   A place's bin follows from sums over bins, and only that bin's candidates are collected -- from the head in LDS, or, where a place lies behind it, in one more
+//   pass over the row -- and walked digit by digit of (logit, index), with counts and weights of a digit's values, until one is left.  Where they are more than LDS takes (equal logits, a
+//   high temperature) every digit is a pass over the row.
+//   Weights e^-z -- of z in 64 bits, e^-(bin / 32) from a table times a polynomial of what is left, below 1/32 -- are added as whole multiples of 2^-scale of the largest one: any order of
+//   work gives the same sums, and what a weight is off by, 2^-28 of it to either side alike, moves one draw in millions to a neighbour, where 32-bit sums would move one in some thousands.
+//   sample_top_kernel   the first pass over a part of a row
+//   sample_head_kernel  the second pass over a part
+//   sample_pick_kernel  the stages; with few parts of a row (many rows) it makes both passes itself
 #include "ps_serve.h"
 
 #include <algorithm>
@@ -15,50 +19,103 @@
 
 namespace {
 typedef unsigned long long u64;
-constexpr int NB = 1280, LIST = 4096, PICK = 1024; // bins below z = 40; candidates of a sorted list; threads of a pick
+constexpr int NB = 1280, LIST = 2048, HEAD = 8192, PICK = 1024; // bins below z = 40; candidates of a sorted list, of the head; threads of a pick
+constexpr int PART_HEAD = 2048; // of a part
+constexpr int QUANTILE = 1014; // of the 1024 groups' largest logits: the head's bound where no count gives one
 constexpr double WIDTH = 1.0 / 32;
 
 struct smp_args {
     const void *logits;
-    long long n, rows, stride;
+    long long rows, stride;
+    int n; // up to 2^24
     const float *temperature, *top_p, *min_p, *u;
     const int32_t *top_k;
     int32_t *ids;
     float *prob;
     int parts, scale;
-    float *top;    // [row][part]
-    unsigned *cnt; // [row][NB + 1]
-    u64 *sum;      // [row][NB + 1]
+    float *top;     // [row][1024] the groups' largest logits
+    float *bound;   // [row][2] the bound, the largest logit
+    unsigned *cnt;  // [row][part][NB + 1]
+    u64 *sum;       // [row][part][NB + 1]
+    u64 *head;      // [row][part][PART_HEAD]
+    unsigned *held; // [row][part] candidates in it
 };
 struct F16 { typedef _Float16 T; };
 struct BF16 { typedef __bf16 T; };
 struct F32 { typedef float T; };
-template <class E> __device__ __forceinline__ float logit(const typename E::T *row, long long i) { return (float)row[i]; }
-__device__ __forceinline__ bool candidate(float l) { return l > -INFINITY; } // (NaN is none)
-// f(logit, index) for the numbers lo .. hi of a row, 16 bytes at a time where they are aligned
-template <class E, int THREADS, class F>
-__device__ __forceinline__ void each(const typename E::T *row, long long lo, long long hi, F f) {
-    constexpr int PER = 16 / sizeof(typename E::T);
-    const long long mis = ((uintptr_t)(row + lo) & 15) / sizeof(typename E::T), head = min(hi, lo + (mis ? PER - mis : 0)), body = (hi - head) / PER;
-    if ((long long)threadIdx.x < head - lo) f(logit<E>(row, lo + threadIdx.x), lo + threadIdx.x);
-    const pv_u4 *p = (const pv_u4 *)(row + head);
-    auto unpack = [&](const pv_u4 &v, long long i) {
-        typename E::T x[PER];
-        __builtin_memcpy(x, &v, 16);
+template <int N> __device__ __forceinline__ float at(const float (&l)[N], int e) { // of registers
+    float v = l[0];
 #pragma unroll
-        for (int e = 0; e < PER; e++) f((float)x[e], head + i * PER + e);
+    for (int i = 1; i < N; i++) v = e == i ? l[i] : v;
+    return v;
+}
+__device__ __forceinline__ bool candidate(float l) { return l > -INFINITY; } // (NaN is none)
+// f(numbers, index of the first) for the pieces of 16 bytes of the numbers lo .. hi of a row, four loads of a thread in flight.  What lies before the first whole piece and behind the last goes in
+// a piece each, filled up with minus infinity.  ROLLED: one piece after the other in one place of the code -- a part of a row is a few pieces a thread, and what that costs is fetching instructions
+// (a row's second pass over 64 parts: 11 us unrolled, 8 so); a whole row's passes run unrolled.
+template <class E, int THREADS, bool ROLLED, class F>
+__device__ __forceinline__ void each(const typename E::T *row, int lo, int hi, F f) {
+    typedef typename E::T T;
+    constexpr int PER = 16 / sizeof(T);
+    const int mis = (int)(((uintptr_t)(row + lo) & 15) / sizeof(T)), tid = threadIdx.x;
+    const int head = min(hi, lo + (mis ? PER - mis : 0)), body = (hi - head) / PER, tail = head + body * PER;
+    auto give = [&](const T (&x)[PER], int first) {
+        float l[PER];
+#pragma unroll
+        for (int e = 0; e < PER; e++) l[e] = (float)x[e];
+        f(l, first);
     };
-    long long i = threadIdx.x;
-    for (; i + 3 * THREADS < body; i += 4 * THREADS) { // four loads in flight
-        const pv_u4 a = p[i], b = p[i + THREADS], c = p[i + 2 * THREADS], d = p[i + 3 * THREADS];
-        unpack(a, i);
-        unpack(b, i + THREADS);
-        unpack(c, i + 2 * THREADS);
-        unpack(d, i + 3 * THREADS);
+    const pv_u4 *p = (const pv_u4 *)(row + head);
+    auto piece = [&](const pv_u4 &v, int u) {
+        T x[PER];
+        __builtin_memcpy(x, &v, 16);
+        give(x, head + u * PER);
+    };
+    if constexpr (ROLLED) {
+        for (int i = tid; i < body; i += 4 * THREADS) {
+            pv_u4 v[4];
+#pragma unroll
+            for (int j = 0; j < 4; j++) v[j] = p[min(i + j * THREADS, body - 1)];
+#pragma unroll 1
+            for (int u = i; u < body && u < i + 4 * THREADS; u += THREADS) {
+                piece(v[0], u);
+                v[0] = v[1]; v[1] = v[2]; v[2] = v[3];
+            }
+        }
+    } else if (tid < body) { // a piece is worked on with the next three and the one that takes its place on their way
+        pv_u4 v[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) v[j] = p[min(tid + j * THREADS, body - 1)];
+        for (int i = tid; i < body; i += 4 * THREADS) {
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const pv_u4 x = v[j];
+                v[j] = p[min(i + (j + 4) * THREADS, body - 1)];
+                if (j == 0 || i + j * THREADS < body) piece(x, i + j * THREADS);
+            }
+        }
     }
-    for (; i < body; i += THREADS) unpack(p[i], i);
-    const long long tail = head + body * PER;
-    if ((long long)threadIdx.x < hi - tail) f(logit<E>(row, tail + threadIdx.x), tail + threadIdx.x);
+    const int n = tid == 0 ? head - lo : tid == 64 ? hi - tail : 0, first = tid == 0 ? lo : tail;
+    if (n > 0) {
+        T x[PER];
+#pragma unroll
+        for (int e = 0; e < PER; e++) x[e] = e < n ? row[first + e] : (T)-INFINITY;
+        give(x, first);
+    }
+}
+// sums over a wave's lanes up to and with each
+template <int CTRL, int ROWS> __device__ __forceinline__ u64 moved(u64 v) {
+    const unsigned lo = (unsigned)__builtin_amdgcn_update_dpp(0, (int)(unsigned)v, CTRL, ROWS, 15, false), hi = (unsigned)__builtin_amdgcn_update_dpp(0, (int)(unsigned)(v >> 32), CTRL, ROWS, 15, false);
+    return (u64)hi << 32 | lo;
+}
+__device__ __forceinline__ u64 wave_sums(u64 v) {
+    v += moved<0x111, 15>(v); // row_shr: 1, 2, 4, 8
+    v += moved<0x112, 15>(v);
+    v += moved<0x114, 15>(v);
+    v += moved<0x118, 15>(v);
+    v += moved<0x142, 10>(v); // row_bcast: 15 into rows 1 and 3, 31 into rows 2 and 3
+    v += moved<0x143, 12>(v);
+    return v;
 }
 // logits as whole numbers of the same order, and back
 __device__ __forceinline__ unsigned order_of(float l) {
@@ -68,347 +125,412 @@ __device__ __forceinline__ unsigned order_of(float l) {
 __device__ __forceinline__ float from_order(unsigned o) { return __uint_as_float((o & 0x80000000u) ? o & 0x7fffffffu : ~o); }
 
 struct row_of { // what a row's weights go by
-    double top, inv; // largest logit, 1 / temperature
+    double top, inv; // largest logit, 32 / temperature
     int k;           // candidates at most (0: all)
-    int scale;       // weights are multiples of 2^-scale
 };
 __device__ __forceinline__ row_of row_settings(const smp_args &a, long long r, float top) {
     row_of w;
     const float t = a.temperature ? a.temperature[r] : 1.f;
     w.top = top;
     w.k = a.top_k ? max(a.top_k[r], 0) : 0;
-    w.inv = 1.0;
-    if (t > 0.f) w.inv = 1.0 / (double)t;
+    w.inv = 1 / WIDTH;
+    if (t > 0.f) w.inv = 1 / WIDTH / (double)t;
     else w.k = 1; // the first candidate
-    w.scale = a.scale;
     return w;
 }
+// z in widths of a bin
 __device__ __forceinline__ double z_of(const row_of &w, float l) { return (double)l == w.top ? 0.0 : (w.top - (double)l) * w.inv; }
-__device__ __forceinline__ int bin_of(double z) { return z < NB * WIDTH ? (int)(z * (1 / WIDTH)) : NB; } // (NaN: the rest)
-__device__ __forceinline__ double weight_of(double z, int bin, const double *table) { // bin < NB
-    const double f = bin * WIDTH - z; // -1/32 .. 0
-    double e = 1.0 / 40320;
-    e = fma(e, f, 1.0 / 5040);
-    e = fma(e, f, 1.0 / 720);
-    e = fma(e, f, 1.0 / 120);
-    e = fma(e, f, 1.0 / 24);
-    e = fma(e, f, 1.0 / 6);
-    e = fma(e, f, 0.5);
-    e = fma(e, f, 1.0);
-    e = fma(e, f, 1.0);
-    return table[bin] * e;
+__device__ __forceinline__ int bin_of(double z) { return z < (double)NB ? (int)z : NB; } // (NaN: the rest)
+// The weight as a multiple of 2^-scale (the table holds them so), bin < NB: e^-(bin / 32) in 64 bits times e^-f, f < 1/32, whose difference from 1 is a polynomial in 32 bits: 2^-28 of the weight
+// off, to either side alike.  Half the instructions of a polynomial in 64 bits, in the loop over a whole vocabulary; wherever a weight is asked for it is this one.
+__device__ __forceinline__ u64 weight_of(double z, int bin, const double *table) {
+    const float f = (float)(z - (double)bin) * -(float)WIDTH; // -1/32 .. 0
+    float e = 1.f / 120;
+    e = fmaf(e, f, 1.f / 24);
+    e = fmaf(e, f, 1.f / 6);
+    e = fmaf(e, f, 0.5f);
+    e = fmaf(e, f, 1.f) * f;
+    const double w = fma(table[bin], (double)e, table[bin]);
+    return __double_as_longlong(w + 4503599627370496.0) & 0xfffffffffffffull; // 2^52 + w: w rounded to a whole number, below 2^52
 }
-__device__ __forceinline__ u64 whole(double w, int scale) { return (u64)__double2ull_rn(ldexp(w, scale)); }
-__device__ __forceinline__ void make_table(double *table, int threads) {
-    for (int b = threadIdx.x; b < NB; b += threads) table[b] = exp(-b * WIDTH);
-}
-template <int THREADS> __device__ __forceinline__ float block_max(float v, float *sh) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
-    if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = v;
+// e^-(b / 32) 2^scale, as a product of two of 72 numbers (sh: 72; barriers inside)
+__device__ __forceinline__ void make_table(double *table, double *sh, int threads, int scale) {
+    const int t = threadIdx.x;
+    if (t < 72) sh[t] = t < 40 ? ldexp(exp(-(double)t), scale) : exp(-(t - 40) * WIDTH);
     __syncthreads();
-    v = sh[0];
-    for (int i = 1; i < THREADS / 64; i++) v = fmaxf(v, sh[i]);
+    for (int b = t; b < NB; b += threads) table[b] = sh[b >> 5] * sh[40 + (b & 31)];
     __syncthreads();
-    return v;
 }
-__device__ __forceinline__ void part_of(const smp_args &a, int part, long long &lo, long long &hi) {
-    const long long per = ((a.n + a.parts - 1) / a.parts + 63) / 64 * 64;
+__device__ __forceinline__ void part_of(const smp_args &a, int part, int &lo, int &hi) {
+    const int per = ((a.n + a.parts - 1) / a.parts + 63) / 64 * 64;
     lo = min(a.n, part * per);
     hi = min(a.n, lo + per);
 }
 
-template <class E>
-__global__ __launch_bounds__(256) void sample_top_kernel(const smp_args a) {
-    __shared__ float sh[4];
-    const long long r = blockIdx.y;
-    const typename E::T *row = (const typename E::T *)a.logits + r * a.stride;
-    for (int b = blockIdx.x * 256 + threadIdx.x; b <= NB; b += 256 * a.parts) { a.cnt[r * (NB + 1) + b] = 0; a.sum[r * (NB + 1) + b] = 0; }
-    long long lo, hi;
-    part_of(a, blockIdx.x, lo, hi);
-    float m = -INFINITY;
-    each<E, 256>(row, lo, hi, [&](float l, long long) { m = fmaxf(m, l); });
-    m = block_max<256>(m, sh);
-    if (threadIdx.x == 0) a.top[r * a.parts + blockIdx.x] = m;
+// What a row's passes go by.  tail: the candidates below the bound count too; counts: so does their number
+struct passes {
+    float bound;
+    bool tail, counts;
+};
+__device__ __forceinline__ u64 entry(float l, int i) { return (u64)~order_of(l) << 32 | (unsigned)i; } // ascending: from the largest on, equal ones by index
+__device__ __forceinline__ passes passes_of(int k, float bound) { return passes{bound, k < 1 || k > QUANTILE, k > 0}; }
+struct digit_lds { // 256 values of a digit: candidates and weights, and where a count or a sum is reached
+    unsigned cnt[256];
+    u64 sum[256];
+    u64 out[4];
+};
+// The digit at which a count (by_weight: a sum) reaches goal, which c and x, what lies before, are raised to; one wave.  Lane l has digits 4 l .. 4 l + 3.
+__device__ __forceinline__ void find_digit(digit_lds &d, bool by_weight, u64 goal, u64 c, u64 x) {
+    const int lane = threadIdx.x & 63;
+    u64 cs[4], ss[4], ct = 0, st = 0;
+#pragma unroll
+    for (int e = 0; e < 4; e++) { cs[e] = d.cnt[4 * lane + e]; ss[e] = d.sum[4 * lane + e]; ct += cs[e]; st += ss[e]; }
+    c += wave_sums(ct) - ct;
+    x += wave_sums(st) - st;
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+        const u64 before = by_weight ? x : c, with = before + (by_weight ? ss[e] : cs[e]);
+        if (before < goal && with >= goal) { d.out[0] = (u64)(4 * lane + e); d.out[1] = c; d.out[2] = x; d.out[3] = cs[e]; }
+        c += cs[e];
+        x += ss[e];
+    }
 }
-__device__ __forceinline__ void add_to_bins(const row_of &w, float l, unsigned *cnt, u64 *sum, const double *table) {
-    if (!candidate(l)) return;
+// The bound of a row from its groups' largest logits, a thread each; top: the largest of all.  From the first bit on in which they differ 16 bits, digit by digit; what differs behind them lets a
+// few more into the head.
+__device__ __forceinline__ void row_bound(const smp_args &a, long long r, float mine, digit_lds &d, float &top, passes &ps) {
+    const unsigned o = ~order_of(mine); // ascending: from the largest on
+    unsigned lo = o, hi = o;
+#pragma unroll
+    for (int x = 32; x > 0; x >>= 1) { lo = min(lo, (unsigned)__shfl_xor((int)lo, x, 64)); hi = max(hi, (unsigned)__shfl_xor((int)hi, x, 64)); }
+    if (threadIdx.x < 256) { d.cnt[threadIdx.x] = 0; d.sum[threadIdx.x] = 0; }
+    if (threadIdx.x == 0) { d.out[0] = ~0ull; d.out[1] = 0; }
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) { atomicMin(&d.out[0], (u64)lo); atomicMax(&d.out[1], (u64)hi); }
+    __syncthreads();
+    lo = (unsigned)d.out[0];
+    hi = (unsigned)d.out[1];
+    top = from_order(~lo);
+    const int k = row_settings(a, r, top).k, first = 31 - __clz(lo ^ hi); // (-1: all are equal)
+    ps = passes_of(k, 0.f);
+    const u64 goal = (u64)(ps.tail ? QUANTILE : k);
+    unsigned mask = first >= 31 ? 0 : ~0u << (first + 1), found = lo & mask;
+    u64 before = 0;
+    int shift = max(0, first - 7);
+#pragma unroll 1
+    for (int i = 0; i < 2; i++) {
+        __syncthreads();
+        if ((o & mask) == found) atomicAdd(&d.cnt[o >> shift & 255], 1u);
+        __syncthreads();
+        if (threadIdx.x < 64) find_digit(d, false, goal, before, 0);
+        __syncthreads();
+        mask |= 255u << shift;
+        found = (found & ~(255u << shift)) | (unsigned)d.out[0] << shift;
+        before = d.out[1];
+        if (threadIdx.x < 256) d.cnt[threadIdx.x] = 0;
+        if (shift == 0) break;
+        shift = max(0, shift - 8);
+    }
+    ps.bound = from_order(~min(found | ~mask, ~order_of(-INFINITY)));
+    __syncthreads();
+}
+__device__ __forceinline__ void add_to_bins(const row_of &w, float l, unsigned *cnt, u64 *sum, const double *table, bool counts) {
     const double z = z_of(w, l);
     const int b = bin_of(z);
-    atomicAdd(&cnt[b], 1u);
-    if (b < NB) atomicAdd(&sum[b], whole(weight_of(z, b, table), w.scale));
+    if (counts && candidate(l)) atomicAdd(&cnt[b], 1u);
+    if (b < NB) atomicAdd(&sum[b], weight_of(z, b, table));
 }
-__device__ __forceinline__ float row_top(const smp_args &a, long long r) {
+
+template <class E>
+__global__ __launch_bounds__(256) void sample_top_kernel(const smp_args a) {
+    const long long r = blockIdx.y;
+    const typename E::T *row = (const typename E::T *)a.logits + r * a.stride;
+    int lo, hi;
+    part_of(a, blockIdx.x, lo, hi);
     float m = -INFINITY;
-    for (int i = 0; i < a.parts; i++) m = fmaxf(m, a.top[r * a.parts + i]);
-    return m;
+    each<E, 256, false>(row, lo, hi, [&](const auto &l, int) {
+#pragma unroll
+        for (float x : l) m = fmaxf(m, x);
+    });
+    // 1024 groups a row: of parts / 4 lanes each
+    const int lanes = a.parts / 4;
+    for (int o = 1; o < lanes; o <<= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+    if (threadIdx.x % lanes == 0) a.top[r * 1024 + blockIdx.x * (256 / lanes) + threadIdx.x / lanes] = m;
+}
+// the second pass over lo .. hi: at or above the bound into the head (room for `most`; n counts on); where the others count, all into the bins
+template <class E, bool ROLLED>
+__device__ __forceinline__ void second_pass(const typename E::T *row, int lo, int hi, const row_of &w, const passes &ps, u64 *head, int *n, int most, unsigned *cnt, u64 *sum, const double *table) {
+    each<E, PICK, ROLLED>(row, lo, hi, [&](const auto &l, int first) {
+        constexpr int PER = sizeof(l) / 4;
+        float m = l[0];
+#pragma unroll
+        for (int e = 1; e < PER; e++) m = fmaxf(m, l[e]);
+        if (m >= ps.bound && candidate(m)) {
+            unsigned high = 0;
+#pragma unroll
+            for (int e = 0; e < PER; e++) high |= (l[e] >= ps.bound && candidate(l[e]) ? 1u : 0u) << e;
+            int k = atomicAdd(n, __popc(high));
+            while (high) {
+                const int e = __ffs(high) - 1;
+                high &= high - 1;
+                if (k < most) head[k] = entry(at(l, e), first + e);
+                k++;
+            }
+        }
+        if (ps.tail)
+#pragma unroll
+            for (int e = 0; e < PER; e++) add_to_bins(w, l[e], cnt, sum, table, ps.counts);
+    });
 }
 template <class E>
-__global__ __launch_bounds__(256) void sample_bins_kernel(const smp_args a) {
+__global__ __launch_bounds__(PICK) void sample_head_kernel(const smp_args a) {
     __shared__ unsigned cnt[NB + 1];
     __shared__ u64 sum[NB + 1];
     __shared__ double table[NB];
+    __shared__ u64 list[PART_HEAD];
+    __shared__ int n_list;
     const long long r = blockIdx.y;
     const typename E::T *row = (const typename E::T *)a.logits + r * a.stride;
-    for (int b = threadIdx.x; b <= NB; b += 256) { cnt[b] = 0; sum[b] = 0; }
-    make_table(table, 256);
-    const row_of w = row_settings(a, r, row_top(a, r));
+    float top;
+    passes ps;
+    row_bound(a, r, a.top[r * 1024 + threadIdx.x], *(digit_lds *)list, top, ps);
     __syncthreads();
-    long long lo, hi;
+    const row_of w = row_settings(a, r, top);
+    if (ps.tail) {
+        for (int b = threadIdx.x; b <= NB; b += PICK) { cnt[b] = 0; sum[b] = 0; }
+        make_table(table, (double *)list, PICK, a.scale);
+    }
+    if (threadIdx.x == 0) n_list = 0;
+    __syncthreads();
+    int lo, hi;
     part_of(a, blockIdx.x, lo, hi);
-    each<E, 256>(row, lo, hi, [&](float l, long long) { add_to_bins(w, l, cnt, sum, table); });
+    second_pass<E, true>(row, lo, hi, w, ps, list, &n_list, PART_HEAD, cnt, sum, table);
     __syncthreads();
-    for (int b = threadIdx.x; b <= NB; b += 256)
-        if (cnt[b]) { atomicAdd(&a.cnt[r * (NB + 1) + b], cnt[b]); if (sum[b]) atomicAdd(&a.sum[r * (NB + 1) + b], sum[b]); }
+    // side by side with the other parts': sums between work-groups of different XCDs would be atomics at the memory (33 rows of 16 parts: 35 us of 47)
+    const long long part = r * a.parts + blockIdx.x;
+    if (threadIdx.x == 0) {
+        a.held[part] = (unsigned)n_list;
+        if (blockIdx.x == 0) { a.bound[2 * r] = ps.bound; a.bound[2 * r + 1] = top; }
+    }
+    if (ps.tail)
+        for (int b = threadIdx.x; b <= NB; b += PICK) {
+            if (ps.counts) a.cnt[part * (NB + 1) + b] = cnt[b];
+            a.sum[part * (NB + 1) + b] = sum[b];
+        }
+    for (int i = threadIdx.x; i < min(n_list, PART_HEAD); i += PICK) a.head[part * PART_HEAD + i] = list[i];
 }
 
-// What a pick holds.  cx / wx: candidates and weights before a bin.  The list: candidates of the bins la .. lb - 1 in order, lw the weights up to and with each.
+// What a pick holds.  cx / wx: candidates and weights before a bin.  The list: the candidates of a bin (where they fit).
 struct pick_lds {
     unsigned cx[NB + 2];
     u64 wx[NB + 2];
     double table[NB];
-    u64 list[LIST], lw[LIST];
-    u64 sh[32];
-    float shf[32];
-    unsigned dcnt[256];
-    u64 dsum[256];
-    int n_list, la, lb;
-    u64 out[4];
+    u64 head[HEAD];
+    union {
+        u64 list[LIST];
+        struct {
+            u64 sum[NB + 1]; // (while the bins are made)
+            unsigned cnt[NB + 1];
+        } bins;
+    };
+    digit_lds d;
+    int n_head, n[4], place[4]; // a stage each
+    u64 both[2], sh[16], few[64];
+    int n_few;
 };
-__device__ __forceinline__ u64 scan64(u64 v, u64 *sh, u64 *total) { // sum over the threads before this one
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    u64 x = v;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const u64 y = __shfl_up(x, o, 64);
-        if (lane >= o) x += y;
-    }
-    if (lane == 63) sh[wave] = x;
-    __syncthreads();
-    u64 before = 0, all = 0;
-    for (int i = 0; i < PICK / 64; i++) { if (i < wave) before += sh[i]; all += sh[i]; }
-    __syncthreads();
-    *total = all;
-    return before + x - v;
-}
 template <class E>
 struct picker {
     const smp_args &a;
     const typename E::T *row;
     row_of w;
     pick_lds &s;
+    int in_head; // the bins before this one are in the head whole
+    int bin = -1, n_list = 0; // what was collected last
 
-    __device__ __forceinline__ u64 weight(unsigned order) const {
-        const double z = z_of(w, from_order(order));
+    __device__ __forceinline__ u64 weight(u64 v) const { // of an entry
+        const double z = z_of(w, from_order(~(unsigned)(v >> 32)));
         const int b = bin_of(z);
-        return b < NB ? whole(weight_of(z, b, s.table), w.scale) : 0;
+        return b < NB ? weight_of(z, b, s.table) : 0;
     }
-    // the candidates of bin b in a list, or false where they are too many for one; from the first bin on where they all fit
-    __device__ bool collect(int b) {
-        if (s.la <= b && b < s.lb) return true;
-        const int la = s.cx[b + 1] <= LIST ? 0 : b, lb = b + 1, n = (int)(s.cx[lb] - s.cx[la]);
-        if (n > LIST) return false;
-        __syncthreads();
-        if (threadIdx.x == 0) { s.n_list = 0; s.la = la; s.lb = lb; }
-        __syncthreads();
-        // a bin's logits lie between two of its neighbours' -- the exact bin decides
-        each<E, PICK>(row, 0, a.n, [&](float l, long long i) {
-            if (!candidate(l)) return;
-            const int x = bin_of(z_of(w, l));
-            if (x >= la && x < lb) s.list[atomicAdd(&s.n_list, 1)] = (u64)~order_of(l) << 32 | (unsigned)i;
-        });
-        __syncthreads();
-        int P = 1;
-        while (P < n) P <<= 1;
-        for (int i = n + threadIdx.x; i < P; i += PICK) s.list[i] = ~0ull;
-        __syncthreads();
-        for (int k = 2; k <= P; k <<= 1)
-            for (int j = k >> 1; j > 0; j >>= 1) {
-                for (int i = threadIdx.x; i < P / 2; i += PICK) {
-                    const int x = (i & ~(j - 1)) * 2 + (i & (j - 1)), y = x + j;
-                    const u64 p = s.list[x], q = s.list[y];
-                    if ((p > q) == ((x & k) == 0)) { s.list[x] = q; s.list[y] = p; }
-                }
-                __syncthreads();
+    // the logits of bin b lie between these two, a little widened: most others are passed by without arithmetic in 64 bits
+    __device__ __forceinline__ void range_of(int b, float &lo, float &hi) const {
+        const double zl = b / w.inv, zh = (b + 1) / w.inv, size = fabs(w.top);
+        const bool known = size < INFINITY;
+        hi = known && zl < 1e30 ? (float)(w.top - zl + 1e-5 * (size + zl)) : INFINITY;
+        lo = known && zh < 1e30 && b < NB ? (float)(w.top - zh - 1e-5 * (size + zh)) : -INFINITY;
+    }
+    // f(entry, weight) for the candidates of bin b in the row
+    template <class F> __device__ __forceinline__ void each_of_bin(int b, F f) {
+        float lo, hi;
+        range_of(b, lo, hi);
+        each<E, PICK, false>(row, 0, a.n, [&](const auto &l, int first) {
+            unsigned some = 0;
+#pragma unroll
+            for (int e = 0; e < (int)(sizeof(l) / 4); e++) some |= (l[e] >= lo && l[e] <= hi ? 1u : 0u) << e;
+            while (some) {
+                const int e = __ffs(some) - 1;
+                some &= some - 1;
+                const float v = at(l, e);
+                const double z = z_of(w, v);
+                if (bin_of(z) == b && candidate(v)) f(entry(v, first + e), b < NB ? weight_of(z, b, s.table) : (u64)0);
             }
-        // weights up to and with each: a thread has four in a row
-        u64 v[LIST / PICK], own = 0, all;
-#pragma unroll
-        for (int e = 0; e < LIST / PICK; e++) {
-            const int i = threadIdx.x * (LIST / PICK) + e;
-            v[e] = i < n ? weight(~(unsigned)(s.list[i] >> 32)) : 0;
-            own += v[e];
-        }
-        u64 before = scan64(own, s.sh, &all);
-#pragma unroll
-        for (int e = 0; e < LIST / PICK; e++) {
-            const int i = threadIdx.x * (LIST / PICK) + e;
-            before += v[e];
-            if (i < n) s.lw[i] = before;
-        }
-        __syncthreads();
-        return true;
+        });
     }
-    // A bin that is too large for a list: the candidate at which a count (by_weight: a sum of weights) within the bin is reached, digit by digit.  -> its order, the candidates and weights before
-    // those that are equal to it, and how many equal ones up to it
-    __device__ void descend(int b, bool by_weight, u64 goal, unsigned &order, u64 &c_before, u64 &w_before, u64 &nth) {
-        unsigned found = 0, mask = 0;
-        c_before = w_before = 0;
-        for (int shift = 24; shift >= 0; shift -= 8) {
-            for (int i = threadIdx.x; i < 256; i += PICK) { s.dcnt[i] = 0; s.dsum[i] = 0; }
-            __syncthreads();
-            each<E, PICK>(row, 0, a.n, [&](float l, long long) {
-                if (!candidate(l)) return;
-                const double z = z_of(w, l);
-                const unsigned o = ~order_of(l); // ascending: from the largest on
-                if (bin_of(z) != b || (o & mask) != found) return;
-                atomicAdd(&s.dcnt[o >> shift & 255], 1u);
-                if (b < NB) atomicAdd(&s.dsum[o >> shift & 255], whole(weight_of(z, b, s.table), w.scale));
+    // the candidates of bin b into the list; false where they are too many.  (The stages that ask count in places of their own, so that none waits to clear one.)
+    __device__ __forceinline__ bool collect(int b, int stage) {
+        if (bin == b) return n_list <= LIST;
+        bin = b;
+        auto put = [&](u64 v, u64) {
+            const int k = atomicAdd(&s.n[stage], 1);
+            if (k < LIST) s.list[k] = v;
+        };
+        if (b < in_head) {
+            for (int i = threadIdx.x; i < s.n_head; i += PICK) {
+                const u64 v = s.head[i];
+                if (bin_of(z_of(w, from_order(~(unsigned)(v >> 32)))) == b) put(v, 0);
+            }
+        } else each_of_bin(b, put);
+        __syncthreads();
+        n_list = s.n[stage];
+        return n_list <= LIST;
+    }
+    // f(entry, weight) for the candidates of the bin that was collected last
+    template <class F> __device__ __forceinline__ void each_collected(bool listed, F f) {
+        if (listed) {
+            for (int i = threadIdx.x; i < n_list; i += PICK) f(s.list[i], weight(s.list[i]));
+        } else each_of_bin(bin, f);
+    }
+    // The candidate of bin b at which a count (by_weight: a sum of weights) within the bin reaches goal >= 1, digit by digit of its entry -> its entry, its place within the bin, the weights up to it
+    __device__ __forceinline__ void select(bool listed, bool by_weight, u64 goal, u64 &found, u64 &place, u64 &sum) {
+        place = sum = 0;
+        if (listed && n_list <= 64) return of_few(s.list, n_list, by_weight, goal, found, place, sum);
+        // from the first bit on in which logits of the bin can differ
+        float lo, hi;
+        range_of(bin, lo, hi);
+        const unsigned from = ~order_of(hi), to = ~order_of(lo);
+        const int bits = 64 - __clz(from ^ to); // (32: index alone)
+        u64 mask = bits >= 64 ? 0 : ~0ull << bits;
+        found = (u64)from << 32 & mask;
+        int shift = bits - 8;
+        if (threadIdx.x < 256) { s.d.cnt[threadIdx.x] = 0; s.d.sum[threadIdx.x] = 0; }
+        __syncthreads();
+#pragma unroll 1
+        for (;; shift = max(0, shift - 8)) {
+            each_collected(listed, [&](u64 v, u64 x) {
+                if ((v & mask) != found) return;
+                const int k = (int)(v >> shift & 255);
+                atomicAdd(&s.d.cnt[k], 1u);
+                atomicAdd(&s.d.sum[k], x);
             });
             __syncthreads();
-            if (threadIdx.x == 0) {
-                u64 c = c_before, x = w_before;
-                int d = 0;
-                for (; d < 255; d++) {
-                    if ((by_weight ? x + s.dsum[d] : c + s.dcnt[d]) >= goal) break;
-                    c += s.dcnt[d];
-                    x += s.dsum[d];
-                }
-                s.out[0] = d; s.out[1] = c; s.out[2] = x;
-            }
+            if (threadIdx.x < 64) find_digit(s.d, by_weight, goal, place, sum);
             __syncthreads();
-            found |= (unsigned)s.out[0] << shift;
-            mask |= 255u << shift;
-            c_before = s.out[1];
-            w_before = s.out[2];
+            // (the lowest digits may overlap the ones before them: those bits are the same in all that are left)
+            mask |= 255ull << shift;
+            found = (found & ~(255ull << shift)) | s.d.out[0] << shift;
+            place = s.d.out[1];
+            sum = s.d.out[2];
+            const u64 left = s.d.out[3];
+            __syncthreads();
+            if (threadIdx.x < 256) { s.d.cnt[threadIdx.x] = 0; s.d.sum[threadIdx.x] = 0; }
+            if (left <= 64) break; // (the last digit leaves one)
             __syncthreads();
         }
-        order = ~found;
-        const u64 each_w = weight(order);
-        nth = by_weight ? (each_w ? (goal - w_before + each_w - 1) / each_w : 1) : goal - c_before;
-        if (nth < 1) nth = 1;
-    }
-    // weights of the first c candidates of bin b
-    __device__ u64 weight_of_first(int b, u64 c) {
-        if (c == 0) return 0;
-        if (c == s.cx[b + 1] - s.cx[b]) return s.wx[b + 1] - s.wx[b];
-        if (collect(b)) return s.lw[s.cx[b] - s.cx[s.la] + c - 1] - (s.wx[b] - s.wx[s.la]);
-        unsigned o;
-        u64 cb, wb, nth;
-        descend(b, false, c, o, cb, wb, nth);
-        return wb + nth * weight(o);
-    }
-    // the first place of bin b whose weights, added up to and with it, reach goal >= 1 -> how many that are
-    __device__ u64 place_of(int b, u64 goal) {
-        if (collect(b)) {
-            const u64 off = s.wx[b] - s.wx[s.la];
-            int lo = (int)(s.cx[b] - s.cx[s.la]), hi = (int)(s.cx[b + 1] - s.cx[s.la]) - 1;
-            const int first = lo;
-            while (lo < hi) {
-                const int m = (lo + hi) / 2;
-                if (s.lw[m] - off >= goal) hi = m;
-                else lo = m + 1;
-            }
-            return lo - first + 1;
-        }
-        unsigned o;
-        u64 cb, wb, nth;
-        descend(b, true, goal, o, cb, wb, nth);
-        return cb + nth;
-    }
-    // candidates of bin b with a weight of at least `least`
-    __device__ u64 at_least(int b, double least) {
-        u64 mine = 0, all;
-        each<E, PICK>(row, 0, a.n, [&](float l, long long) {
-            if (!candidate(l)) return;
-            const double z = z_of(w, l);
-            if (bin_of(z) == b && weight_of(z, b, s.table) >= least) mine++;
+        each_collected(listed, [&](u64 v, u64) {
+            if ((v & mask) == found) s.few[atomicAdd(&s.n_few, 1)] = v;
         });
-        scan64(mine, s.sh, &all);
-        return all;
+        __syncthreads();
+        const u64 c = place, x = sum;
+        of_few(s.few, s.n_few, by_weight, goal - (by_weight ? x : c), found, place, sum);
+        place += c;
+        sum += x;
     }
-    // the c-th candidate of bin b: its index, and its weight
-    __device__ int candidate_at(int b, u64 c, u64 &wt) {
-        if (collect(b)) {
-            const u64 x = s.list[s.cx[b] - s.cx[s.la] + c - 1];
-            wt = weight(~(unsigned)(x >> 32));
-            return (int)(unsigned)x;
-        }
-        unsigned o;
-        u64 cb, wb, nth;
-        descend(b, false, c, o, cb, wb, nth);
-        wt = weight(o);
-        // the nth of the equal ones by index: a thread looks through a stretch of the row
-        const long long per = (a.n + PICK - 1) / PICK, lo = min(a.n, threadIdx.x * per), hi = min(a.n, lo + per);
-        u64 mine = 0, all;
-        auto equal = [&](long long i) { const float l = logit<E>(row, i); return candidate(l) && order_of(l) == o; };
-        for (long long i = lo; i < hi; i++) mine += equal(i);
-        const u64 before = scan64(mine, s.sh, &all);
-        if (before < nth && nth <= before + mine) {
-            u64 k = before;
-            for (long long i = lo; i < hi; i++)
-                if (equal(i) && ++k == nth) { s.out[0] = (u64)i; break; }
+    // the same among at most 64 entries: a wave, each lane against all
+    __device__ __forceinline__ void of_few(const u64 *few, int n, bool by_weight, u64 goal, u64 &found, u64 &place, u64 &sum) {
+        if (threadIdx.x < 64) {
+            const u64 v = (int)threadIdx.x < n ? few[threadIdx.x] : ~0ull, x = (int)threadIdx.x < n ? weight(v) : 0; // (no index is that large)
+            u64 c = 0, upto = 0;
+#pragma unroll 4
+            for (int i = 0; i < n; i++) {
+                const u64 o = (u64)(unsigned)__builtin_amdgcn_readlane((int)(v >> 32), i) << 32 | (unsigned)__builtin_amdgcn_readlane((int)v, i);
+                const u64 y = (u64)(unsigned)__builtin_amdgcn_readlane((int)(x >> 32), i) << 32 | (unsigned)__builtin_amdgcn_readlane((int)x, i);
+                if (o <= v) { c++; upto += y; }
+            }
+            if (v != ~0ull && (by_weight ? upto - x < goal && upto >= goal : c == goal)) { s.d.out[0] = v; s.d.out[1] = c; s.d.out[2] = upto; }
         }
         __syncthreads();
-        const int id = (int)s.out[0];
+        found = s.d.out[0];
+        place = s.d.out[1];
+        sum = s.d.out[2];
+        if (threadIdx.x == 0) s.n_few = 0;
         __syncthreads();
-        return id;
     }
-    // the first bin behind whose end a count or a sum has reached goal (goal <= the whole)
-    template <class X> __device__ __forceinline__ int bin_reaching(const X *before, u64 goal) const {
-        int lo = 0, hi = NB;
-        while (lo < hi) {
-            const int m = (lo + hi) / 2;
-            if (before[m + 1] >= goal) hi = m;
-            else lo = m + 1;
-        }
-        return lo;
+    // the bin in which sums before each of them (and behind the last) reach goal >= 1
+    template <class X> __device__ __forceinline__ int reaching(const X *before, u64 goal, int stage) {
+        for (int i = threadIdx.x; i < NB; i += PICK)
+            if (before[i] < goal && before[i + 1] >= goal) s.place[stage] = i;
+        __syncthreads();
+        return s.place[stage];
     }
-    __device__ void pick(long long r) {
-        if (s.cx[NB + 1] == 0) { // no candidate
-            if (threadIdx.x == 0) { a.ids[r] = -1; if (a.prob) a.prob[r] = 0.f; }
-            return;
-        }
-        int bl = NB; // what stays: the bins before bl and the first cl of bin bl (the last bin's weights are 0)
-        u64 cl = 0;
-        if (w.k > 0 && (unsigned)w.k < s.cx[NB]) {
-            bl = bin_reaching(s.cx, (u64)w.k);
-            cl = (u64)w.k - s.cx[bl];
-        }
-        u64 total = s.wx[bl] + weight_of_first(bl, cl);
-        const float p = a.top_p ? a.top_p[r] : 1.f, m = a.min_p ? a.min_p[r] : 0.f;
-        int bp = bl;
-        u64 cp = cl;
-        if (p < 1.f) {
-            const double goal = ceil((double)fmaxf(p, 0.f) * (double)total);
-            const u64 g = max((u64)1, min(total, (u64)goal));
-            bp = min(bl, bin_reaching(s.wx, g));
-            cp = place_of(bp, g - s.wx[bp]);
-        }
-        if (m > 0.f) {
-            const double least = fmin((double)m, 1.0);
-            int lo = 0, hi = NB - 1; // the last bin whose largest weight is `least` or more
-            while (lo < hi) {
-                const int x = (lo + hi + 1) / 2;
-                if (s.table[x] >= least) lo = x;
-                else hi = x - 1;
+    __device__ __forceinline__ void pick(long long r, float p, float m, float uf) {
+        // what stays: the bins before b and the first c of bin b (the last bin's weights are 0)
+        int b = NB;
+        u64 c = 0, total = s.wx[NB];
+        enum { COUNT, SUM, LEAST, DRAW };
+#pragma unroll 1
+        for (int stage = COUNT; stage <= DRAW; stage++) {
+            int x = 0; // the bin that the stage's place is in, and what it asks for there
+            u64 goal = 0;
+            u64 least = 0;
+            if (stage == LEAST) {
+                if (!(m > 0.f)) continue;
+                least = (u64)__double2ull_rn(ldexp(fmin((double)m, 1.0), a.scale));
+                // the last bin whose largest weight is `least` or more
+                for (int i = threadIdx.x; i < NB; i += PICK)
+                    if (s.table[i] >= (double)least && (i == NB - 1 || s.table[i + 1] < (double)least)) s.place[stage] = i;
+                __syncthreads();
+                x = s.place[stage];
+                if (x > b || (x == b && c == 0)) continue;
+            } else {
+                if (stage == COUNT) {
+                    if (!(w.k > 0 && (unsigned)w.k < s.cx[NB])) continue;
+                    goal = (u64)w.k;
+                    x = reaching(s.cx, goal, stage);
+                    goal -= s.cx[x];
+                } else {
+                    if (stage == SUM) {
+                        if (!(p < 1.f)) continue;
+                        goal = max((u64)1, min(total, (u64)ceil((double)fmaxf(p, 0.f) * (double)total)));
+                    } else { // the first sum that is above u * total
+                        const double at = uf > 0.f ? floor((double)uf * (double)total) : 0.0;
+                        goal = at >= (double)total ? total : min(total, (u64)at + 1);
+                    }
+                    x = min(b, reaching(s.wx, goal, stage));
+                    goal -= s.wx[x];
+                }
             }
-            if (lo < bp || (lo == bp && cp > 0)) {
-                const u64 c = at_least(lo, least);
-                if (lo < bp || c < cp) { bp = lo; cp = c; }
+            const bool listed = collect(x, stage);
+            u64 found = 0, n = 0, sum = 0; // the place within the bin, and the weights up to it
+            if (stage == LEAST) {
+                if (threadIdx.x == 0) s.both[0] = s.both[1] = 0;
+                __syncthreads();
+                each_collected(listed, [&](u64, u64 wt) {
+                    if (wt >= least) { atomicAdd(&s.both[0], (u64)1); atomicAdd(&s.both[1], wt); }
+                });
+                __syncthreads();
+                n = s.both[0];
+                sum = s.both[1];
+                __syncthreads();
+            } else select(listed, stage != COUNT, goal, found, n, sum);
+            if (stage == DRAW) {
+                if (threadIdx.x == 0) {
+                    a.ids[r] = (int)(unsigned)found;
+                    if (a.prob) a.prob[r] = (float)((double)weight(found) / (double)total);
+                }
+            } else if (x < b || c == 0 || n < c) { // (c == 0: bin b was not cut)
+                b = x;
+                c = n;
+                total = s.wx[x] + sum;
             }
-        }
-        if (bp != bl || cp != cl) total = s.wx[bp] + weight_of_first(bp, cp);
-        const float uf = a.u[r];
-        const double at = uf > 0.f ? floor((double)uf * (double)total) : 0.0;
-        const u64 g = at >= (double)total ? total : min(total, (u64)at + 1); // the first sum that is above u * total
-        int b = min(bp, bin_reaching(s.wx, g));
-        u64 wt;
-        const u64 c = place_of(b, g - s.wx[b]);
-        const int id = candidate_at(b, c, wt);
-        if (threadIdx.x == 0) {
-            a.ids[r] = id;
-            if (a.prob) a.prob[r] = (float)((double)wt / (double)total);
         }
     }
 };
@@ -419,34 +541,110 @@ __global__ __launch_bounds__(PICK) void sample_pick_kernel(const smp_args a) {
     pick_lds &s = *(pick_lds *)raw;
     const long long r = blockIdx.x;
     const typename E::T *row = (const typename E::T *)a.logits + r * a.stride;
-    make_table(s.table, PICK);
-    float top;
-    unsigned *cnt = (unsigned *)s.list; // (before there is a list)
-    u64 *sum = s.lw;
-    if (threadIdx.x == 0) { s.la = s.lb = 0; }
+    unsigned *cnt = s.bins.cnt;
+    u64 *sum = s.bins.sum;
+    const float p = a.top_p ? a.top_p[r] : 1.f, m = a.min_p ? a.min_p[r] : 0.f, uf = a.u[r];
+    float mine = -INFINITY, top;
+    passes ps;
+    if constexpr (OWN)
+        each<E, PICK, false>(row, 0, a.n, [&](const auto &l, int) {
+#pragma unroll
+            for (float x : l) mine = fmaxf(mine, x);
+        });
+    make_table(s.table, (double *)s.head, PICK, a.scale);
+    if constexpr (OWN) row_bound(a, r, mine, s.d, top, ps);
+    else {
+        top = a.bound[2 * r + 1];
+        ps = passes_of(row_settings(a, r, top).k, a.bound[2 * r]);
+    }
+    if (!candidate(top)) {
+        if (threadIdx.x == 0) { a.ids[r] = -1; if (a.prob) a.prob[r] = 0.f; }
+        return;
+    }
+    const row_of w = row_settings(a, r, top);
+    for (int b = threadIdx.x; b <= NB; b += PICK) {
+        unsigned c = 0;
+        u64 x = 0;
+        if (!OWN && ps.tail)
+#pragma unroll 8
+            for (int q = 0; q < a.parts; q++) {
+                if (ps.counts) c += a.cnt[(r * a.parts + q) * (NB + 1) + b];
+                x += a.sum[(r * a.parts + q) * (NB + 1) + b];
+            }
+        cnt[b] = c;
+        sum[b] = x;
+    }
+    if (threadIdx.x < 4) { s.n[threadIdx.x] = 0; s.place[threadIdx.x] = NB; s.n_head = s.n_few = 0; }
+    __syncthreads();
     if constexpr (OWN) {
-        for (int b = threadIdx.x; b <= NB; b += PICK) { cnt[b] = 0; sum[b] = 0; }
-        float m = -INFINITY;
-        each<E, PICK>(row, 0, a.n, [&](float l, long long) { m = fmaxf(m, l); });
-        top = block_max<PICK>(m, s.shf);
-    } else top = row_top(a, r);
-    picker<E> pk{a, row, row_settings(a, r, top), s};
-    if constexpr (OWN) {
+        second_pass<E, false>(row, 0, a.n, w, ps, s.head, &s.n_head, HEAD, cnt, sum, s.table);
         __syncthreads();
-        each<E, PICK>(row, 0, a.n, [&](float l, long long) { add_to_bins(pk.w, l, cnt, sum, s.table); });
-    } else {
-        for (int b = threadIdx.x; b <= NB; b += PICK) { cnt[b] = a.cnt[r * (NB + 1) + b]; sum[b] = a.sum[r * (NB + 1) + b]; }
+    } else { // the parts' heads one behind the other, a wave a part
+        const int lane = threadIdx.x & 63;
+        const unsigned n = lane < a.parts ? a.held[r * a.parts + lane] : 0;
+        unsigned before = n > PART_HEAD ? HEAD + 1 : n; // (too many anywhere: no head)
+        const unsigned own = before;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const unsigned y = __shfl_up(before, o, 64);
+            if (lane >= o) before += y;
+        }
+        const unsigned all = __shfl(before, 63, 64);
+        before -= own;
+        if (all <= HEAD)
+            for (int q = threadIdx.x >> 6; q < a.parts; q += PICK / 64) {
+                const unsigned at = __shfl(before, q, 64), m = __shfl(own, q, 64);
+                for (unsigned i = lane; i < m; i += 64) s.head[at + i] = a.head[(r * a.parts + q) * PART_HEAD + i];
+            }
+        if (threadIdx.x == 0) s.n_head = (int)all;
+        __syncthreads();
+    }
+    int in_head = ps.tail ? bin_of(z_of(w, ps.bound)) : NB + 1;
+    if (s.n_head > HEAD) { // no head, and every candidate in the bins
+        in_head = 0;
+        if (!ps.tail) {
+            const passes all{NAN, true, true}; // (nothing is at or above it)
+            second_pass<E, true>(row, 0, a.n, w, all, s.head, &s.n[0], 0, cnt, sum, s.table);
+        }
+    } else if (!ps.tail) {
+        for (int i = threadIdx.x; i < s.n_head; i += PICK) add_to_bins(w, from_order(~(unsigned)(s.head[i] >> 32)), cnt, sum, s.table, true);
     }
     __syncthreads();
-    // sums before each bin: a thread has two bins
-    u64 all;
-    const int b0 = 2 * threadIdx.x, b1 = b0 + 1;
-    const u64 c0 = b0 <= NB ? cnt[b0] : 0, c1 = b1 <= NB ? cnt[b1] : 0, w0 = b0 <= NB ? sum[b0] : 0, w1 = b1 <= NB ? sum[b1] : 0;
-    const u64 cb = scan64(c0 + c1, s.sh, &all), wb = scan64(w0 + w1, s.sh, &all);
-    if (b0 <= NB + 1) { s.cx[b0] = (unsigned)cb; s.wx[b0] = wb; }
-    if (b1 <= NB + 1) { s.cx[b1] = (unsigned)(cb + c0); s.wx[b1] = wb + w0; }
+    // sums before each bin: a thread of four waves has six bins
+    constexpr int EACH = 6;
+    static_assert(256 * EACH >= NB + 2, "");
+    const int t = threadIdx.x, lane = t & 63;
+    unsigned c[EACH], cs = 0, cp = 0;
+    u64 x[EACH], xs = 0, xp = 0;
+    if (t < 256) {
+#pragma unroll
+        for (int e = 0; e < EACH; e++) {
+            const int b = t * EACH + e;
+            c[e] = b <= NB ? cnt[b] : 0;
+            x[e] = b <= NB ? sum[b] : 0;
+            cs += c[e];
+            xs += x[e];
+        }
+        cp = (unsigned)wave_sums(cs);
+        xp = wave_sums(xs);
+        if (lane == 63) { s.sh[t >> 6] = xp; s.sh[4 + (t >> 6)] = cp; }
+    }
     __syncthreads();
-    pk.pick(r);
+    if (t < 256) {
+        cp -= cs;
+        xp -= xs;
+        for (int i = 0; i < t >> 6; i++) { xp += s.sh[i]; cp += (unsigned)s.sh[4 + i]; }
+#pragma unroll
+        for (int e = 0; e < EACH; e++) {
+            const int b = t * EACH + e;
+            if (b <= NB + 1) { s.cx[b] = cp; s.wx[b] = xp; }
+            cp += c[e];
+            xp += x[e];
+        }
+    }
+    __syncthreads();
+    picker<E> pk{a, row, w, s, in_head};
+    pk.pick(r, p, m, uf);
 }
 
 template <class E>
@@ -460,28 +658,33 @@ void launch(const smp_args &a, hipStream_t st) {
     }
     if (ps_first_on_device(&seen[1])) (void)hipFuncSetAttribute((const void *)sample_pick_kernel<E, false>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
     hipLaunchKernelGGL((sample_top_kernel<E>), dim3((unsigned)a.parts, (unsigned)a.rows), dim3(256), 0, st, a);
-    hipLaunchKernelGGL((sample_bins_kernel<E>), dim3((unsigned)a.parts, (unsigned)a.rows), dim3(256), 0, st, a);
+    hipLaunchKernelGGL((sample_head_kernel<E>), dim3((unsigned)a.parts, (unsigned)a.rows), dim3(PICK), 0, st, a);
     hipLaunchKernelGGL((sample_pick_kernel<E, false>), dim3((unsigned)a.rows), dim3(PICK), lds, st, a);
 }
 } // namespace
 
 size_t psv_sample_space(int n_cu, int dtype, const void *logits, int64_t n, int64_t rows, int64_t stride, const ps_sample_params *p, int32_t *ids, float *prob, void *base, bool launch_, hipStream_t st) {
     smp_args a{};
-    // a row alone where there is a row for half the CUs; else parts of at least 2048 logits, as many as fill the chip twice
-    a.parts = rows * 2 > n_cu ? 1 : (int)std::max<int64_t>(1, std::min<int64_t>({(2 * n_cu + rows - 1) / std::max<int64_t>(rows, 1), (n + 2047) / 2048, 128}));
+    // a row alone where there is a row for half the CUs; else 4, 8 .. 64 parts (1024 groups of a row in all) of at least 1024 logits, as many as the chip takes at once
+    a.parts = 1;
+    if (rows * 2 <= n_cu && n >= 4096)
+        for (a.parts = 4; a.parts < 64 && a.parts * 2 * rows <= 2 * n_cu && a.parts * 2 * 1024 <= n;) a.parts *= 2;
     ps_carve ws{(char *)base};
     if (a.parts > 1) {
-        a.top = ws.take<float>((size_t)(rows * a.parts));
-        a.cnt = ws.take<unsigned>((size_t)rows * (NB + 1));
-        a.sum = ws.take<u64>((size_t)rows * (NB + 1));
+        a.top = ws.take<float>((size_t)rows * 1024);
+        a.bound = ws.take<float>((size_t)rows * 2);
+        a.cnt = ws.take<unsigned>((size_t)rows * a.parts * (NB + 1));
+        a.sum = ws.take<u64>((size_t)rows * a.parts * (NB + 1));
+        a.head = ws.take<u64>((size_t)rows * a.parts * PART_HEAD);
+        a.held = ws.take<unsigned>((size_t)rows * a.parts);
     }
     if (!launch_) return ws.at;
-    a.logits = logits; a.n = n; a.rows = rows; a.stride = stride;
+    a.logits = logits; a.n = (int)n; a.rows = rows; a.stride = stride;
     a.temperature = p->temperature; a.top_k = p->top_k; a.top_p = p->top_p; a.min_p = p->min_p; a.u = p->u;
     a.ids = ids; a.prob = prob;
     int bits = 0;
     while (((int64_t)1 << bits) < n) bits++;
-    a.scale = 62 - bits; // a row's weights add up to at most 2^62
+    a.scale = std::min(51, 62 - bits); // a row's weights add up to at most 2^62, one is below 2^52
     if (dtype == PS_F32) launch<F32>(a, st);
     else if (dtype == PS_F16) launch<F16>(a, st);
     else launch<BF16>(a, st);
