@@ -37,6 +37,8 @@ struct ca_args {
     float *part; // [seq][kv head][16 rows][part]: 16 x dim results, 16 maxima, 16 sums
     float *lse;  // [seq][kv head][T R] log2 of the sum of weights (+inf: no weights)
     int parts, tiles; // tiles of 16 rows
+    int wparts;       // parts of the rows that the weights are summed in
+    float *wpart;     // [seq][kv head][part][slot]
 };
 struct ca_lens { int n0, cnt, len; };
 __device__ __forceinline__ ca_lens lens_of(const ca_args &a, int s) {
@@ -106,7 +108,7 @@ __device__ __forceinline__ pv_f4 dot(const frame<E, DP> &k, const frame<E, DP> &
     return c;
 }
 
-constexpr int VPAD = 8; // numbers behind a value row in LDS
+constexpr int VPAD = 16; // numbers behind a value row in LDS: four rows of eight banks side by side
 
 template <class E, int DP, int RT>
 __global__ __launch_bounds__(256) void cache_attn_kernel(const ca_args a) {
@@ -351,6 +353,7 @@ __global__ __launch_bounds__(256) void cache_join_kernel(const ca_args a) {
     for (int e = (threadIdx.x & 15) * 4; e < a.dim; e += 64) {
         pv_f4 v = {0.f, 0.f, 0.f, 0.f};
         for (int i = 0; i < n; i++) {
+            if (part[i * step + 16 * a.dim + rr] == -INFINITY) continue; // (no result is left there)
             const float f = __builtin_amdgcn_exp2f(part[i * step + 16 * a.dim + rr] - ms);
             const pv_f4 x = *(const pv_f4 *)(part + i * step + rr * a.dim + e);
 #pragma unroll
@@ -418,6 +421,314 @@ __global__ __launch_bounds__(256) void cache_weight_kernel(const ca_args a) {
     w_out[j] = j < L.n0 && w_in ? w_in[j] + sum : sum;
 }
 
+typedef float f16v __attribute__((ext_vector_type(16)));
+template <class E> __device__ __forceinline__ f16v mfma32(const pv_u4 &x, const pv_u4 &y, const f16v &c);
+template <> __device__ __forceinline__ f16v mfma32<BF16>(const pv_u4 &x, const pv_u4 &y, const f16v &c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(b8, x), __builtin_bit_cast(b8, y), c, 0, 0, 0);
+}
+template <> __device__ __forceinline__ f16v mfma32<F16>(const pv_u4 &x, const pv_u4 &y, const f16v &c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8, x), __builtin_bit_cast(h8, y), c, 0, 0, 0);
+}
+// new rows into the caches, for the forms that read everything from there: 16 bytes a thread
+__global__ __launch_bounds__(256) void cache_append_kernel(const ca_args a, int row_bytes) {
+    const int s = blockIdx.y;
+    const ca_lens L = lens_of(a, s);
+    const int per = row_bytes / 16, x = blockIdx.x * 256 + threadIdx.x, t = x / (a.G * per), g = x / per % a.G, e = x % per * 16;
+    if (t >= L.cnt) return;
+    const long long to = s * a.seq + (L.n0 + t) * a.slot + g * a.head + e, from = s * a.new_seq + t * a.new_row + (long long)g * row_bytes + e;
+    *(pv_u4 *)(a.k + to) = *(const pv_u4 *)(a.k_new + from);
+    *(pv_u4 *)(a.v + to) = *(const pv_u4 *)(a.v_new + from);
+    if (e == 0 && a.pos_new && a.pos) a.pos[((long long)s * a.G + g) * a.n_ctx + L.n0 + t] = a.pos_new[(long long)s * a.T + t];
+}
+
+// Many rows of a 16-bit cache: 128 of a kv head against a part of its keys, a wave 32 of them against all, 64 keys at a time through two LDS stages that the four waves fill.  The products are
+// v_mfma_f32_32x32x16: S^T = K Q^T with the queries in registers (a lane: one row, 16 keys a tile), O^T = V^T P^T with the weights as they come, values transposed on their way out of LDS.
+// The weights go into the second product as one 16-bit number each (rounded like the result is: 2^-9 of a weight, bf16, to either side); their sum is taken before they are rounded.
+// What bounds it: the first operands of both products from LDS, 32 KB a wave and 64 keys beside 32 instructions of 32 clocks, and as many clocks of soft-max, which two work-groups a CU overlap.
+constexpr int ROWS = 128, KEYS = 64;
+template <class E, int DP>
+__global__ __launch_bounds__(256, 2) void cache_rows_kernel(const ca_args a) {
+    constexpr int KS = DP / 16, MD = DP / 32, KR = DP + 8, VR = DP + 32, PER = DP / 8, ST = KEYS * PER / 256; // rows in LDS: 16 banks further for the next value row, 4 for the next key
+    __shared__ __attribute__((aligned(16))) unsigned short kl[2][KEYS * KR], vl[2][KEYS * VR];
+    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, c = lane & 31, h = lane >> 5;
+    const int rows_all = a.T * a.R, blocks = (rows_all + ROWS - 1) / ROWS;
+    int id = blockIdx.x;
+    const int rb = blocks - 1 - id % blocks; id /= blocks; // (the longest causal rows first)
+    const int split = id % a.parts; id /= a.parts;
+    const int g = id % a.G, s = id / a.G;
+    const ca_lens L = lens_of(a, s);
+    const int rows = L.cnt * a.R, chunk = chunk_of(L.len, a.parts), k0 = split * chunk, k1 = min(L.len, k0 + chunk);
+    if (rb * ROWS >= rows || k0 >= L.len) return;
+    const int r0 = rb * ROWS + wave * 32, row = min(r0 + c, rows - 1), tok = row / a.R, first = min(r0, rows - 1) / a.R;
+    const int kend = a.tree ? k1 : min(k1, L.n0 + min(rb * ROWS + ROWS - 1, rows - 1) / a.R + 1); // behind the last key that a row of the work-group sees
+    const char *kb_ = a.k + s * a.seq + g * a.head, *vb_ = a.v + s * a.seq + g * a.head;
+    pv_u4 qf[KS];
+    {
+        const char *q = a.q + s * a.q_seq + tok * a.q_row + (long long)(g * a.R + row % a.R) * a.dim * 2;
+#pragma unroll
+        for (int st = 0; st < KS; st++) {
+            const int e = 16 * st + 8 * h;
+            qf[st] = *(const pv_u4 *)(q + (e < a.dim ? e * 2 : 0));
+            if (e >= a.dim) qf[st] = (pv_u4){0, 0, 0, 0};
+        }
+    }
+    f16v o[MD];
+#pragma unroll
+    for (int m = 0; m < MD; m++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) o[m][i] = 0.f;
+    float mx = -INFINITY, l = 0.f;
+    bool odd = false;
+    pv_u4 ks[ST], vs[ST];
+    auto fetch = [&](int kb) {
+#pragma unroll
+        for (int i = 0; i < ST; i++) {
+            const int x = tid + 256 * i, j = kb + x / PER, e = x % PER * 8;
+            const long long at = min(j, L.len - 1) * a.slot + (e < a.dim ? e * 2 : 0);
+            ks[i] = *(const pv_u4 *)(kb_ + at);
+            vs[i] = *(const pv_u4 *)(vb_ + at);
+            if (e >= a.dim) ks[i] = (pv_u4){0, 0, 0, 0};
+            if (j >= L.len || e >= a.dim) vs[i] = (pv_u4){0, 0, 0, 0};
+        }
+    };
+    auto put = [&](int kb, int buf) {
+#pragma unroll
+        for (int i = 0; i < ST; i++) {
+            const int x = tid + 256 * i, r = x / PER, e = x % PER * 8;
+            if (kb + KEYS > L.n0 && kb + r >= L.n0) { // a new token's infinities and NaN stay out of the products
+#pragma unroll
+                for (int y = 0; y < 4; y++)
+                    if (odd16<E>(vs[i][y])) { odd = true; vs[i][y] = without_odd<E>(vs[i][y]); }
+            }
+            *(pv_u4 *)(kl[buf] + r * KR + e) = ks[i];
+            *(pv_u4 *)(vl[buf] + r * VR + e) = vs[i];
+        }
+    };
+    if (k0 < kend) { fetch(k0); put(k0, 0); }
+    __syncthreads();
+    int cur = 0;
+#pragma unroll 1
+    for (int kb = k0; kb < kend; kb += KEYS, cur ^= 1) {
+        const bool more = kb + KEYS < kend;
+        if (more) fetch(kb + KEYS);
+        f16v z[2];
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+#pragma unroll
+            for (int i = 0; i < 16; i++) z[u][i] = 0.f;
+#pragma unroll
+            for (int st = 0; st < KS; st++) z[u] = mfma32<E>(*(const pv_u4 *)(kl[cur] + (32 * u + c) * KR + 16 * st + 8 * h), qf[st], z[u]);
+        }
+        if (!a.tree) {
+            if (kb + KEYS > L.n0 + first + 1) { // (what lies behind the last token lies behind this one's)
+                const int last = L.n0 + tok - kb - 4 * h;
+#pragma unroll
+                for (int u = 0; u < 2; u++)
+#pragma unroll
+                    for (int i = 0; i < 16; i++)
+                        if (32 * u + 8 * (i >> 2) + (i & 3) > last) z[u][i] = -INFINITY;
+            }
+        } else if (kb + KEYS > L.n0) {
+            const uint8_t *see = a.tree + ((long long)s * a.T + tok) * a.T;
+#pragma unroll
+            for (int u = 0; u < 2; u++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) {
+                    const int j = kb + 32 * u + 8 * (i >> 2) + 4 * h + (i & 3), x = j - L.n0;
+                    const bool seen = see[min(max(x, 0), L.cnt - 1)] != 0;
+                    if (j >= k1 || (x >= 0 && !seen)) z[u][i] = -INFINITY;
+                }
+        }
+        float top = fmaxf(z[0][0], z[1][0]);
+#pragma unroll
+        for (int i = 1; i < 16; i++) top = fmaxf(fmaxf(z[0][i], z[1][i]), top);
+        top = fmaxf(top, __shfl_xor(top, 32, 64)) * a.sc2;
+        if (__any(top > mx)) { // most blocks behind the first few raise no maximum
+            const float mn = fmaxf(mx, top), ms = mn == -INFINITY ? 0.f : mn, al = __builtin_amdgcn_exp2f(mx - ms);
+            l *= al;
+#pragma unroll
+            for (int m = 0; m < MD; m++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) o[m][i] *= al;
+            mx = mn;
+        }
+        const float ms = mx == -INFINITY ? 0.f : mx;
+        pv_u4 pk[4];
+        float sum = 0.f;
+#pragma unroll
+        for (int u = 0; u < 2; u++)
+#pragma unroll
+            for (int i = 0; i < 16; i += 2) {
+                const float p0 = __builtin_amdgcn_exp2f(fmaf(z[u][i], a.sc2, -ms)), p1 = __builtin_amdgcn_exp2f(fmaf(z[u][i + 1], a.sc2, -ms));
+                sum += p0 + p1;
+                pk[2 * u + (i >> 3)][(i >> 1) & 3] = round2<E>(p0, p1);
+            }
+        l += sum;
+        const unsigned short *base = vl[cur] + (4 * h + ((lane & 15) >> 2)) * VR + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+        typedef __attribute__((address_space(3))) s4 lds_s4;
+#pragma unroll
+        for (int k = 0; k < 4; k++)
+#pragma unroll
+            for (int m = 0; m < MD; m++) {
+                const s4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)(base + 16 * k * VR + 32 * m)), y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)(base + (16 * k + 8) * VR + 32 * m));
+                const pv_u2 xx = __builtin_bit_cast(pv_u2, x), yy = __builtin_bit_cast(pv_u2, y);
+                o[m] = mfma32<E>((pv_u4){xx[0], xx[1], yy[0], yy[1]}, pk[k], o[m]);
+            }
+        if (more) put(kb + KEYS, cur ^ 1);
+        __syncthreads();
+    }
+    odd = __syncthreads_or(odd);
+    l += __shfl_xor(l, 32, 64);
+    if (r0 + c >= rows) return;
+    if (odd)
+        for (int j = max(k0, L.n0); j < kend; j++) {
+            if (!sees(a, s, tok, j - L.n0)) continue;
+            const char *src = vb_ + j * a.slot;
+#pragma unroll
+            for (int m = 0; m < MD; m++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) {
+                    const int e = 32 * m + 8 * (i >> 2) + 4 * h + (i & 3);
+                    if (e >= a.dim) continue;
+                    const float x = number<E>(src + e * 2);
+                    if (odd32(x)) o[m][i] += x;
+                }
+        }
+    const float ms = mx == -INFINITY ? 0.f : mx;
+    if (a.parts > 1) {
+        float *part = a.part + ((((long long)s * a.G + g) * a.tiles + row / 16) * a.parts + split) * (16 * (a.dim + 2));
+        const int rr = row % 16;
+#pragma unroll
+        for (int m = 0; m < MD; m++)
+#pragma unroll
+            for (int i = 0; i < 16; i += 4) {
+                const int e = 32 * m + 2 * i + 4 * h;
+                if (e < a.dim) *(pv_f4 *)(part + rr * a.dim + e) = (pv_f4){o[m][i], o[m][i + 1], o[m][i + 2], o[m][i + 3]};
+            }
+        if (h == 0) { part[16 * a.dim + rr] = mx; part[16 * a.dim + 16 + rr] = l; }
+        return;
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    char *dst = a.out + s * a.o_seq + tok * a.o_row + (long long)(g * a.R + row % a.R) * a.dim * 2;
+#pragma unroll
+    for (int m = 0; m < MD; m++)
+#pragma unroll
+        for (int i = 0; i < 16; i += 4) {
+            const int e = 32 * m + 2 * i + 4 * h;
+            if (e < a.dim) *(pv_u2 *)(dst + e * 2) = (pv_u2){round2<E>(o[m][i] * inv, o[m][i + 1] * inv), round2<E>(o[m][i + 2] * inv, o[m][i + 3] * inv)};
+        }
+    if (h == 0) a.lse[((long long)s * a.G + g) * a.T * a.R + row] = l == 0.f ? INFINITY : ms + log2f(l);
+}
+
+// The weights that slots receive from many rows of a 16-bit cache: 256 keys of a kv head (a wave 64 of them, in registers) against a part of the rows, 32 at a time through LDS.  Sums over rows run in
+// a lane's registers; the parts' sums are left side by side (one part: added to what there is).
+template <class E, int DP>
+__global__ __launch_bounds__(256, 2) void cache_receive_kernel(const ca_args a) {
+    constexpr int KS = DP / 16, QR = DP + 8, PER = DP / 8, ST = 32 * PER / 256;
+    __shared__ __attribute__((aligned(16))) unsigned short ql[2][32 * QR];
+    __shared__ float lsl[2][32];
+    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, c = lane & 31, h = lane >> 5;
+    const int blocks = (a.n_ctx + 255) / 256;
+    int id = blockIdx.x;
+    const int split = id % a.wparts; id /= a.wparts;
+    const int b = id % blocks; id /= blocks;
+    const int g = id % a.G, s = id / a.G;
+    const ca_lens L = lens_of(a, s);
+    if (b * 256 >= L.len) return;
+    const int kb = b * 256 + wave * 64, rows = L.cnt * a.R, tiles = (rows + 31) / 32, per = (tiles + a.wparts - 1) / a.wparts;
+    // rows of tokens before the work-group's first key see none of its keys
+    const int from = a.tree || b * 256 < L.n0 ? 0 : (b * 256 - L.n0) * a.R / 32;
+    const int t0 = max(from, split * per), t1 = min(tiles, split * per + per);
+    pv_u4 kf[2][KS];
+#pragma unroll
+    for (int u = 0; u < 2; u++) {
+        const char *k = a.k + s * a.seq + g * a.head + min(kb + 32 * u + c, L.len - 1) * a.slot;
+#pragma unroll
+        for (int st = 0; st < KS; st++) {
+            const int e = 16 * st + 8 * h;
+            kf[u][st] = *(const pv_u4 *)(k + (e < a.dim ? e * 2 : 0));
+            if (e >= a.dim) kf[u][st] = (pv_u4){0, 0, 0, 0};
+        }
+    }
+    const float *lse = a.lse + ((long long)s * a.G + g) * a.T * a.R;
+    pv_u4 qs[ST];
+    float ls = 0.f;
+    auto fetch = [&](int tile) {
+#pragma unroll
+        for (int i = 0; i < ST; i++) {
+            const int x = tid + 256 * i, row = min(tile * 32 + x / PER, rows - 1), e = x % PER * 8;
+            qs[i] = *(const pv_u4 *)(a.q + s * a.q_seq + row / a.R * a.q_row + (long long)(g * a.R + row % a.R) * a.dim * 2 + (e < a.dim ? e * 2 : 0));
+            if (e >= a.dim) qs[i] = (pv_u4){0, 0, 0, 0};
+        }
+        if (tid < 32) ls = tile * 32 + tid < rows ? lse[tile * 32 + tid] : INFINITY;
+    };
+    auto put = [&](int buf) {
+#pragma unroll
+        for (int i = 0; i < ST; i++) { const int x = tid + 256 * i; *(pv_u4 *)(ql[buf] + x / PER * QR + x % PER * 8) = qs[i]; }
+        if (tid < 32) lsl[buf][tid] = ls;
+    };
+    float w[2][16] = {};
+    if (t0 < t1) { fetch(t0); put(0); }
+    __syncthreads();
+    int cur = 0;
+#pragma unroll 1
+    for (int tile = t0; tile < t1; tile++, cur ^= 1) {
+        if (tile + 1 < t1) fetch(tile + 1);
+        const float mine = lsl[cur][c];
+        const int tok = min(tile * 32 + c, rows - 1) / a.R;
+        f16v z[2];
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+#pragma unroll
+            for (int i = 0; i < 16; i++) z[u][i] = 0.f;
+        }
+#pragma unroll
+        for (int st = 0; st < KS; st++) {
+            const pv_u4 q = *(const pv_u4 *)(ql[cur] + c * QR + 16 * st + 8 * h);
+            z[0] = mfma32<E>(kf[0][st], q, z[0]);
+            z[1] = mfma32<E>(kf[1][st], q, z[1]);
+        }
+        if (kb + 64 <= (a.tree ? L.n0 : L.n0 + tile * 32 / a.R + 1)) { // all see all
+#pragma unroll
+            for (int u = 0; u < 2; u++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) w[u][i] += __builtin_amdgcn_exp2f(fmaf(z[u][i], a.sc2, -mine));
+        } else if (kb < L.len) {
+#pragma unroll
+            for (int u = 0; u < 2; u++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) {
+                    const int j = kb + 32 * u + 8 * (i >> 2) + 4 * h + (i & 3);
+                    if (mine != INFINITY && j < L.len && (j < L.n0 || sees(a, s, tok, j - L.n0))) w[u][i] += __builtin_amdgcn_exp2f(fmaf(z[u][i], a.sc2, -mine));
+                }
+        }
+        if (tile + 1 < t1) put(cur ^ 1);
+        __syncthreads();
+    }
+    const long long at = ((long long)s * a.G + g) * a.n_ctx;
+#pragma unroll
+    for (int u = 0; u < 2; u++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+            float v = w[u][i];
+#pragma unroll
+            for (int x = 1; x < 32; x <<= 1) v += __shfl_xor(v, x, 64);
+            const int j = kb + 32 * u + 8 * (i >> 2) + 4 * h + (i & 3);
+            if (c != 0 || j >= L.len) continue;
+            if (a.wparts > 1) a.wpart[(((long long)s * a.G + g) * a.wparts + split) * a.n_ctx + j] = v;
+            else a.weight_out[at + j] = j < L.n0 && a.weight ? a.weight[at + j] + v : v;
+        }
+}
+__global__ __launch_bounds__(256) void cache_gather_kernel(const ca_args a) { // the parts' sums, in order
+    const int j = blockIdx.x * 256 + threadIdx.x, g = blockIdx.y, s = blockIdx.z;
+    const ca_lens L = lens_of(a, s);
+    if (j >= L.len) return;
+    const long long head = (long long)s * a.G + g, at = head * a.n_ctx + j;
+    float v = 0.f;
+    for (int p = 0; p < a.wparts; p++) v += a.wpart[(head * a.wparts + p) * a.n_ctx + j];
+    a.weight_out[at] = j < L.n0 && a.weight ? a.weight[at] + v : v;
+}
+
 // an accepted path: a work-group per kv head and sequence, token after token (a row moves down, or stays)
 __global__ __launch_bounds__(256) void cache_take_kernel(char *k, char *v, long long seq, long long slot, long long head, int n_ctx, int row_bytes, const int32_t *n_kv, const int32_t *count, const int32_t *take,
                                                          int n_take, int32_t *pos, float *weight) {
@@ -460,8 +771,20 @@ __global__ __launch_bounds__(256) void cache_count_kernel(int32_t *n_kv, const i
 }
 
 template <class E, int DP>
-void launch_attn(const ca_args &a, hipStream_t st) {
+void launch_attn(const ca_args &a, bool many, hipStream_t st) {
     const long long heads = (long long)a.n_seqs * a.G;
+    if constexpr (E::SIZE == 2) {
+        if (many) {
+            const int row_bytes = a.dim * 2, pieces = a.T * a.G * (row_bytes / 16);
+            if (a.k_new) hipLaunchKernelGGL(cache_append_kernel, dim3((unsigned)((pieces + 255) / 256), (unsigned)a.n_seqs), dim3(256), 0, st, a, row_bytes);
+            hipLaunchKernelGGL((cache_rows_kernel<E, DP>), dim3((unsigned)(heads * a.parts * ((a.T * a.R + ROWS - 1) / ROWS))), dim3(256), 0, st, a);
+            if (a.parts > 1) hipLaunchKernelGGL((cache_join_kernel<E>), dim3((unsigned)(heads * a.tiles)), dim3(256), 0, st, a);
+            if (!a.weight_out) return;
+            hipLaunchKernelGGL((cache_receive_kernel<E, DP>), dim3((unsigned)(heads * ((a.n_ctx + 255) / 256) * a.wparts)), dim3(256), 0, st, a);
+            if (a.wparts > 1) hipLaunchKernelGGL(cache_gather_kernel, dim3((unsigned)((a.n_ctx + 255) / 256), (unsigned)a.G, (unsigned)a.n_seqs), dim3(256), 0, st, a);
+            return;
+        }
+    }
     // two tiles of rows a wave where there are two: its keys are read once for both
     if (a.tiles > 1) hipLaunchKernelGGL((cache_attn_kernel<E, DP, 2>), dim3((unsigned)(heads * a.parts * ((a.tiles + 1) / 2))), dim3(256), 0, st, a);
     else hipLaunchKernelGGL((cache_attn_kernel<E, DP, 1>), dim3((unsigned)(heads * a.parts)), dim3(256), 0, st, a);
@@ -477,11 +800,19 @@ size_t psv_attn_space(int n_cu, const ps_kv_cache &c, const ps_cache_attn_params
     const long long heads = (long long)c.n_seqs * c.kv_heads, rows = (long long)p.n_new * R;
     ca_args a{};
     a.tiles = (int)((rows + 15) / 16);
-    const long long groups = heads * ((a.tiles + 1) / 2);
-    a.parts = (int)std::min<long long>({std::max<long long>((3 * n_cu + groups - 1) / groups, (c.n_ctx + 1023) / 1024), (c.n_ctx + 127) / 128, 64});
+    // more than 32 rows of a 16-bit cache: 128 rows a work-group (its maxima are of scores before the scale, which has to be above 0)
+    const bool many = size == 2 && rows > 32 && p.scale > 0.f && p.scale < 1e30f;
+    const long long groups = heads * (many ? (rows + ROWS - 1) / ROWS : (a.tiles + 1) / 2);
+    a.parts = (int)std::min<long long>({std::max<long long>(((many ? 2 : 3) * n_cu + groups - 1) / groups, many ? 1 : (c.n_ctx + 1023) / 1024), (c.n_ctx + 127) / 128, 64});
     ps_carve ws{(char *)base};
     a.lse = ws.take<float>((size_t)(heads * rows));
     if (a.parts > 1) a.part = ws.take<float>((size_t)(heads * a.tiles * a.parts * 16 * (c.dim + 2)));
+    a.wparts = 1;
+    if (many && p.weight_out) { // parts of the rows until the chip is full twice, 128 rows at least
+        const long long blocks = heads * ((c.n_ctx + 255) / 256);
+        a.wparts = (int)std::max<long long>(1, std::min<long long>({(4 * n_cu + blocks - 1) / blocks, (rows + 127) / 128, 16}));
+        if (a.wparts > 1) a.wpart = ws.take<float>((size_t)(heads * a.wparts * c.n_ctx));
+    }
     if (!launch) return ws.at;
     a.k = (char *)c.k; a.v = (char *)c.v; a.out = (char *)p.out; a.q = (const char *)p.q; a.k_new = (const char *)p.k_new; a.v_new = (const char *)p.v_new;
     a.seq = c.seq_stride * size; a.slot = c.slot_stride * size; a.head = c.head_stride * size;
@@ -490,9 +821,9 @@ size_t psv_attn_space(int n_cu, const ps_kv_cache &c, const ps_cache_attn_params
     a.n_seqs = c.n_seqs; a.n_ctx = c.n_ctx; a.G = c.kv_heads; a.dim = c.dim; a.R = R; a.T = p.n_new;
     a.sc2 = p.scale * 1.44269504088896340736f;
     a.n_kv = c.n_kv; a.count = p.count; a.pos_new = p.pos_new; a.pos = c.pos; a.tree = p.tree; a.weight = c.weight; a.weight_out = p.weight_out;
-    if (c.dtype == PS_F32) c.dim > 64 ? launch_attn<F32, 128>(a, st) : launch_attn<F32, 64>(a, st);
-    else if (c.dtype == PS_F16) c.dim > 64 ? launch_attn<F16, 128>(a, st) : launch_attn<F16, 64>(a, st);
-    else c.dim > 64 ? launch_attn<BF16, 128>(a, st) : launch_attn<BF16, 64>(a, st);
+    if (c.dtype == PS_F32) c.dim > 64 ? launch_attn<F32, 128>(a, many, st) : launch_attn<F32, 64>(a, many, st);
+    else if (c.dtype == PS_F16) c.dim > 64 ? launch_attn<F16, 128>(a, many, st) : launch_attn<F16, 64>(a, many, st);
+    else c.dim > 64 ? launch_attn<BF16, 128>(a, many, st) : launch_attn<BF16, 64>(a, many, st);
     return ws.at;
 }
 
