@@ -4,7 +4,8 @@
 //   cache_attn_kernel     16 RT rows of one kv head against a part of its keys; the waves of a work-group share the part (blocks of 32 keys in turn), join in LDS, and leave sum, maximum and
 //                         unnormed result of the part -- or the result itself where there is one part.  New rows go into the cache on the way.
 //   cache_join_kernel     the parts of a row together; a row's log-sum of weights is left for
-//   cache_weight_kernel   64 keys against all rows once more: the soft-max weights from the scores and the log-sums, summed over rows in a fixed order
+//   cache_score_kernel    up to 32 rows: a slot's weights from the scores, which cache_attn_kernel leaves beside its result
+//   cache_rows_kernel, cache_receive_kernel, cache_gather_kernel   the same for more rows of a 16-bit cache, cache_weight_kernel of an fp32 one: the scores are made again for the weights
 // S^T = K Q^T, so that a lane has one row and maximum and sum run over its own registers and two lane moves; the second product O^T = V^T P^T takes its 32 keys in any order that both operands
 // share, so a lane's weights are its piece of the operand as they are.  16-bit values pass through LDS, a wave's own stretch, and come back transposed (ds_read_b64_tr_b16: 4 keys x 16 numbers).
 // Lengths are read on the device; a part is ceil(length / parts) keys, so that a fixed grid serves any length.
@@ -28,6 +29,7 @@ struct ca_args {
     const char *q, *k_new, *v_new;
     long long seq, slot, head, q_seq, q_row, o_seq, o_row, new_seq, new_row; // strides in bytes
     int n_seqs, n_ctx, G, dim, R, T;
+    unsigned by_R; // 2^32 / R, rounded up: what a row of fewer than 2^32 / R is divided with (R 1: 0)
     float sc2; // scale * log2(e): scores are held in units of log 2
     const int32_t *n_kv, *count, *pos_new;
     int32_t *pos;
@@ -35,12 +37,14 @@ struct ca_args {
     const float *weight;
     float *weight_out;
     float *part; // [seq][kv head][16 rows][part]: 16 x dim results, 16 maxima, 16 sums
+    float *score; // [seq][kv head][slot][score_rows]: scores of few rows for the weights, or NULL
     float *lse;  // [seq][kv head][T R] log2 of the sum of weights (+inf: no weights)
-    int parts, tiles; // tiles of 16 rows
+    int parts, tiles, score_rows; // tiles of 16 rows
     int wparts;       // parts of the rows that the weights are summed in
     float *wpart;     // [seq][kv head][part][slot]
 };
 struct ca_lens { int n0, cnt, len; };
+__device__ __forceinline__ int token_of(const ca_args &a, int row) { return a.by_R ? (int)__umulhi((unsigned)row, a.by_R) : row; }
 __device__ __forceinline__ ca_lens lens_of(const ca_args &a, int s) {
     ca_lens l;
     l.n0 = min(max(a.n_kv[s], 0), a.n_ctx);
@@ -111,7 +115,7 @@ __device__ __forceinline__ pv_f4 dot(const frame<E, DP> &k, const frame<E, DP> &
 constexpr int VPAD = 16; // numbers behind a value row in LDS: four rows of eight banks side by side
 
 template <class E, int DP, int RT>
-__global__ __launch_bounds__(256) void cache_attn_kernel(const ca_args a) {
+__global__ __launch_bounds__(256, E::SIZE == 4 ? 1 : 2) void cache_attn_kernel(const ca_args a) {
     constexpr int NS = STEPS<E, DP>, ND = DP / 16, OP = DP + 4, VR = DP + VPAD;
     constexpr int VBYTES = E::SIZE == 2 ? 4 * 32 * VR * 2 : 0, OBYTES = 4 * 16 * OP * 4;
     __shared__ __attribute__((aligned(16))) char lds[VBYTES > OBYTES ? VBYTES : OBYTES];
@@ -136,8 +140,8 @@ __global__ __launch_bounds__(256) void cache_attn_kernel(const ca_args a) {
 #pragma unroll
     for (int r = 0; r < RT; r++) {
         const int row = min((rb * RT + r) * 16 + c, L.cnt * a.R - 1); // rows behind the last repeat it
-        tok[r] = row / a.R;
-        get_row<E, DP>(qf[r], a.q + s * a.q_seq + tok[r] * a.q_row + (long long)(g * a.R + row % a.R) * a.dim * E::SIZE, q4, a.dim);
+        tok[r] = token_of(a, row);
+        get_row<E, DP>(qf[r], a.q + s * a.q_seq + tok[r] * a.q_row + (long long)(g * a.R + row - tok[r] * a.R) * a.dim * E::SIZE, q4, a.dim);
         m[r] = -INFINITY;
         l[r] = 0.f;
 #pragma unroll
@@ -225,6 +229,14 @@ __global__ __launch_bounds__(256) void cache_attn_kernel(const ca_args a) {
                     z[r][u][i] = v;
                     top = fmaxf(top, v);
                 }
+            if (a.score) {
+                float *sc = a.score + (((long long)s * a.G + g) * a.n_ctx + kb + 4 * q4) * a.score_rows + (rb * RT + r) * 16 + c;
+#pragma unroll
+                for (int u = 0; u < 2; u++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++)
+                        if ((rb * RT + r) * 16 + c < L.cnt * a.R && kb + 16 * u + 4 * q4 + i < k1) sc[(16 * u + i) * a.score_rows] = z[r][u][i];
+            }
             top = fmaxf(top, __shfl_xor(top, 16, 64));
             top = fmaxf(top, __shfl_xor(top, 32, 64));
             const float mn = fmaxf(m[r], top), ms = mn == -INFINITY ? 0.f : mn, al = __builtin_amdgcn_exp2f(m[r] - ms);
@@ -299,7 +311,7 @@ __global__ __launch_bounds__(256) void cache_attn_kernel(const ca_args a) {
         const float ms = top == -INFINITY ? 0.f : top;
 #pragma unroll
         for (int w = 0; w < 4; w++) { f[w] = __builtin_amdgcn_exp2f(lm[w][rr] - ms); sum = fmaf(ll[w][rr], f[w], sum); }
-        const int t = row / a.R, hd = g * a.R + row % a.R;
+        const int t = token_of(a, row), hd = g * a.R + row - t * a.R;
         float *part = a.part + ((((long long)s * a.G + g) * a.tiles + tile) * a.parts + split) * (16 * (a.dim + 2));
         const float inv = sum == 0.f ? 0.f : 1.f / sum;
         for (int e = (tid & 15) * 4; e < a.dim; e += 64) {
@@ -337,39 +349,83 @@ __global__ __launch_bounds__(256) void cache_attn_kernel(const ca_args a) {
 // a row's parts: 16 lanes a row, 16 rows a work-group
 template <class E>
 __global__ __launch_bounds__(256) void cache_join_kernel(const ca_args a) {
+    __shared__ float f[64][16]; // what a part's result is multiplied with
+    __shared__ float total[16];
     int id = blockIdx.x;
     const int tile = id % a.tiles; id /= a.tiles;
     const int g = id % a.G, s = id / a.G, rr = threadIdx.x >> 4, row = tile * 16 + rr;
     const ca_lens L = lens_of(a, s);
-    if (row >= L.cnt * a.R) return;
-    const int chunk = chunk_of(L.len, a.parts), n = (L.len + chunk - 1) / chunk, t = row / a.R, hd = g * a.R + row % a.R;
+    if (tile * 16 >= L.cnt * a.R) return;
+    const int chunk = chunk_of(L.len, a.parts), n = (L.len + chunk - 1) / chunk, t = token_of(a, row), hd = g * a.R + row - t * a.R;
     const long long step = 16 * (a.dim + 2);
     const float *part = a.part + (((long long)s * a.G + g) * a.tiles + tile) * a.parts * step;
-    float top = -INFINITY, sum = 0.f;
-    for (int i = 0; i < n; i++) top = fmaxf(top, part[i * step + 16 * a.dim + rr]);
-    const float ms = top == -INFINITY ? 0.f : top;
-    for (int i = 0; i < n; i++) sum = fmaf(part[i * step + 16 * a.dim + 16 + rr], __builtin_amdgcn_exp2f(part[i * step + 16 * a.dim + rr] - ms), sum);
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    if (threadIdx.x < 64) { // four lanes a row
+        const int r = threadIdx.x & 15, first = threadIdx.x >> 4;
+        float top = -INFINITY, sum = 0.f;
+        for (int i = first; i < n; i += 4) top = fmaxf(top, part[i * step + 16 * a.dim + r]);
+        top = fmaxf(top, __shfl_xor(top, 16, 64));
+        top = fmaxf(top, __shfl_xor(top, 32, 64));
+        const float ms = top == -INFINITY ? 0.f : top;
+        for (int i = first; i < n; i += 4) {
+            const float m = part[i * step + 16 * a.dim + r], x = __builtin_amdgcn_exp2f(m - ms);
+            sum = fmaf(part[i * step + 16 * a.dim + 16 + r], x, sum);
+            f[i][r] = m == -INFINITY ? 0.f : x; // (no result is left there)
+        }
+        sum += __shfl_xor(sum, 16, 64);
+        sum += __shfl_xor(sum, 32, 64);
+        if (first == 0) {
+            total[r] = sum;
+            if (tile * 16 + r < L.cnt * a.R) a.lse[((long long)s * a.G + g) * a.T * a.R + tile * 16 + r] = sum == 0.f ? INFINITY : ms + log2f(sum);
+        }
+    }
+    __syncthreads();
+    if (row >= L.cnt * a.R) return;
+    const float inv = total[rr] == 0.f ? 0.f : 1.f / total[rr];
     for (int e = (threadIdx.x & 15) * 4; e < a.dim; e += 64) {
         pv_f4 v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
         for (int i = 0; i < n; i++) {
-            if (part[i * step + 16 * a.dim + rr] == -INFINITY) continue; // (no result is left there)
-            const float f = __builtin_amdgcn_exp2f(part[i * step + 16 * a.dim + rr] - ms);
+            const float w = f[i][rr];
             const pv_f4 x = *(const pv_f4 *)(part + i * step + rr * a.dim + e);
 #pragma unroll
-            for (int y = 0; y < 4; y++) v[y] = fmaf(x[y], f, v[y]);
+            for (int y = 0; y < 4; y++) v[y] = w == 0.f ? v[y] : fmaf(x[y], w, v[y]);
         }
         char *dst = a.out + s * a.o_seq + t * a.o_row + ((long long)hd * a.dim + e) * E::SIZE;
         if constexpr (E::SIZE == 2) *(pv_u2 *)dst = (pv_u2){round2<E>(v[0] * inv, v[1] * inv), round2<E>(v[2] * inv, v[3] * inv)};
         else *(pv_f4 *)dst = (pv_f4){v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv};
     }
-    if ((threadIdx.x & 15) == 0) a.lse[((long long)s * a.G + g) * a.T * a.R + row] = sum == 0.f ? INFINITY : ms + log2f(sum);
 }
 
-// 64 keys of a kv head; the waves take the 16-row tiles in turn (SHARE), or 64 keys each where there is one tile or two
-template <class E, int DP, bool SHARE>
+// the weights of few rows from the scores that the attention has left, a thread a key
+constexpr int SCORE_KEYS = 1024;
+__global__ __launch_bounds__(256) void cache_score_kernel(const ca_args a) {
+    const int blocks = (a.n_ctx + SCORE_KEYS - 1) / SCORE_KEYS;
+    int id = blockIdx.x;
+    const int b = id % blocks; id /= blocks;
+    const int g = id % a.G, s = id / a.G;
+    const ca_lens L = lens_of(a, s);
+    if (b * SCORE_KEYS >= L.len) return;
+    const long long head = (long long)s * a.G + g;
+    const int rows = L.cnt * a.R, pitch = a.score_rows, end = min(L.len, (b + 1) * SCORE_KEYS);
+    __shared__ float lse[32];
+    if (threadIdx.x < 32) lse[threadIdx.x] = (int)threadIdx.x < rows ? a.lse[head * a.T * a.R + threadIdx.x] : INFINITY;
+    __syncthreads();
+    for (int j = b * SCORE_KEYS + threadIdx.x; j < end; j += 256) {
+        const long long at = head * a.n_ctx + j;
+        float w = 0.f;
+        for (int row = 0; row < rows; row += 4) {
+            const pv_f4 z = *(const pv_f4 *)(a.score + at * pitch + row);
+#pragma unroll
+            for (int i = 0; i < 4; i++) w += lse[row + i] == INFINITY ? 0.f : __builtin_amdgcn_exp2f(z[i] - lse[row + i]);
+        }
+        a.weight_out[at] = j < L.n0 && a.weight ? a.weight[at] + w : w;
+    }
+}
+
+// fp32 caches, more rows: 64 keys of a kv head; the waves take the 16-row tiles in turn
+template <class E, int DP>
 __global__ __launch_bounds__(256) void cache_weight_kernel(const ca_args a) {
-    constexpr int NS = STEPS<E, DP>, KEYS = SHARE ? 64 : 256;
+    constexpr int NS = STEPS<E, DP>, KEYS = 64;
     __shared__ float red[4][64];
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, c = lane & 15, q4 = lane >> 4;
     const int blocks = (a.n_ctx + KEYS - 1) / KEYS;
@@ -378,7 +434,7 @@ __global__ __launch_bounds__(256) void cache_weight_kernel(const ca_args a) {
     const int g = id % a.G, s = id / a.G;
     const ca_lens L = lens_of(a, s);
     if (b * KEYS >= L.len) return;
-    const int kb = b * KEYS + (SHARE ? 0 : wave * 64);
+    const int kb = b * KEYS;
     const float *w_in = a.weight ? a.weight + ((long long)s * a.G + g) * a.n_ctx : nullptr;
     float *w_out = a.weight_out + ((long long)s * a.G + g) * a.n_ctx;
     pv_u4 kf[4][NS];
@@ -388,11 +444,11 @@ __global__ __launch_bounds__(256) void cache_weight_kernel(const ca_args a) {
         for (int u = 0; u < 4; u++) get_row<E, DP>(kf[u], a.k + s * a.seq + g * a.head + min(kb + 16 * u + c, L.len - 1) * a.slot, q4, a.dim);
         const int rows = L.cnt * a.R;
         const float *lse = a.lse + ((long long)s * a.G + g) * a.T * a.R;
-        for (int tile = SHARE ? wave : 0; tile * 16 < rows; tile += SHARE ? 4 : 1) {
-            const int row = min(tile * 16 + c, rows - 1), t = row / a.R;
-            if (!a.tree && min(tile * 16 + 15, rows - 1) / a.R < kb - L.n0) continue; // all these tokens come before these keys
+        for (int tile = wave; tile * 16 < rows; tile += 4) {
+            const int row = min(tile * 16 + c, rows - 1), t = token_of(a, row);
+            if (!a.tree && token_of(a, min(tile * 16 + 15, rows - 1)) < kb - L.n0) continue; // all these tokens come before these keys
             pv_u4 qf[NS];
-            get_row<E, DP>(qf, a.q + s * a.q_seq + t * a.q_row + (long long)(g * a.R + row % a.R) * a.dim * E::SIZE, q4, a.dim);
+            get_row<E, DP>(qf, a.q + s * a.q_seq + t * a.q_row + (long long)(g * a.R + row - t * a.R) * a.dim * E::SIZE, q4, a.dim);
             const float ls = tile * 16 + c < rows ? lse[row] : INFINITY;
 #pragma unroll
             for (int u = 0; u < 4; u++) {
@@ -415,9 +471,9 @@ __global__ __launch_bounds__(256) void cache_weight_kernel(const ca_args a) {
             if (c == 0) red[wave][16 * u + 4 * q4 + i] = w[u][i];
         }
     __syncthreads();
-    const int j = SHARE ? kb + lane : b * KEYS + tid;
-    if (j >= L.len || (SHARE && wave)) return;
-    const float sum = SHARE ? (red[0][lane] + red[1][lane]) + (red[2][lane] + red[3][lane]) : red[wave][lane];
+    const int j = kb + lane;
+    if (j >= L.len || wave) return;
+    const float sum = (red[0][lane] + red[1][lane]) + (red[2][lane] + red[3][lane]);
     w_out[j] = j < L.n0 && w_in ? w_in[j] + sum : sum;
 }
 
@@ -446,6 +502,29 @@ __global__ __launch_bounds__(256) void cache_append_kernel(const ca_args a, int 
 // The weights go into the second product as one 16-bit number each (rounded like the result is: 2^-9 of a weight, bf16, to either side); their sum is taken before they are rounded.
 // What bounds it: the first operands of both products from LDS, 32 KB a wave and 64 keys beside 32 instructions of 32 clocks, and as many clocks of soft-max, which two work-groups a CU overlap.
 constexpr int ROWS = 128, KEYS = 64;
+// which of a lane's 16 keys of a tile its token sees, a bit each: key i is x0 + 8 (i / 4) + i % 4 behind the slots that were held.  (A tree: eight loads at once: 32 take registers that the tiles need, one at a time was 16 us of a small step.)
+__device__ __forceinline__ unsigned sees16(const ca_args &a, const ca_lens &L, int s, int tok, int x0) {
+    unsigned bits = 0;
+    if (!a.tree) { // those up to its own: so many of each four
+        const int n = min(tok, L.cnt - 1) - x0 + 1;
+#pragma unroll
+        for (int q = 0; q < 4; q++) bits |= ((1u << min(max(n - 8 * q, 0), 4)) - 1) << 4 * q;
+        return bits;
+    }
+    const uint8_t *see = a.tree + ((long long)s * a.T + tok) * a.T;
+#pragma unroll 1
+    for (int h = 0; h < 16; h += 8) {
+        uint8_t v[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[i] = see[min(max(x0 + 2 * h + 8 * (i >> 2) + (i & 3), 0), L.cnt - 1)];
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const int x = x0 + 2 * h + 8 * (i >> 2) + (i & 3);
+            bits |= (x < 0 || (x < L.cnt && v[i]) ? 1u : 0u) << (h + i);
+        }
+    }
+    return bits;
+}
 template <class E, int DP>
 __global__ __launch_bounds__(256, 2) void cache_rows_kernel(const ca_args a) {
     constexpr int KS = DP / 16, MD = DP / 32, KR = DP + 8, VR = DP + 32, PER = DP / 8, ST = KEYS * PER / 256; // rows in LDS: 16 banks further for the next value row, 4 for the next key
@@ -453,25 +532,27 @@ __global__ __launch_bounds__(256, 2) void cache_rows_kernel(const ca_args a) {
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, c = lane & 31, h = lane >> 5;
     const int rows_all = a.T * a.R, blocks = (rows_all + ROWS - 1) / ROWS;
     int id = blockIdx.x;
-    const int rb = blocks - 1 - id % blocks; id /= blocks; // (the longest causal rows first)
-    const int split = id % a.parts; id /= a.parts;
-    const int g = id % a.G, s = id / a.G;
+    // neighbours are kv heads, so that a head's keys stay in one XCD's L2; the rows with the most causal keys first, those with the fewest from the middle on: a CU's two work-groups add up alike
+    const int heads = a.n_seqs * a.G, hs = id % heads, s = hs / a.G, g = hs - s * a.G; id /= heads;
+    const int split = id % a.parts, p = id / a.parts, half = (blocks + 1) / 2, rb = p < half ? blocks - 1 - p : p - half;
     const ca_lens L = lens_of(a, s);
     const int rows = L.cnt * a.R, chunk = chunk_of(L.len, a.parts), k0 = split * chunk, k1 = min(L.len, k0 + chunk);
     if (rb * ROWS >= rows || k0 >= L.len) return;
-    const int r0 = rb * ROWS + wave * 32, row = min(r0 + c, rows - 1), tok = row / a.R, first = min(r0, rows - 1) / a.R;
-    const int kend = a.tree ? k1 : min(k1, L.n0 + min(rb * ROWS + ROWS - 1, rows - 1) / a.R + 1); // behind the last key that a row of the work-group sees
+    const int r0 = rb * ROWS + wave * 32, row = min(r0 + c, rows - 1), tok = token_of(a, row), first = token_of(a, min(r0, rows - 1));
+    const int kend = a.tree ? k1 : min(k1, L.n0 + token_of(a, min(rb * ROWS + ROWS - 1, rows - 1)) + 1); // behind the last key that a row of the work-group sees
     const char *kb_ = a.k + s * a.seq + g * a.head, *vb_ = a.v + s * a.seq + g * a.head;
     pv_u4 qf[KS];
     {
-        const char *q = a.q + s * a.q_seq + tok * a.q_row + (long long)(g * a.R + row % a.R) * a.dim * 2;
+        const char *q = a.q + s * a.q_seq + tok * a.q_row + (long long)(g * a.R + row - tok * a.R) * a.dim * 2;
 #pragma unroll
         for (int st = 0; st < KS; st++) {
             const int e = 16 * st + 8 * h;
             qf[st] = *(const pv_u4 *)(q + (e < a.dim ? e * 2 : 0));
             if (e >= a.dim) qf[st] = (pv_u4){0, 0, 0, 0};
+            if (a.sc2 < 0.f) qf[st] ^= 0x80008000u; // a negative scale turns the queries round
         }
     }
+    const float sc = fabsf(a.sc2);
     f16v o[MD];
 #pragma unroll
     for (int m = 0; m < MD; m++)
@@ -480,7 +561,16 @@ __global__ __launch_bounds__(256, 2) void cache_rows_kernel(const ca_args a) {
     float mx = -INFINITY, l = 0.f;
     bool odd = false;
     pv_u4 ks[ST], vs[ST];
+    long long off[ST]; // of a thread's pieces of a tile
+#pragma unroll
+    for (int i = 0; i < ST; i++) { const int x = tid + 256 * i, e = x % PER * 8; off[i] = x / PER * a.slot + (e < a.dim ? e * 2 : 0); }
     auto fetch = [&](int kb) {
+        if (kb + KEYS <= L.len && a.dim == DP) {
+            const char *kt = kb_ + kb * a.slot, *vt = vb_ + kb * a.slot;
+#pragma unroll
+            for (int i = 0; i < ST; i++) { ks[i] = *(const pv_u4 *)(kt + off[i]); vs[i] = *(const pv_u4 *)(vt + off[i]); }
+            return;
+        }
 #pragma unroll
         for (int i = 0; i < ST; i++) {
             const int x = tid + 256 * i, j = kb + x / PER, e = x % PER * 8;
@@ -513,36 +603,23 @@ __global__ __launch_bounds__(256, 2) void cache_rows_kernel(const ca_args a) {
         if (more) fetch(kb + KEYS);
         f16v z[2];
 #pragma unroll
-        for (int u = 0; u < 2; u++) {
+        for (int i = 0; i < 16; i++) z[0][i] = z[1][i] = 0.f;
 #pragma unroll
-            for (int i = 0; i < 16; i++) z[u][i] = 0.f;
+        for (int st = 0; st < KS; st++)
 #pragma unroll
-            for (int st = 0; st < KS; st++) z[u] = mfma32<E>(*(const pv_u4 *)(kl[cur] + (32 * u + c) * KR + 16 * st + 8 * h), qf[st], z[u]);
-        }
-        if (!a.tree) {
-            if (kb + KEYS > L.n0 + first + 1) { // (what lies behind the last token lies behind this one's)
-                const int last = L.n0 + tok - kb - 4 * h;
+            for (int u = 0; u < 2; u++) z[u] = mfma32<E>(*(const pv_u4 *)(kl[cur] + (32 * u + c) * KR + 16 * st + 8 * h), qf[st], z[u]);
+        if (kb + KEYS > (a.tree ? L.n0 : L.n0 + first + 1)) {
 #pragma unroll
-                for (int u = 0; u < 2; u++)
+            for (int u = 0; u < 2; u++) {
+                const unsigned bits = sees16(a, L, s, tok, kb + 32 * u + 4 * h - L.n0);
 #pragma unroll
-                    for (int i = 0; i < 16; i++)
-                        if (32 * u + 8 * (i >> 2) + (i & 3) > last) z[u][i] = -INFINITY;
+                for (int i = 0; i < 16; i++) z[u][i] = bits >> i & 1 ? z[u][i] : -INFINITY;
             }
-        } else if (kb + KEYS > L.n0) {
-            const uint8_t *see = a.tree + ((long long)s * a.T + tok) * a.T;
-#pragma unroll
-            for (int u = 0; u < 2; u++)
-#pragma unroll
-                for (int i = 0; i < 16; i++) {
-                    const int j = kb + 32 * u + 8 * (i >> 2) + 4 * h + (i & 3), x = j - L.n0;
-                    const bool seen = see[min(max(x, 0), L.cnt - 1)] != 0;
-                    if (j >= k1 || (x >= 0 && !seen)) z[u][i] = -INFINITY;
-                }
         }
-        float top = fmaxf(z[0][0], z[1][0]);
+        float top = fmaxf(z[0][0], z[1][0]); // (of scores before the scale, which is above 0 here)
 #pragma unroll
         for (int i = 1; i < 16; i++) top = fmaxf(fmaxf(z[0][i], z[1][i]), top);
-        top = fmaxf(top, __shfl_xor(top, 32, 64)) * a.sc2;
+        top = fmaxf(top, __shfl_xor(top, 32, 64)) * sc;
         if (__any(top > mx)) { // most blocks behind the first few raise no maximum
             const float mn = fmaxf(mx, top), ms = mn == -INFINITY ? 0.f : mn, al = __builtin_amdgcn_exp2f(mx - ms);
             l *= al;
@@ -559,7 +636,7 @@ __global__ __launch_bounds__(256, 2) void cache_rows_kernel(const ca_args a) {
         for (int u = 0; u < 2; u++)
 #pragma unroll
             for (int i = 0; i < 16; i += 2) {
-                const float p0 = __builtin_amdgcn_exp2f(fmaf(z[u][i], a.sc2, -ms)), p1 = __builtin_amdgcn_exp2f(fmaf(z[u][i + 1], a.sc2, -ms));
+                const float p0 = __builtin_amdgcn_exp2f(fmaf(z[u][i], sc, -ms)), p1 = __builtin_amdgcn_exp2f(fmaf(z[u][i + 1], sc, -ms));
                 sum += p0 + p1;
                 pk[2 * u + (i >> 3)][(i >> 1) & 3] = round2<E>(p0, p1);
             }
@@ -609,7 +686,7 @@ __global__ __launch_bounds__(256, 2) void cache_rows_kernel(const ca_args a) {
         return;
     }
     const float inv = l == 0.f ? 0.f : 1.f / l;
-    char *dst = a.out + s * a.o_seq + tok * a.o_row + (long long)(g * a.R + row % a.R) * a.dim * 2;
+    char *dst = a.out + s * a.o_seq + tok * a.o_row + (long long)(g * a.R + row - tok * a.R) * a.dim * 2;
 #pragma unroll
     for (int m = 0; m < MD; m++)
 #pragma unroll
@@ -620,13 +697,13 @@ __global__ __launch_bounds__(256, 2) void cache_rows_kernel(const ca_args a) {
     if (h == 0) a.lse[((long long)s * a.G + g) * a.T * a.R + row] = l == 0.f ? INFINITY : ms + log2f(l);
 }
 
-// The weights that slots receive from many rows of a 16-bit cache: 256 keys of a kv head (a wave 64 of them, in registers) against a part of the rows, 32 at a time through LDS.  Sums over rows run in
+// The weights that slots receive from many rows of a 16-bit cache: 256 keys of a kv head (a wave 64 of them, in registers) against a part of the rows, 64 at a time through LDS.  Sums over rows run in
 // a lane's registers; the parts' sums are left side by side (one part: added to what there is).
 template <class E, int DP>
 __global__ __launch_bounds__(256, 2) void cache_receive_kernel(const ca_args a) {
-    constexpr int KS = DP / 16, QR = DP + 8, PER = DP / 8, ST = 32 * PER / 256;
-    __shared__ __attribute__((aligned(16))) unsigned short ql[2][32 * QR];
-    __shared__ float lsl[2][32];
+    constexpr int KS = DP / 16, QR = DP + 8, PER = DP / 8, QT = 64, ST = QT * PER / 256;
+    __shared__ __attribute__((aligned(16))) unsigned short ql[2][QT * QR];
+    __shared__ float lsl[2][QT];
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, c = lane & 31, h = lane >> 5;
     const int blocks = (a.n_ctx + 255) / 256;
     int id = blockIdx.x;
@@ -635,9 +712,9 @@ __global__ __launch_bounds__(256, 2) void cache_receive_kernel(const ca_args a) 
     const int g = id % a.G, s = id / a.G;
     const ca_lens L = lens_of(a, s);
     if (b * 256 >= L.len) return;
-    const int kb = b * 256 + wave * 64, rows = L.cnt * a.R, tiles = (rows + 31) / 32, per = (tiles + a.wparts - 1) / a.wparts;
+    const int kb = b * 256 + wave * 64, rows = L.cnt * a.R, tiles = (rows + QT - 1) / QT, per = (tiles + a.wparts - 1) / a.wparts;
     // rows of tokens before the work-group's first key see none of its keys
-    const int from = a.tree || b * 256 < L.n0 ? 0 : (b * 256 - L.n0) * a.R / 32;
+    const int from = a.tree || b * 256 < L.n0 ? 0 : (b * 256 - L.n0) * a.R / QT;
     const int t0 = max(from, split * per), t1 = min(tiles, split * per + per);
     pv_u4 kf[2][KS];
 #pragma unroll
@@ -656,16 +733,16 @@ __global__ __launch_bounds__(256, 2) void cache_receive_kernel(const ca_args a) 
     auto fetch = [&](int tile) {
 #pragma unroll
         for (int i = 0; i < ST; i++) {
-            const int x = tid + 256 * i, row = min(tile * 32 + x / PER, rows - 1), e = x % PER * 8;
-            qs[i] = *(const pv_u4 *)(a.q + s * a.q_seq + row / a.R * a.q_row + (long long)(g * a.R + row % a.R) * a.dim * 2 + (e < a.dim ? e * 2 : 0));
+            const int x = tid + 256 * i, row = min(tile * QT + x / PER, rows - 1), tok = token_of(a, row), e = x % PER * 8;
+            qs[i] = *(const pv_u4 *)(a.q + s * a.q_seq + tok * a.q_row + (long long)(g * a.R + row - tok * a.R) * a.dim * 2 + (e < a.dim ? e * 2 : 0));
             if (e >= a.dim) qs[i] = (pv_u4){0, 0, 0, 0};
         }
-        if (tid < 32) ls = tile * 32 + tid < rows ? lse[tile * 32 + tid] : INFINITY;
+        if (tid < QT) ls = tile * QT + tid < rows ? lse[tile * QT + tid] : INFINITY;
     };
     auto put = [&](int buf) {
 #pragma unroll
         for (int i = 0; i < ST; i++) { const int x = tid + 256 * i; *(pv_u4 *)(ql[buf] + x / PER * QR + x % PER * 8) = qs[i]; }
-        if (tid < 32) lsl[buf][tid] = ls;
+        if (tid < QT) lsl[buf][tid] = ls;
     };
     float w[2][16] = {};
     if (t0 < t1) { fetch(t0); put(0); }
@@ -674,8 +751,11 @@ __global__ __launch_bounds__(256, 2) void cache_receive_kernel(const ca_args a) 
 #pragma unroll 1
     for (int tile = t0; tile < t1; tile++, cur ^= 1) {
         if (tile + 1 < t1) fetch(tile + 1);
-        const float mine = lsl[cur][c];
-        const int tok = min(tile * 32 + c, rows - 1) / a.R;
+#pragma unroll 1
+        for (int sub = 0; sub < QT / 32; sub++) {
+        const int r0 = tile * QT + 32 * sub;
+        const float mine = lsl[cur][32 * sub + c];
+        const int tok = token_of(a, min(r0 + c, rows - 1));
         f16v z[2];
 #pragma unroll
         for (int u = 0; u < 2; u++) {
@@ -684,23 +764,26 @@ __global__ __launch_bounds__(256, 2) void cache_receive_kernel(const ca_args a) 
         }
 #pragma unroll
         for (int st = 0; st < KS; st++) {
-            const pv_u4 q = *(const pv_u4 *)(ql[cur] + c * QR + 16 * st + 8 * h);
+            const pv_u4 q = *(const pv_u4 *)(ql[cur] + (32 * sub + c) * QR + 16 * st + 8 * h);
             z[0] = mfma32<E>(kf[0][st], q, z[0]);
             z[1] = mfma32<E>(kf[1][st], q, z[1]);
         }
-        if (kb + 64 <= (a.tree ? L.n0 : L.n0 + tile * 32 / a.R + 1)) { // all see all
+        if (kb + 64 <= (a.tree ? L.n0 : L.n0 + token_of(a, r0) + 1)) { // all see all
 #pragma unroll
             for (int u = 0; u < 2; u++)
 #pragma unroll
                 for (int i = 0; i < 16; i++) w[u][i] += __builtin_amdgcn_exp2f(fmaf(z[u][i], a.sc2, -mine));
         } else if (kb < L.len) {
 #pragma unroll
-            for (int u = 0; u < 2; u++)
+            for (int u = 0; u < 2; u++) {
+                const unsigned bits = mine == INFINITY ? 0 : sees16(a, L, s, tok, kb + 32 * u + 4 * h - L.n0);
 #pragma unroll
                 for (int i = 0; i < 16; i++) {
-                    const int j = kb + 32 * u + 8 * (i >> 2) + 4 * h + (i & 3);
-                    if (mine != INFINITY && j < L.len && (j < L.n0 || sees(a, s, tok, j - L.n0))) w[u][i] += __builtin_amdgcn_exp2f(fmaf(z[u][i], a.sc2, -mine));
+                    const float p = __builtin_amdgcn_exp2f(fmaf(z[u][i], a.sc2, -mine));
+                    w[u][i] += bits >> i & 1 ? p : 0.f;
                 }
+            }
+        }
         }
         if (tile + 1 < t1) put(cur ^ 1);
         __syncthreads();
@@ -790,8 +873,8 @@ void launch_attn(const ca_args &a, bool many, hipStream_t st) {
     else hipLaunchKernelGGL((cache_attn_kernel<E, DP, 1>), dim3((unsigned)(heads * a.parts)), dim3(256), 0, st, a);
     if (a.parts > 1) hipLaunchKernelGGL((cache_join_kernel<E>), dim3((unsigned)(heads * a.tiles)), dim3(256), 0, st, a);
     if (!a.weight_out) return;
-    if (a.tiles > 2) hipLaunchKernelGGL((cache_weight_kernel<E, DP, true>), dim3((unsigned)(heads * ((a.n_ctx + 63) / 64))), dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((cache_weight_kernel<E, DP, false>), dim3((unsigned)(heads * ((a.n_ctx + 255) / 256))), dim3(256), 0, st, a);
+    if (a.tiles <= 2) hipLaunchKernelGGL(cache_score_kernel, dim3((unsigned)(heads * ((a.n_ctx + SCORE_KEYS - 1) / SCORE_KEYS))), dim3(256), 0, st, a);
+    else if constexpr (E::SIZE == 4) hipLaunchKernelGGL((cache_weight_kernel<E, DP>), dim3((unsigned)(heads * ((a.n_ctx + 63) / 64))), dim3(256), 0, st, a);
 }
 } // namespace
 
@@ -800,13 +883,15 @@ size_t psv_attn_space(int n_cu, const ps_kv_cache &c, const ps_cache_attn_params
     const long long heads = (long long)c.n_seqs * c.kv_heads, rows = (long long)p.n_new * R;
     ca_args a{};
     a.tiles = (int)((rows + 15) / 16);
-    // more than 32 rows of a 16-bit cache: 128 rows a work-group (its maxima are of scores before the scale, which has to be above 0)
-    const bool many = size == 2 && rows > 32 && p.scale > 0.f && p.scale < 1e30f;
+    // more than 32 rows of a 16-bit cache: 128 rows a work-group
+    const bool many = size == 2 && rows > 32;
     const long long groups = heads * (many ? (rows + ROWS - 1) / ROWS : (a.tiles + 1) / 2);
-    a.parts = (int)std::min<long long>({std::max<long long>(((many ? 2 : 3) * n_cu + groups - 1) / groups, many ? 1 : (c.n_ctx + 1023) / 1024), (c.n_ctx + 127) / 128, 64});
+    a.parts = (int)std::min<long long>({std::max<long long>(((many ? 1 : 3) * n_cu + groups - 1) / groups, many ? 1 : (c.n_ctx + 1023) / 1024), (c.n_ctx + 127) / 128, 64});
     ps_carve ws{(char *)base};
     a.lse = ws.take<float>((size_t)(heads * rows));
     if (a.parts > 1) a.part = ws.take<float>((size_t)(heads * a.tiles * a.parts * 16 * (c.dim + 2)));
+    a.score_rows = (int)((rows + 3) / 4 * 4);
+    if (p.weight_out && a.tiles <= 2) a.score = ws.take<float>((size_t)(heads * c.n_ctx * a.score_rows));
     a.wparts = 1;
     if (many && p.weight_out) { // parts of the rows until the chip is full twice, 128 rows at least
         const long long blocks = heads * ((c.n_ctx + 255) / 256);
@@ -819,7 +904,8 @@ size_t psv_attn_space(int n_cu, const ps_kv_cache &c, const ps_cache_attn_params
     a.q_seq = p.q_seq_stride * size; a.q_row = p.q_row_stride * size; a.o_seq = p.out_seq_stride * size; a.o_row = p.out_row_stride * size;
     a.new_seq = p.new_seq_stride * size; a.new_row = p.new_row_stride * size;
     a.n_seqs = c.n_seqs; a.n_ctx = c.n_ctx; a.G = c.kv_heads; a.dim = c.dim; a.R = R; a.T = p.n_new;
-    a.sc2 = p.scale * 1.44269504088896340736f;
+    a.by_R = R == 1 ? 0 : (unsigned)((((unsigned long long)1 << 32) + R - 1) / R);
+    a.sc2 = p.scale == 0.f ? 1e-37f : p.scale * 1.44269504088896340736f; // (never 0: a masked score is minus infinity times it)
     a.n_kv = c.n_kv; a.count = p.count; a.pos_new = p.pos_new; a.pos = c.pos; a.tree = p.tree; a.weight = c.weight; a.weight_out = p.weight_out;
     if (c.dtype == PS_F32) c.dim > 64 ? launch_attn<F32, 128>(a, many, st) : launch_attn<F32, 64>(a, many, st);
     else if (c.dtype == PS_F16) c.dim > 64 ? launch_attn<F16, 128>(a, many, st) : launch_attn<F16, 64>(a, many, st);

@@ -41,9 +41,9 @@ const char *wrong_attn(const ps_kv_cache *k, const ps_cache_attn_params *p) {
     const int size = number_size(k->dtype);
     if (p->heads < 1 || p->heads % k->kv_heads) return "the query heads must be a multiple of the cache's heads";
     if (p->n_new < 0 || p->n_new > k->n_ctx) return "more new tokens than slots";
-    if (!std::isfinite(p->scale)) return "the scale is not a number";
+    if (!(std::fabs(p->scale) <= 1e30f)) return "the scale is not a number, or above 1e30";
     const int64_t heads = (int64_t)k->n_seqs * k->kv_heads, rows = (int64_t)p->n_new * (p->heads / k->kv_heads);
-    if (rows > (1 << 24) || (int64_t)p->n_new * k->kv_heads * 32 > INT32_MAX || heads * ((rows + 15) / 16) * 64 > INT32_MAX || heads * ((k->n_ctx + 63) / 64) > INT32_MAX) return "too many rows";
+    if (rows > (1 << 24) || rows * (p->heads / k->kv_heads) > UINT32_MAX || (int64_t)p->n_new * k->kv_heads * 32 > INT32_MAX || heads * ((rows + 15) / 16) * 64 > INT32_MAX || heads * ((k->n_ctx + 63) / 64) > INT32_MAX) return "too many rows";
     if (!k->n_seqs || !p->n_new) return nullptr;
     if (!p->q || !p->out || p->q == p->out) return "q and out are missing or the same";
     if (!p->k_new != !p->v_new) return "new keys and values come together";
