@@ -13,7 +13,7 @@
 namespace {
 typedef __bf16 b8 __attribute__((ext_vector_type(8)));
 typedef __bf16 b2 __attribute__((ext_vector_type(2)));
-constexpr int TILE = 16, ADAPT_SELF = 256;
+constexpr int TILE = 16, ADAPT_SELF = 64; // 253 tokens of 64 adapters: 57 us without a plan, 50 with one; 4 of 3: 11 and 17
 struct ad_args {
     const uint16_t *down, *up;
     const int32_t *rank, *ids;
@@ -22,7 +22,7 @@ struct ad_args {
     const float *base;
     float *out;
     long long N, K, KP, RP, ldx, ldo;
-    int n_slots, T, parts, vec;
+    int n_slots, T, parts, vec, columns; // columns of a work-group of the second product
     int32_t *order, *tiles; // the plan: tokens by adapter; [0] tiles, then (adapter, first, tokens) each
     float *h;               // [part][tile][RP][16]
 };
@@ -46,8 +46,8 @@ __device__ __forceinline__ int adapter_of(const ad_args &a, int t) { // -1: none
     const int i = a.ids[t];
     return i >= 0 && i < a.n_slots && a.rank[i] > 0 ? i : -1;
 }
-// The work-group's tile: its adapter (-2: no such tile), its tokens in tok[16].  Without a plan tile b belongs to token b where that is the first, 17th, 33rd .. of its adapter (T <= 256, a
-// thread a token).
+// The work-group's tile: its adapter (-2: no such tile), its tokens in tok[16].  Without a plan tile b belongs to token b where that is the first, 17th, 33rd .. of its adapter (T <= 64, a thread a
+// token).
 __device__ __forceinline__ int tile_of(const ad_args &a, int b, int *tok, int *n, int *sh) {
     const int tid = threadIdx.x;
     if (a.order) {
@@ -78,31 +78,55 @@ __device__ __forceinline__ int tile_of(const ad_args &a, int b, int *tok, int *n
     return me;
 }
 
-// the tokens by adapter: slot n_slots stands for none
-__global__ __launch_bounds__(1024) void adapt_plan_kernel(const ad_args a, int32_t *count) { // count [n_slots + 1]: global scratch
-    __shared__ int run[3];
-    const int tid = threadIdx.x, bins = a.n_slots + 1;
-    for (int i = tid; i < bins; i += 1024) __hip_atomic_store(&count[i], 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+// the tokens by adapter: slot n_slots stands for none.  count [n_slots + 1]: LDS where it has room, else global scratch.  Lanes of a wave that have the same adapter count as one: in a prompt they
+// all have (2048 tokens of 4 adapters: 69 us with an atomic a token).
+constexpr int PLAN_LDS = 8192;
+// The lanes of a wave that count for adapter i: those of the first two adapters found there together, the others each for itself.  f(adapter, lanes, whether this lane adds for them)
+template <class F> __device__ __forceinline__ void by_adapter(int i, bool there, F f) {
+    const int lane = threadIdx.x & 63;
+    unsigned long long todo = __ballot(there);
+#pragma unroll 1
+    for (int k = 0; k < 2 && todo; k++) {
+        const int one = __builtin_amdgcn_readlane(i, __ffsll(todo) - 1);
+        const unsigned long long same = __ballot(there && i == one) & todo;
+        if (same >> lane & 1) f(one, same);
+        todo &= ~same;
+    }
+    if (todo >> lane & 1) f(i, 1ull << lane);
+}
+__global__ __launch_bounds__(1024) void adapt_plan_kernel(const ad_args a, int32_t *spare) {
+    extern __shared__ int32_t in_lds[];
+    __shared__ int sc[16], st[16], run[2];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, bins = a.n_slots + 1;
+    const bool lds = bins <= PLAN_LDS;
+    auto add = [&](int i, int n) { return lds ? atomicAdd(&in_lds[i], n) : atomicAdd(&spare[i], n); };
+    auto get = [&](int i) { return lds ? in_lds[i] : __hip_atomic_load(&spare[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); };
+    auto set = [&](int i, int v) { if (lds) in_lds[i] = v; else __hip_atomic_store(&spare[i], v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); };
+    for (int i = tid; i < bins; i += 1024) set(i, 0);
+    if (tid < 2) run[tid] = 0;
     __syncthreads();
-    for (int t = tid; t < a.T; t += 1024) { const int i = adapter_of(a, t); atomicAdd(&count[i < 0 ? a.n_slots : i], 1); }
+    auto slot = [&](int t) { const int i = t < a.T ? adapter_of(a, t) : 0; return i < 0 ? a.n_slots : i; };
+    for (int t = tid; t - lane < a.T; t += 1024) by_adapter(slot(t), t < a.T, [&](int i, unsigned long long same) { if (lane == __ffsll(same) - 1) add(i, (int)__popcll(same)); });
     __syncthreads();
-    __shared__ int sc[1024], st[1024];
-    if (tid == 0) run[0] = run[1] = 0;
     for (int base = 0; base < bins; base += 1024) {
-        const int i = base + tid, c = i < bins ? __hip_atomic_load(&count[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0, nt = (c + TILE - 1) / TILE;
-        sc[tid] = c;
-        st[tid] = nt;
-        __syncthreads();
-        for (int o = 1; o < 1024; o <<= 1) {
-            const int x = tid >= o ? sc[tid - o] : 0, y = tid >= o ? st[tid - o] : 0;
-            __syncthreads();
-            sc[tid] += x;
-            st[tid] += y;
-            __syncthreads();
+        const int i = base + tid, c = i < bins ? get(i) : 0, nt = (c + TILE - 1) / TILE;
+        int x = c, y = nt;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const int u = __shfl_up(x, o, 64), v = __shfl_up(y, o, 64);
+            if (lane >= o) { x += u; y += v; }
         }
-        const int first = run[0] + sc[tid] - c, tile = run[1] + st[tid] - nt;
+        if (lane == 63) { sc[wave] = x; st[wave] = y; }
+        __syncthreads();
+        int before_c = run[0], before_t = run[1], all_c = 0, all_t = 0;
+        for (int w = 0; w < 16; w++) {
+            if (w < wave) { before_c += sc[w]; before_t += st[w]; }
+            all_c += sc[w];
+            all_t += st[w];
+        }
+        const int first = before_c + x - c, tile = before_t + y - nt;
         if (i < bins) {
-            __hip_atomic_store(&count[i], first, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            set(i, first);
             for (int k = 0; k < nt; k++) {
                 int32_t *t = a.tiles + 1 + 3 * (tile + k);
                 t[0] = i == a.n_slots ? -1 : i;
@@ -111,14 +135,17 @@ __global__ __launch_bounds__(1024) void adapt_plan_kernel(const ad_args a, int32
             }
         }
         __syncthreads();
-        if (tid == 1023) { run[0] += sc[1023]; run[1] += st[1023]; }
+        if (tid == 0) { run[0] += all_c; run[1] += all_t; }
         __syncthreads();
     }
     if (tid == 0) a.tiles[0] = run[1];
-    for (int t = tid; t < a.T; t += 1024) { // (the order of an adapter's tokens is nobody's business: a token's result does not depend on its tile)
-        const int i = adapter_of(a, t);
-        a.order[atomicAdd(&count[i < 0 ? a.n_slots : i], 1)] = t;
-    }
+    for (int t = tid; t - lane < a.T; t += 1024) // (the order of an adapter's tokens is nobody's business: a token's result does not depend on its tile)
+        by_adapter(slot(t), t < a.T, [&](int i, unsigned long long same) {
+            const int leader = __ffsll(same) - 1;
+            int at = lane == leader ? add(i, (int)__popcll(same)) : 0;
+            at = __shfl(at, leader, 64);
+            a.order[at + (int)__popcll(same & ((1ull << lane) - 1))] = t;
+        });
 }
 
 template <bool F32X>
@@ -138,6 +165,7 @@ __global__ __launch_bounds__(256) void adapt_down_kernel(const ad_args a) {
         pv_f4 h[4];
 #pragma unroll
         for (int r = 0; r < 4; r++) h[r] = (pv_f4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll 2
         for (long long s = s0 + wave; s < s1; s += 4) {
             const long long k = 32 * s + 8 * q4;
             pv_u4 p1, p2, p3;
@@ -194,13 +222,12 @@ __global__ __launch_bounds__(256) void adapt_up_kernel(const ad_args a) {
     int n;
     const int ad = tile_of(a, b, tok, &n, sh);
     if (ad == -2) return;
-    const long long n0 = (long long)blockIdx.y * 256 + wave * 64;
-    pv_f4 o[4];
-#pragma unroll
-    for (int e = 0; e < 4; e++) o[e] = (pv_f4){0.f, 0.f, 0.f, 0.f};
     float scale = 0.f;
+    int r16 = 0, ld = 0;
     if (ad >= 0) {
-        const int rank = a.rank[ad], r16 = (rank + 15) / 16 * 16, ld = 3 * r16 + 8;
+        const int rank = a.rank[ad];
+        r16 = (rank + 15) / 16 * 16;
+        ld = 3 * r16 + 8;
         scale = a.scale[ad];
         for (int i = tid; i < r16 * 8; i += 256) { // two ranks of a token
             const int t = i & 15, r = (i >> 4) * 2;
@@ -219,39 +246,48 @@ __global__ __launch_bounds__(256) void adapt_up_kernel(const ad_args a) {
             *(unsigned *)(hl + t * ld + 2 * r16 + r) = u3;
         }
         __syncthreads();
-        const uint16_t *up = a.up + (long long)ad * a.N * a.RP;
-        for (int k0 = 0; k0 < 3 * r16; k0 += 32) {
-            const int k = k0 + 8 * q4;
-            const bool there = k < 3 * r16;
-            const pv_u4 hv = there ? *(const pv_u4 *)(hl + c * ld + k) : (pv_u4){0, 0, 0, 0};
-            const int r = k % r16;
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const long long col = min(n0 + 4 * c + e, a.N - 1);
-                const pv_u4 u = there ? *(const pv_u4 *)(up + col * r16 + r) : (pv_u4){0, 0, 0, 0};
-                o[e] = mfma(hv, u, o[e]);
-            }
-        }
     }
-    const long long col = n0 + 4 * c;
+    const uint16_t *up = a.up + (long long)max(ad, 0) * a.N * a.RP;
+    const long long end = min(a.N, (long long)(blockIdx.y + 1) * a.columns);
+    for (long long n0 = (long long)blockIdx.y * a.columns + wave * 64; n0 < end; n0 += 256) {
+        const long long col = n0 + 4 * c;
+        pv_f4 o[4], v[4];
+        // base is on its way while the products are made
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const int t = 4 * q4 + i;
-        if (t >= n || col >= a.N) continue;
-        const long long at = tok[t] * a.ldo + col;
-        if (a.vec & 2) {
-            pv_f4 v = a.base ? *(const pv_f4 *)(a.base + at) : (pv_f4){0.f, 0.f, 0.f, 0.f};
-            if (ad >= 0) {
+        for (int i = 0; i < 4; i++) {
+            o[i] = v[i] = (pv_f4){0.f, 0.f, 0.f, 0.f};
+            const int t = 4 * q4 + i;
+            if ((a.vec & 2) && a.base && t < n && col < a.N) v[i] = *(const pv_f4 *)(a.base + tok[t] * a.ldo + col);
+        }
+        for (int r0 = 0; r0 < r16; r0 += 32) {
+            const int r = r0 + 8 * q4;
+            const bool there = r < r16;
+            pv_u4 u[4], hv[3];
 #pragma unroll
-                for (int e = 0; e < 4; e++) v[e] = fmaf(o[e][i], scale, v[e]);
-            }
-            *(pv_f4 *)(a.out + at) = v;
-        } else {
+            for (int e = 0; e < 4; e++) u[e] = there ? *(const pv_u4 *)(up + min(col + e, a.N - 1) * r16 + r) : (pv_u4){0, 0, 0, 0};
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-                if (col + e >= a.N) continue;
-                const float v = a.base ? a.base[at + e] : 0.f;
-                a.out[at + e] = ad >= 0 ? fmaf(o[e][i], scale, v) : v;
+            for (int x = 0; x < 3; x++) hv[x] = there ? *(const pv_u4 *)(hl + c * ld + x * r16 + r) : (pv_u4){0, 0, 0, 0};
+#pragma unroll
+            for (int x = 2; x >= 0; x--)
+#pragma unroll
+                for (int e = 0; e < 4; e++) o[e] = mfma(hv[x], u[e], o[e]);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int t = 4 * q4 + i;
+            if (t >= n || col >= a.N) continue;
+            const long long at = tok[t] * a.ldo + col;
+            if (a.vec & 2) {
+#pragma unroll
+                for (int e = 0; e < 4; e++) v[i][e] = ad >= 0 ? fmaf(o[e][i], scale, v[i][e]) : v[i][e];
+                *(pv_f4 *)(a.out + at) = v[i];
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    if (col + e >= a.N) continue;
+                    const float x = a.base ? a.base[at + e] : 0.f;
+                    a.out[at + e] = ad >= 0 ? fmaf(o[e][i], scale, x) : x;
+                }
             }
         }
     }
@@ -276,9 +312,12 @@ size_t psv_adapt_space(const ps_adapters &s, int x_dtype, const void *x, int64_t
     a.N = s.N; a.K = s.K; a.KP = s.KP; a.RP = s.RP; a.ldx = ldx; a.ldo = ldo; a.n_slots = s.n_slots; a.T = T;
     const int size = x_dtype == PS_F32 ? 4 : 2;
     a.vec = ((uintptr_t)x % 16 == 0 && ldx * size % 16 == 0 ? 1 : 0) | ((uintptr_t)out % 16 == 0 && (uintptr_t)base_out % 16 == 0 && ldo % 4 == 0 && s.N % 4 == 0 ? 2 : 0);
-    if (T > ADAPT_SELF) hipLaunchKernelGGL(adapt_plan_kernel, dim3(1), dim3(1024), 0, st, a, count);
+    if (T > ADAPT_SELF) hipLaunchKernelGGL(adapt_plan_kernel, dim3(1), dim3(1024), s.n_slots + 1 <= PLAN_LDS ? (size_t)(s.n_slots + 1) * 4 : 0, st, a, count);
     if (x_dtype == PS_F32) hipLaunchKernelGGL(adapt_down_kernel<true>, dim3(most, a.parts), dim3(256), 0, st, a);
     else hipLaunchKernelGGL(adapt_down_kernel<false>, dim3(most, a.parts), dim3(256), 0, st, a);
-    hipLaunchKernelGGL(adapt_up_kernel, dim3(most, (unsigned)((s.N + 255) / 256)), dim3(256), (size_t)TILE * (3 * s.RP + 8) * 2, st, a);
+    // 256 columns a work-group until the chip is full four times, then more
+    const int64_t stretches = (s.N + 255) / 256, groups = std::min<int64_t>(stretches, std::max<int64_t>(1, (16 * s.n_cu + most - 1) / most));
+    a.columns = (int)((stretches + groups - 1) / groups * 256);
+    hipLaunchKernelGGL(adapt_up_kernel, dim3(most, (unsigned)((s.N + a.columns - 1) / a.columns)), dim3(256), (size_t)TILE * (3 * s.RP + 8) * 2, st, a);
     return ws.at;
 }
