@@ -8,6 +8,7 @@
 #include <algorithm>
 
 namespace {
+typedef int i4 __attribute__((ext_vector_type(4)));
 constexpr int EV_THREADS = 1024, EV_LDS_KEYS = 32768;
 struct ev_args {
     char *k, *v;
@@ -27,31 +28,25 @@ __device__ __forceinline__ unsigned order_of(float w) {
     if ((u & 0x7fffffffu) > 0x7f800000u) return 0u;
     return min((u & 0x80000000u) ? ~u : u | 0x80000000u, 0xfffffffeu);
 }
-// sum over the threads before this one; *total: over all (sh: 17 numbers; barriers inside)
+// sums over a wave's lanes up to and with each
+template <int CTRL, int ROWS> __device__ __forceinline__ int moved(int v) { return __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 15, false); }
+__device__ __forceinline__ int wave_sums(int v) {
+    v += moved<0x111, 15>(v); // row_shr: 1, 2, 4, 8
+    v += moved<0x112, 15>(v);
+    v += moved<0x114, 15>(v);
+    v += moved<0x118, 15>(v);
+    v += moved<0x142, 10>(v); // row_bcast: 15 into rows 1 and 3, 31 into rows 2 and 3
+    v += moved<0x143, 12>(v);
+    return v;
+}
+// sum over the threads before this one; *total: over all (sh: 16 numbers; barriers inside)
 __device__ __forceinline__ int scan_before(int v, int *sh, int *total) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    int x = v;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const int y = __shfl_up(x, o, 64);
-        if (lane >= o) x += y;
-    }
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, x = wave_sums(v);
     if (lane == 63) sh[wave] = x;
     __syncthreads();
-    if (threadIdx.x < 64) {
-        int y = threadIdx.x < EV_THREADS / 64 ? sh[threadIdx.x] : 0;
-        const int own = y;
-#pragma unroll
-        for (int o = 1; o < EV_THREADS / 64; o <<= 1) {
-            const int z = __shfl_up(y, o, 64);
-            if (lane >= o) y += z;
-        }
-        if (threadIdx.x < EV_THREADS / 64) sh[threadIdx.x] = y - own;
-        if (threadIdx.x == EV_THREADS / 64 - 1) sh[16] = y;
-    }
-    __syncthreads();
-    const int before = sh[wave] + x - v;
-    *total = sh[16];
+    const int y = lane < EV_THREADS / 64 ? sh[lane] : 0, z = wave_sums(y);
+    *total = __builtin_amdgcn_readlane(z, 63);
+    const int before = __builtin_amdgcn_readlane(z - y, wave) + x - v;
     __syncthreads();
     return before;
 }
@@ -59,7 +54,8 @@ __device__ __forceinline__ int scan_before(int v, int *sh, int *total) {
 __global__ __launch_bounds__(EV_THREADS) void evict_choose_kernel(const ev_args a) {
     extern __shared__ unsigned keys[]; // in_lds: a key per held slot
     __shared__ unsigned hist[2048];
-    __shared__ int sh[17], counts[1024], pre[1024], cut[2], newest_;
+    __shared__ unsigned stay[EV_THREADS];
+    __shared__ int sh[16], cut[2], newest_;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, g = blockIdx.x, s = blockIdx.y;
     const long long head = (long long)s * a.G + g, at = head * a.n_ctx;
     const int n = min(max(a.n_kv[s], 0), a.n_ctx), keep = a.keep;
@@ -75,9 +71,34 @@ __global__ __launch_bounds__(EV_THREADS) void evict_choose_kernel(const ev_args 
         if (tid == 0) { a.meta[2 * head] = 0; a.meta[2 * head + 1] = n; }
         return;
     }
+    // four slots at a time where a head's numbers are 16-byte aligned, four such pieces of a thread in flight
+    const bool wide = a.n_ctx % 4 == 0 && ((uintptr_t)a.weight | (uintptr_t)a.pos) % 16 == 0;
+    auto load_pos = [&](int j) {
+        if (wide) return *(const i4 *)(p + j);
+        return (i4){p[j], p[min(j + 1, n - 1)], p[min(j + 2, n - 1)], p[min(j + 3, n - 1)]};
+    };
+    auto load_weight = [&](int j) {
+        if (wide) return *(const pv_f4 *)(w + j);
+        return (pv_f4){w[j], w[min(j + 1, n - 1)], w[min(j + 2, n - 1)], w[min(j + 3, n - 1)]};
+    };
+    constexpr int STEP = EV_THREADS * 4, AT_ONCE = 4 * STEP;
+    i4 v[4];
+    pv_f4 u[4];
+    const bool once = n <= AT_ONCE; // positions and weights of so many slots are loaded together, and once
     // the largest position
     int top = INT32_MIN;
-    for (int j = tid; j < n; j += EV_THREADS) top = max(top, p[j]);
+    for (int base = 4 * tid; base < n; base += AT_ONCE) {
+#pragma unroll
+        for (int x = 0; x < 4; x++) v[x] = load_pos(base + x * STEP < n ? base + x * STEP : base);
+        if (once)
+#pragma unroll
+            for (int x = 0; x < 4; x++) u[x] = load_weight(base + x * STEP < n ? base + x * STEP : base);
+#pragma unroll
+        for (int x = 0; x < 4; x++)
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                if (base + x * STEP + e < n) top = max(top, v[x][e]);
+    }
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) top = max(top, __shfl_xor(top, o, 64));
     if (tid == 0) newest_ = INT32_MIN;
@@ -86,19 +107,55 @@ __global__ __launch_bounds__(EV_THREADS) void evict_choose_kernel(const ev_args 
     if (lane == 0) atomicMax(&newest_, top);
     __syncthreads();
     const long long since = (long long)newest_ - a.recent; // positions above it are recent
-    auto key_of = [&](int j) { return p[j] < a.first || p[j] > since ? 0xffffffffu : order_of(w[j]); };
-    auto key = [&](int j) { return a.in_lds ? keys[j] : key_of(j); };
+    auto key_from = [&](int pos, float weight) { return pos < a.first || pos > since ? 0xffffffffu : order_of(weight); };
+    auto key = [&](int j) { return a.in_lds ? keys[j] : key_from(p[j], w[j]); };
+    // The first digit's histogram, and the keys into LDS.  Weights of 0 (most of a soft-max's) and protected slots are many of one key each: a thread counts its own, they would be additions to one
+    // place of the LDS one behind the other (16384 slots, a third of them 0: 10 us).
+    constexpr unsigned ZERO = 0x80000000u, KEPT = 0xffffffffu;
+    int zeros = 0, kept_ = 0;
+    auto count = [&](unsigned k, int shift, int bits) {
+        if (k == ZERO) zeros++;
+        else if (k == KEPT) kept_++;
+        else atomicAdd(&hist[k >> shift & ((1u << bits) - 1)], 1u);
+    };
+    auto settle = [&](int shift, int bits) { // what the threads have counted into the histogram
+        zeros = wave_sums(zeros);
+        kept_ = wave_sums(kept_);
+        if (lane == 63 && zeros) atomicAdd(&hist[ZERO >> shift & ((1u << bits) - 1)], (unsigned)zeros);
+        if (lane == 63 && kept_) atomicAdd(&hist[KEPT >> shift & ((1u << bits) - 1)], (unsigned)kept_);
+        zeros = kept_ = 0;
+    };
+    for (int base = 4 * tid; base < n; base += AT_ONCE) {
+        if (!once)
+#pragma unroll
+            for (int x = 0; x < 4; x++) {
+                const int j = base + x * STEP < n ? base + x * STEP : base;
+                v[x] = load_pos(j);
+                u[x] = load_weight(j);
+            }
+#pragma unroll
+        for (int x = 0; x < 4; x++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const int j = base + x * STEP + e;
+                if (j >= n) continue;
+                const unsigned k = key_from(v[x][e], u[x][e]);
+                if (a.in_lds) keys[j] = k;
+                count(k, 21, 11);
+            }
+    }
     // the keep-th largest key, digit by digit
     unsigned found = 0, mask = 0;
     int need = keep;
-#pragma unroll
+#pragma unroll 1
     for (int d = 0; d < 3; d++) {
         const int shift = d == 0 ? 21 : d == 1 ? 10 : 0, bits = d == 2 ? 10 : 11;
-        for (int j = tid; j < n; j += EV_THREADS) {
-            const unsigned x = d == 0 ? key_of(j) : key(j);
-            if (d == 0 && a.in_lds) keys[j] = x;
-            if ((x & mask) == found) atomicAdd(&hist[x >> shift & ((1u << bits) - 1)], 1u);
-        }
+        if (d)
+            for (int j = tid; j < n; j += EV_THREADS) {
+                const unsigned x = key(j);
+                if ((x & mask) == found) count(x, shift, bits);
+            }
+        settle(shift, bits);
         __syncthreads();
         // from the largest digit down: thread t has digits 2047 - 2 t and 2046 - 2 t
         const int hi = (int)hist[2047 - 2 * tid], lo = (int)hist[2046 - 2 * tid];
@@ -113,56 +170,48 @@ __global__ __launch_bounds__(EV_THREADS) void evict_choose_kernel(const ev_args 
         need = cut[1]; // of those that share the digits so far
         __syncthreads();
     }
-    // the walk: of the slots whose key is the one found, the first `need` stay
+    // the walk: of the slots whose key is the one found, the first `need` stay.  A thread has up to 32 slots in a row, a bit each.
     int ties = 0, holes = 0, moves = 0;
     int32_t *hole = a.hole + head * a.cap, *moved = a.moved + head * a.cap;
-    const unsigned long long below = (1ull << lane) - 1;
-    for (int base = 0; base < n; base += 65536) {
-        const int nb = min(1024, (n - base + 63) / 64);
-        for (int b = wave; b < nb; b += EV_THREADS / 64) {
-            const int j = base + 64 * b + lane;
-            const unsigned long long eq = __ballot(j < n && key(min(j, n - 1)) == found);
-            if (lane == 0) counts[b] = __popcll(eq);
+    for (int base = 0; base < n; base += EV_LDS_KEYS) {
+        const int end = min(n, base + EV_LDS_KEYS), per = (end - base + EV_THREADS - 1) / EV_THREADS, j0 = base + tid * per;
+        unsigned gt = 0, eq = 0;
+        int i = tid % per; // (each begins elsewhere: 32 lanes would read one LDS bank)
+        for (int x = 0; x < per; x++, i = i + 1 == per ? 0 : i + 1) {
+            if (j0 + i >= end) continue;
+            const unsigned k = key(j0 + i);
+            gt |= (k > found ? 1u : 0u) << i;
+            eq |= (k == found ? 1u : 0u) << i;
         }
-        __syncthreads();
         int all;
-        const int t0 = ties + scan_before(tid < nb ? counts[tid] : 0, sh, &all);
-        pre[tid] = t0;
+        int room = need - (ties + scan_before((int)__popc(eq), sh, &all));
         ties += all;
-        __syncthreads();
-        auto stays = [&](int b, int j) {
-            const unsigned x = key(min(j, n - 1));
-            const unsigned long long eq = __ballot(j < n && x == found);
-            return j < n && (x > found || (x == found && pre[b] + (int)__popcll(eq & below) < need));
-        };
-        for (int b = wave; b < nb; b += EV_THREADS / 64) {
-            const int j = base + 64 * b + lane;
-            const bool kept = stays(b, j);
-            const int h = __popcll(__ballot(j < n && j < keep && !kept)), m = __popcll(__ballot(kept && j >= keep));
-            if (lane == 0) counts[b] = h << 8 | m;
-        }
-        __syncthreads();
-        const int c = tid < nb ? counts[tid] : 0;
-        int all_h, all_m;
-        const int h0 = holes + scan_before(c >> 8, sh, &all_h), m0 = moves + scan_before(c & 255, sh, &all_m);
-        counts[tid] = h0;
-        hist[tid] = (unsigned)m0;
-        holes += all_h;
-        moves += all_m;
-        __syncthreads();
-        for (int b = wave; b < nb; b += EV_THREADS / 64) {
-            const int j = base + 64 * b + lane;
-            const bool kept = stays(b, j);
-            const bool h = j < n && j < keep && !kept, m = kept && j >= keep;
-            const unsigned long long hb = __ballot(h), mb = __ballot(m);
-            if (h) hole[counts[b] + (int)__popcll(hb & below)] = j;
-            if (m) moved[(int)hist[b] + (int)__popcll(mb & below)] = j;
-            if (kept && j < keep) {
-                if (wo) wo[j] = w[j];
-                if (po) po[j] = p[j];
+        unsigned kept = gt;
+        if (room >= (int)__popc(eq)) kept |= eq;
+        else
+            for (; room > 0; room--) { // its lowest ones
+                kept |= eq & -eq;
+                eq &= eq - 1;
             }
+        auto ones = [](int k) { return k >= 32 ? ~0u : k <= 0 ? 0u : (1u << k) - 1; };
+        const unsigned there = ones(min(per, end - j0)), below = ones(keep - j0);
+        unsigned h = there & below & ~kept, m = there & kept & ~below;
+        const int before = scan_before((int)(__popc(h) << 16 | __popc(m)), sh, &all); // (at most 32768 each)
+        int hi = holes + (int)((unsigned)before >> 16), mi = moves + (before & 0xffff);
+        holes += (int)((unsigned)all >> 16);
+        moves += all & 0xffff;
+        for (; h; h &= h - 1) hole[hi++] = j0 + __ffs(h) - 1;
+        for (; m; m &= m - 1) moved[mi++] = j0 + __ffs(m) - 1;
+        if (wo || po) { // what stays where it is, into the caller's new arrays
+            stay[tid] = kept;
+            __syncthreads();
+            for (int j = base + tid; j < min(end, keep); j += EV_THREADS)
+                if (stay[(j - base) / per] >> ((j - base) % per) & 1) {
+                    if (wo) wo[j] = w[j];
+                    if (po) po[j] = p[j];
+                }
+            __syncthreads();
         }
-        __syncthreads();
     }
     if (tid == 0) { a.meta[2 * head] = moves; a.meta[2 * head + 1] = keep; }
 }
