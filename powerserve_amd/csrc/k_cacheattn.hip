@@ -40,6 +40,8 @@ struct ca_args {
     float *score; // [seq][kv head][slot][score_rows]: scores of few rows for the weights, or NULL
     float *lse;  // [seq][kv head][T R] log2 of the sum of weights (+inf: no weights)
     int parts, tiles, score_rows; // tiles of 16 rows
+    int share, *chunks; // few rows of up to 256 sequences: work-groups that all their keys are shared out to, and keys of a part of each sequence; else 0, NULL
+    int plain; // offsets within 32 slots fit 32 bits
     int wparts;       // parts of the rows that the weights are summed in
     float *wpart;     // [seq][kv head][part][slot]
 };
@@ -52,7 +54,11 @@ __device__ __forceinline__ ca_lens lens_of(const ca_args &a, int s) {
     l.len = l.n0 + l.cnt;
     return l;
 }
-__device__ __forceinline__ int chunk_of(int len, int parts) { return max(128, ((len + parts - 1) / parts + 127) / 128 * 128); }
+// keys of a part of sequence s
+__device__ __forceinline__ int chunk_of(const ca_args &a, int s, int len) {
+    if (a.chunks) return a.chunks[s];
+    return max(128, ((len + a.parts - 1) / a.parts + 127) / 128 * 128);
+}
 __device__ __forceinline__ bool sees(const ca_args &a, int s, int t, int u) { return a.tree ? a.tree[((long long)s * a.T + t) * a.T + u] != 0 : u <= t; }
 
 template <class E> __device__ __forceinline__ pv_f4 mfma(const pv_u4 &x, const pv_u4 &y, const pv_f4 &c);
@@ -120,15 +126,63 @@ __global__ __launch_bounds__(256, E::SIZE == 4 ? 1 : 2) void cache_attn_kernel(c
     constexpr int VBYTES = E::SIZE == 2 ? 4 * 32 * VR * 2 : 0, OBYTES = 4 * 16 * OP * 4;
     __shared__ __attribute__((aligned(16))) char lds[VBYTES > OBYTES ? VBYTES : OBYTES];
     __shared__ float lm[4][16], ll[4][16];
-    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, c = lane & 15, q4 = lane >> 4;
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, c = lane & 15, q4 = lane >> 4;
     const int blocks = (a.tiles + RT - 1) / RT;
+    // Parts of a step's work, all of much the same size: the keys of all sequences shared out, so that one long sequence among short ones does not keep a few work-groups busy and none is started
+    // for slots that nobody holds.  Every work-group finds the same plan from the lengths (a thread a sequence).
+    __shared__ int before[257], chunk_at[256];
+    int items = a.n_seqs * a.G * a.parts * blocks;
+    if (a.share) {
+        __shared__ int sums[4];
+        const ca_lens mine = tid < a.n_seqs ? lens_of(a, tid) : ca_lens{0, 0, 0};
+        const int len = mine.cnt ? mine.len : 0;
+        int x = len;
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) x += __shfl_xor(x, o, 64);
+        if (lane == 0) sums[wave] = x;
+        __syncthreads();
+        const long long all = (long long)sums[0] + sums[1] + sums[2] + sums[3], even = (all * a.G * blocks + a.share - 1) / a.share;
+        const int chunk = (int)((max(even, (long long)((len + a.parts - 1) / a.parts)) + 127) / 128 * 128), n = len ? (len + max(chunk, 128) - 1) / max(chunk, 128) : 0;
+        chunk_at[tid] = max(chunk, 128);
+        if (blockIdx.x == 0 && tid < a.n_seqs) a.chunks[tid] = max(chunk, 128);
+        x = n;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const int y = __shfl_up(x, o, 64);
+            if (lane >= o) x += y;
+        }
+        __syncthreads();
+        if (lane == 63) sums[wave] = x;
+        __syncthreads();
+        for (int i = 0; i < wave; i++) x += sums[i];
+        before[tid + 1] = x;
+        if (tid == 0) before[0] = 0;
+        __syncthreads();
+        items = before[256] * a.G * blocks;
+    }
     int id = blockIdx.x;
+    if (id >= items) return;
     const int rb = id % blocks; id /= blocks;
-    const int split = id % a.parts; id /= a.parts;
-    const int g = id % a.G, s = id / a.G;
+    int g, s, split, chunk;
+    if (a.share) {
+        g = id % a.G; id /= a.G;
+        int lo = 0, hi = a.n_seqs - 1; // the last sequence whose parts begin at id or before
+        while (lo < hi) {
+            const int m = (lo + hi + 1) / 2;
+            if (before[m] <= id) lo = m;
+            else hi = m - 1;
+        }
+        s = lo;
+        split = id - before[s];
+    } else {
+        split = id % a.parts; id /= a.parts;
+        g = id % a.G;
+        s = id / a.G;
+    }
     const ca_lens L = lens_of(a, s);
-    const int chunk = chunk_of(L.len, a.parts), k0 = split * chunk, k1 = min(L.len, k0 + chunk);
-    if (L.cnt == 0 || (k0 >= L.len && split > 0) || rb * RT * 16 >= L.cnt * a.R) return;
+    chunk = a.share ? chunk_at[s] : chunk_of(a, s, L.len);
+    const int k0 = split * chunk, k1 = min(L.len, k0 + chunk);
+    if (L.cnt == 0 || k0 >= L.len || rb * RT * 16 >= L.cnt * a.R) return;
     const char *kb_ = a.k + s * a.seq + g * a.head, *vb_ = a.v + s * a.seq + g * a.head;
     const char *kn = a.k_new ? a.k_new + s * a.new_seq + (long long)g * a.dim * E::SIZE : nullptr, *vn = a.k_new ? a.v_new + s * a.new_seq + (long long)g * a.dim * E::SIZE : nullptr;
     auto row_at = [&](const char *held, const char *fresh, int j) { return fresh && j >= L.n0 ? fresh + (j - L.n0) * a.new_row : held + j * a.slot; };
@@ -154,7 +208,22 @@ __global__ __launch_bounds__(256, E::SIZE == 4 ? 1 : 2) void cache_attn_kernel(c
     constexpr int LPR = DP / 8, RPI = 64 / LPR, VI = E::SIZE == 2 ? 32 / RPI : 8 * (DP / 64);
     pv_u4 kf[2][NS], vf[VI];
     const int vr = lane / LPR, vc = lane % LPR * 8;
+    constexpr int ES = E::SIZE;
+    const unsigned ko = c * (unsigned)a.slot + q4 * 16, vo = ES == 2 ? vr * (unsigned)a.slot + vc * 2 : 4 * q4 * (unsigned)a.slot + c * 16;
     auto fetch = [&](int kb) {
+        if (RT == 1 && kb + 32 <= L.n0 && kb + 32 <= k1 && a.plain && a.dim == DP) { // slots that were held: one place a wave, and an offset a lane
+            const char *kt = kb_ + kb * a.slot, *vt = vb_ + kb * a.slot;
+#pragma unroll
+            for (int u = 0; u < 2; u++)
+#pragma unroll
+                for (int st = 0; st < NS; st++) kf[u][st] = *(const pv_u4 *)(kt + 16 * u * a.slot + 64 * st + ko);
+#pragma unroll
+            for (int i = 0; i < VI; i++) {
+                const int r = ES == 2 ? i * RPI : 16 * (i / (4 * (DP / 64))) + i / (DP / 64) % 4;
+                vf[i] = *(const pv_u4 *)(vt + r * a.slot + (ES == 2 ? 0 : 256 * (i % (DP / 64))) + vo);
+            }
+            return;
+        }
 #pragma unroll
         for (int u = 0; u < 2; u++) {
             const int j = min(kb + 16 * u + c, k1 - 1);
@@ -356,7 +425,7 @@ __global__ __launch_bounds__(256) void cache_join_kernel(const ca_args a) {
     const int g = id % a.G, s = id / a.G, rr = threadIdx.x >> 4, row = tile * 16 + rr;
     const ca_lens L = lens_of(a, s);
     if (tile * 16 >= L.cnt * a.R) return;
-    const int chunk = chunk_of(L.len, a.parts), n = (L.len + chunk - 1) / chunk, t = token_of(a, row), hd = g * a.R + row - t * a.R;
+    const int chunk = chunk_of(a, s, L.len), n = (L.len + chunk - 1) / chunk, t = token_of(a, row), hd = g * a.R + row - t * a.R;
     const long long step = 16 * (a.dim + 2);
     const float *part = a.part + (((long long)s * a.G + g) * a.tiles + tile) * a.parts * step;
     if (threadIdx.x < 64) { // four lanes a row
@@ -536,7 +605,7 @@ __global__ __launch_bounds__(256, 2) void cache_rows_kernel(const ca_args a) {
     const int heads = a.n_seqs * a.G, hs = id % heads, s = hs / a.G, g = hs - s * a.G; id /= heads;
     const int split = id % a.parts, p = id / a.parts, half = (blocks + 1) / 2, rb = p < half ? blocks - 1 - p : p - half;
     const ca_lens L = lens_of(a, s);
-    const int rows = L.cnt * a.R, chunk = chunk_of(L.len, a.parts), k0 = split * chunk, k1 = min(L.len, k0 + chunk);
+    const int rows = L.cnt * a.R, chunk = chunk_of(a, s, L.len), k0 = split * chunk, k1 = min(L.len, k0 + chunk);
     if (rb * ROWS >= rows || k0 >= L.len) return;
     const int r0 = rb * ROWS + wave * 32, row = min(r0 + c, rows - 1), tok = token_of(a, row), first = token_of(a, min(r0, rows - 1));
     const int kend = a.tree ? k1 : min(k1, L.n0 + token_of(a, min(rb * ROWS + ROWS - 1, rows - 1)) + 1); // behind the last key that a row of the work-group sees
@@ -869,8 +938,9 @@ void launch_attn(const ca_args &a, bool many, hipStream_t st) {
         }
     }
     // two tiles of rows a wave where there are two: its keys are read once for both
-    if (a.tiles > 1) hipLaunchKernelGGL((cache_attn_kernel<E, DP, 2>), dim3((unsigned)(heads * a.parts * ((a.tiles + 1) / 2))), dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((cache_attn_kernel<E, DP, 1>), dim3((unsigned)(heads * a.parts)), dim3(256), 0, st, a);
+    const unsigned grid = (unsigned)(a.share ? a.share + heads * ((a.tiles + 1) / 2) : heads * a.parts * ((a.tiles + 1) / 2)); // (shared out: a sequence's last part may be a short one)
+    if (a.tiles > 1) hipLaunchKernelGGL((cache_attn_kernel<E, DP, 2>), dim3(grid), dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((cache_attn_kernel<E, DP, 1>), dim3(grid), dim3(256), 0, st, a);
     if (a.parts > 1) hipLaunchKernelGGL((cache_join_kernel<E>), dim3((unsigned)(heads * a.tiles)), dim3(256), 0, st, a);
     if (!a.weight_out) return;
     if (a.tiles <= 2) hipLaunchKernelGGL(cache_score_kernel, dim3((unsigned)(heads * ((a.n_ctx + SCORE_KEYS - 1) / SCORE_KEYS))), dim3(256), 0, st, a);
@@ -886,11 +956,16 @@ size_t psv_attn_space(int n_cu, const ps_kv_cache &c, const ps_cache_attn_params
     // more than 32 rows of a 16-bit cache: 128 rows a work-group
     const bool many = size == 2 && rows > 32;
     const long long groups = heads * (many ? (rows + ROWS - 1) / ROWS : (a.tiles + 1) / 2);
-    a.parts = (int)std::min<long long>({std::max<long long>(((many ? 1 : 3) * n_cu + groups - 1) / groups, many ? 1 : (c.n_ctx + 1023) / 1024), (c.n_ctx + 127) / 128, 64});
+    a.parts = (int)std::min<long long>({std::max<long long>(((many ? 1 : 3) * n_cu + groups - 1) / groups, many ? 1 : (c.n_ctx + 511) / 512), (c.n_ctx + 127) / 128, 64});
+    a.plain = c.slot_stride >= 0 && c.slot_stride < (1 << 24);
     ps_carve ws{(char *)base};
     a.lse = ws.take<float>((size_t)(heads * rows));
     if (a.parts > 1) a.part = ws.take<float>((size_t)(heads * a.tiles * a.parts * 16 * (c.dim + 2)));
     a.score_rows = (int)((rows + 3) / 4 * 4);
+    if (!many && a.parts > 1 && c.n_seqs > 1 && c.n_seqs <= 256) {
+        a.share = 4 * n_cu;
+        a.chunks = ws.take<int>(c.n_seqs);
+    }
     if (p.weight_out && a.tiles <= 2) a.score = ws.take<float>((size_t)(heads * c.n_ctx * a.score_rows));
     a.wparts = 1;
     if (many && p.weight_out) { // parts of the rows until the chip is full twice, 128 rows at least
