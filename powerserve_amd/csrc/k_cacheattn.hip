@@ -30,7 +30,7 @@ struct ca_args {
     long long seq, slot, head, q_seq, q_row, o_seq, o_row, new_seq, new_row; // strides in bytes
     int n_seqs, n_ctx, G, dim, R, T;
     unsigned by_R; // 2^32 / R, rounded up: what a row of fewer than 2^32 / R is divided with (R 1: 0)
-    float sc2; // scale * log2(e): scores are held in units of log 2
+    float sc2; // scale, times log2(e) where scores are held in units of log 2
     const int32_t *n_kv, *count, *pos_new;
     int32_t *pos;
     const uint8_t *tree;
@@ -38,7 +38,7 @@ struct ca_args {
     float *weight_out;
     float *part; // [seq][kv head][16 rows][part]: 16 x dim results, 16 maxima, 16 sums
     float *score; // [seq][kv head][slot][score_rows]: scores of few rows for the weights, or NULL
-    float *lse;  // [seq][kv head][T R] log2 of the sum of weights (+inf: no weights)
+    float *lse;  // [seq][kv head][T R] logarithm, in the scores' units, of the sum of weights (+inf: no weights)
     int parts, tiles, score_rows; // tiles of 16 rows
     int share, *chunks; // few rows of up to 256 sequences: work-groups that all their keys are shared out to, and keys of a part of each sequence; else 0, NULL
     int plain; // offsets within 32 slots fit 32 bits
@@ -86,6 +86,16 @@ template <class E> __device__ __forceinline__ unsigned without_odd(unsigned u) {
     constexpr unsigned m = __is_same(E, BF16) ? 0x7f80u : 0x7c00u;
     return ((u & m) == m ? 0u : u & 0xffffu) | ((u >> 16 & m) == m ? 0u : u & 0xffff0000u);
 }
+// Scores of 16-bit caches are held in units of log 2, and 2^x is the instruction's.  Those of fp32 caches are as they are, and e^x is 2^(x log2 e) with what the product rounds off put back: 2^-23 of
+// it, where the instruction alone would have 2^-24 of the exponent.
+template <class E> __device__ __forceinline__ float ex(float x) {
+    if constexpr (E::SIZE == 2) return __builtin_amdgcn_exp2f(x);
+    else {
+        const float y = x * 1.44269504f, lo = fmaf(x, 1.44269504f, -y) + x * 1.92596299e-8f, e = __builtin_amdgcn_exp2f(y);
+        return x < -104.f ? 0.f : fmaf(e, lo * 0.693147181f, e);
+    }
+}
+template <class E> __device__ __forceinline__ float lg(float x) { return E::SIZE == 2 ? log2f(x) : logf(x); }
 __device__ __forceinline__ bool odd32(float v) { return (__float_as_uint(v) & 0x7f800000u) == 0x7f800000u; }
 template <class E> __device__ __forceinline__ float number(const char *p) {
     if constexpr (E::SIZE == 4) return *(const float *)p;
@@ -308,13 +318,13 @@ __global__ __launch_bounds__(256, E::SIZE == 4 ? 1 : 2) void cache_attn_kernel(c
             }
             top = fmaxf(top, __shfl_xor(top, 16, 64));
             top = fmaxf(top, __shfl_xor(top, 32, 64));
-            const float mn = fmaxf(m[r], top), ms = mn == -INFINITY ? 0.f : mn, al = __builtin_amdgcn_exp2f(m[r] - ms);
+            const float mn = fmaxf(m[r], top), ms = mn == -INFINITY ? 0.f : mn, al = ex<E>(m[r] - ms);
             float p[8], sum = 0.f;
 #pragma unroll
             for (int u = 0; u < 2; u++)
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
-                    p[4 * u + i] = __builtin_amdgcn_exp2f(z[r][u][i] - ms);
+                    p[4 * u + i] = ex<E>(z[r][u][i] - ms);
                     sum += p[4 * u + i];
                 }
             m[r] = mn;
@@ -379,7 +389,7 @@ __global__ __launch_bounds__(256, E::SIZE == 4 ? 1 : 2) void cache_attn_kernel(c
         float top = fmaxf(fmaxf(lm[0][rr], lm[1][rr]), fmaxf(lm[2][rr], lm[3][rr])), f[4], sum = 0.f;
         const float ms = top == -INFINITY ? 0.f : top;
 #pragma unroll
-        for (int w = 0; w < 4; w++) { f[w] = __builtin_amdgcn_exp2f(lm[w][rr] - ms); sum = fmaf(ll[w][rr], f[w], sum); }
+        for (int w = 0; w < 4; w++) { f[w] = ex<E>(lm[w][rr] - ms); sum = fmaf(ll[w][rr], f[w], sum); }
         const int t = token_of(a, row), hd = g * a.R + row - t * a.R;
         float *part = a.part + ((((long long)s * a.G + g) * a.tiles + tile) * a.parts + split) * (16 * (a.dim + 2));
         const float inv = sum == 0.f ? 0.f : 1.f / sum;
@@ -410,7 +420,7 @@ __global__ __launch_bounds__(256, E::SIZE == 4 ? 1 : 2) void cache_attn_kernel(c
         }
         if ((tid & 15) == 0) {
             if (a.parts > 1) { part[16 * a.dim + rr] = top; part[16 * a.dim + 16 + rr] = sum; }
-            else a.lse[((long long)s * a.G + g) * a.T * a.R + row] = sum == 0.f ? INFINITY : ms + log2f(sum);
+            else a.lse[((long long)s * a.G + g) * a.T * a.R + row] = sum == 0.f ? INFINITY : ms + lg<E>(sum);
         }
     }
 }
@@ -436,7 +446,7 @@ __global__ __launch_bounds__(256) void cache_join_kernel(const ca_args a) {
         top = fmaxf(top, __shfl_xor(top, 32, 64));
         const float ms = top == -INFINITY ? 0.f : top;
         for (int i = first; i < n; i += 4) {
-            const float m = part[i * step + 16 * a.dim + r], x = __builtin_amdgcn_exp2f(m - ms);
+            const float m = part[i * step + 16 * a.dim + r], x = ex<E>(m - ms);
             sum = fmaf(part[i * step + 16 * a.dim + 16 + r], x, sum);
             f[i][r] = m == -INFINITY ? 0.f : x; // (no result is left there)
         }
@@ -444,7 +454,7 @@ __global__ __launch_bounds__(256) void cache_join_kernel(const ca_args a) {
         sum += __shfl_xor(sum, 32, 64);
         if (first == 0) {
             total[r] = sum;
-            if (tile * 16 + r < L.cnt * a.R) a.lse[((long long)s * a.G + g) * a.T * a.R + tile * 16 + r] = sum == 0.f ? INFINITY : ms + log2f(sum);
+            if (tile * 16 + r < L.cnt * a.R) a.lse[((long long)s * a.G + g) * a.T * a.R + tile * 16 + r] = sum == 0.f ? INFINITY : ms + lg<E>(sum);
         }
     }
     __syncthreads();
@@ -467,6 +477,7 @@ __global__ __launch_bounds__(256) void cache_join_kernel(const ca_args a) {
 
 // the weights of few rows from the scores that the attention has left, a thread a key
 constexpr int SCORE_KEYS = 1024;
+template <class E>
 __global__ __launch_bounds__(256) void cache_score_kernel(const ca_args a) {
     const int blocks = (a.n_ctx + SCORE_KEYS - 1) / SCORE_KEYS;
     int id = blockIdx.x;
@@ -485,7 +496,7 @@ __global__ __launch_bounds__(256) void cache_score_kernel(const ca_args a) {
         for (int row = 0; row < rows; row += 4) {
             const pv_f4 z = *(const pv_f4 *)(a.score + at * pitch + row);
 #pragma unroll
-            for (int i = 0; i < 4; i++) w += lse[row + i] == INFINITY ? 0.f : __builtin_amdgcn_exp2f(z[i] - lse[row + i]);
+            for (int i = 0; i < 4; i++) w += lse[row + i] == INFINITY ? 0.f : ex<E>(z[i] - lse[row + i]);
         }
         a.weight_out[at] = j < L.n0 && a.weight ? a.weight[at] + w : w;
     }
@@ -525,7 +536,7 @@ __global__ __launch_bounds__(256) void cache_weight_kernel(const ca_args a) {
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
                     const int j = kb + 16 * u + 4 * q4 + i;
-                    const float p = ls == INFINITY ? 0.f : __builtin_amdgcn_exp2f(fmaf(z[i], a.sc2, -ls));
+                    const float p = ls == INFINITY ? 0.f : ex<E>(z[i] * a.sc2 - ls);
                     if (kb + 64 <= L.n0 || (j < L.len && (j < L.n0 || sees(a, s, t, j - L.n0)))) w[u][i] += p;
                 }
             }
@@ -943,7 +954,7 @@ void launch_attn(const ca_args &a, bool many, hipStream_t st) {
     else hipLaunchKernelGGL((cache_attn_kernel<E, DP, 1>), dim3(grid), dim3(256), 0, st, a);
     if (a.parts > 1) hipLaunchKernelGGL((cache_join_kernel<E>), dim3((unsigned)(heads * a.tiles)), dim3(256), 0, st, a);
     if (!a.weight_out) return;
-    if (a.tiles <= 2) hipLaunchKernelGGL(cache_score_kernel, dim3((unsigned)(heads * ((a.n_ctx + SCORE_KEYS - 1) / SCORE_KEYS))), dim3(256), 0, st, a);
+    if (a.tiles <= 2) hipLaunchKernelGGL((cache_score_kernel<E>), dim3((unsigned)(heads * ((a.n_ctx + SCORE_KEYS - 1) / SCORE_KEYS))), dim3(256), 0, st, a);
     else if constexpr (E::SIZE == 4) hipLaunchKernelGGL((cache_weight_kernel<E, DP>), dim3((unsigned)(heads * ((a.n_ctx + 63) / 64))), dim3(256), 0, st, a);
 }
 } // namespace
@@ -980,7 +991,7 @@ size_t psv_attn_space(int n_cu, const ps_kv_cache &c, const ps_cache_attn_params
     a.new_seq = p.new_seq_stride * size; a.new_row = p.new_row_stride * size;
     a.n_seqs = c.n_seqs; a.n_ctx = c.n_ctx; a.G = c.kv_heads; a.dim = c.dim; a.R = R; a.T = p.n_new;
     a.by_R = R == 1 ? 0 : (unsigned)((((unsigned long long)1 << 32) + R - 1) / R);
-    a.sc2 = p.scale == 0.f ? 1e-37f : p.scale * 1.44269504088896340736f; // (never 0: a masked score is minus infinity times it)
+    a.sc2 = p.scale == 0.f ? 1e-37f : size == 4 ? p.scale : p.scale * 1.44269504088896340736f; // (never 0: a masked score is minus infinity times it)
     a.n_kv = c.n_kv; a.count = p.count; a.pos_new = p.pos_new; a.pos = c.pos; a.tree = p.tree; a.weight = c.weight; a.weight_out = p.weight_out;
     if (c.dtype == PS_F32) c.dim > 64 ? launch_attn<F32, 128>(a, many, st) : launch_attn<F32, 64>(a, many, st);
     else if (c.dtype == PS_F16) c.dim > 64 ? launch_attn<F16, 128>(a, many, st) : launch_attn<F16, 64>(a, many, st);
