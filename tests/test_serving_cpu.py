@@ -1,0 +1,195 @@
+"""The entries of a serving step of many sequences on the host, without a GPU (tests/fake_hip.cpp in front of the library): what they refuse, before anything is enqueued, what the workspace functions say, on which
+device they launch, and the adapters' memory."""
+from test_host_calls import child, fake  # noqa: F401  (fixtures)
+
+MADE = """
+ctx = hip.Ctx(0)
+a = lambda n=64: ctx.malloc(n)
+def cache(dtype=1, S=2, n_ctx=64, G=2, dim=64, pos=True, weight=True, strides=None):
+    return hip.kv_cache(dtype, a(), a(), a(), S, n_ctx, G, dim, pos=a() if pos else None, weight=a() if weight else None, strides=strides)
+def attn(heads=4, new=3, scale=0.125, **k):
+    return hip.cache_attn_args(a(), a(), heads, new, scale, **k)
+space = a(1 << 20)
+def quiet(f):  # refused, and nothing enqueued
+    fake.fake_reset()
+    why = refused(f)
+    assert count("hipLaunchKernel") == count("hipMemcpy") == count("hipMemset") == 0, why
+    return why
+"""
+
+
+def test_attention_refuses_what_it_cannot_do(child):  # noqa: F811
+    child(MADE + """
+def go(c, p, ws=space, n=1 << 20): return quiet(lambda: ctx.cache_attn(c, p, ws, n))
+assert "type" in go(cache(dtype=8), attn())
+for dim in (0, 4, 12, 136, 256): assert "size" in go(cache(dim=dim), attn())
+for n_ctx in (0, -1, (1 << 28) + 1): go(cache(n_ctx=n_ctx), attn())
+assert "slots" in go(cache(G=0), attn())
+assert "many" in go(cache(S=65536), attn())
+assert "aligned" in go(cache(strides=(8192, 132, 64)), attn()) and "aligned" in go(cache(strides=(8192, 128, 4)), attn()) and "aligned" in go(cache(strides=(8190, 128, 64)), attn())
+for heads in (0, 3, -2): assert "query heads" in go(cache(), attn(heads=heads))
+for new in (-1, 65): assert "new tokens" in go(cache(), attn(new=new))
+for scale in (float("nan"), float("inf"), 2e30): assert "scale" in go(cache(), attn(scale=scale))
+c = cache(); c.k = None
+assert "missing" in go(c, attn())
+c = cache(); c.v = c.k
+assert "same" in go(c, attn())
+c = cache(); c.n_kv = None
+assert "missing" in go(c, attn())
+c = cache(); c.k += 8
+assert "aligned" in go(c, attn())
+p = attn(); p.out = p.q
+assert "same" in go(cache(), p)
+p = attn(); p.q = None
+assert "missing" in go(cache(), p)
+assert "together" in go(cache(), attn(k_new=a())) and "together" in go(cache(), attn(v_new=a()))
+assert "positions" in go(cache(pos=False), attn(pos_new=a()))
+for i in range(6):
+    assert "aligned" in go(cache(), attn(strides=[4 if i == j else 0 for j in range(6)])), i
+p = attn(); p.q += 4
+assert "aligned" in go(cache(), p)
+need = ctx.cache_attn_workspace(cache(), attn())
+assert need > 0
+for ws, n in ((None, need), (space, need - 1), (space + 8, need), (space, 0)): assert "workspace" in go(cache(), attn(), ws, n)
+assert "many" in go(cache(S=60000, n_ctx=1 << 27), attn(new=1 << 20))
+fake.fake_reset()
+ctx.cache_attn(cache(), attn(), space, need)
+assert count("hipLaunchKernel") > 0
+# nothing to do is no error
+fake.fake_reset()
+ctx.cache_attn(cache(), attn(new=0), None, 0)
+ctx.cache_attn(cache(S=0), attn(), None, 0)
+assert count("hipLaunchKernel") == 0 and ctx.cache_attn_workspace(cache(), attn(new=0)) == ctx.cache_attn_workspace(cache(dim=12), attn()) == 0
+quiet(lambda: ctx.cache_advance(cache(), None))
+quiet(lambda: ctx.cache_advance(cache(), a(), a(), -1))
+""")
+
+
+def test_eviction_refuses_what_it_cannot_do(child):  # noqa: F811
+    child(MADE + """
+def go(c, p, ws=space, n=1 << 20): return quiet(lambda: ctx.cache_evict(c, p, ws, n))
+for keep, recent, first in ((0, 0, 0), (-1, 0, 0), (5, 6, 0), (5, 3, 3), (5, -1, 0), (5, 0, -1), (2**31 - 1, 2**31 - 1, 2**31 - 1)):
+    assert "keep" in go(cache(), hip.cache_evict_args(keep, recent, first))
+assert "positions" in go(cache(pos=False), hip.cache_evict_args(8)) and "positions" in go(cache(weight=False), hip.cache_evict_args(8))
+assert "type" in go(cache(dtype=26), hip.cache_evict_args(8))
+need = ctx.cache_evict_workspace(cache(), hip.cache_evict_args(8))
+for ws, n in ((None, need), (space, need - 1), (space + 8, need)): assert "workspace" in go(cache(), hip.cache_evict_args(8), ws, n)
+fake.fake_reset()
+ctx.cache_evict(cache(), hip.cache_evict_args(8), space, need)
+ctx.cache_evict(cache(), hip.cache_evict_args(100), space, need)  # more than there are slots
+assert count("hipLaunchKernel") == 4
+ctx.cache_evict(cache(S=0), hip.cache_evict_args(8), None, 0)
+assert count("hipLaunchKernel") == 4
+""")
+
+
+def test_sampling_refuses_what_it_cannot_do(child):  # noqa: F811
+    child(MADE + """
+u = hip.sample_params(a())
+def go(n=1000, rows=2, p=u, logits=a(), ids=a(), dtype=0, stride=None, ws=space, b=1 << 20): return quiet(lambda: ctx.sample(logits, n, rows, p, ids, dtype=dtype, stride=stride, space=ws, space_bytes=b))
+for n in (0, -5, (1 << 24) + 1): assert "logits" in go(n=n)
+assert "rows" in go(rows=-1) and "rows" in go(rows=1 << 31)
+for dtype in (2, 26, 99): assert "F32" in go(dtype=dtype)
+assert "overlap" in go(stride=999)
+assert "random" in go(p=hip.sample_params(None))
+assert "missing" in go(logits=None) and "missing" in go(ids=None) and "aligned" in go(logits=a() + 2)
+need = ctx.sample_workspace(100000, 2)
+assert need > 0 and "workspace" in go(n=100000, b=need - 1) and "workspace" in go(n=100000, ws=None) and "workspace" in go(n=100000, ws=space + 4)
+assert ctx.sample_workspace(1000, 500) == 0 and ctx.sample_workspace(0, 1) == 0 and ctx.sample_workspace(5, 0) == 0
+fake.fake_reset()
+ctx.sample(a(), 1000, 500, u, a())  # rows enough that each has a work-group: no workspace
+assert count("hipLaunchKernel") == 1
+ctx.sample(None, 1000, 0, u, None)
+assert count("hipLaunchKernel") == 1
+""")
+
+
+def test_adapters_refuse_what_they_cannot_do(child):  # noqa: F811
+    child(MADE + """
+for N, K, slots, rank in ((0, 8, 1, 1), (8, 0, 1, 1), (8, 8, 0, 1), (8, 8, 1, 0), (8, 8, 1, 257), (8, 8, 65537, 1), ((1 << 24) + 1, 8, 1, 1), (8, 8, -1, 1)):
+    quiet(lambda: hip.Adapters(ctx, N, K, slots, rank))
+s = hip.Adapters(ctx, 8, 12, 2, 4)
+down, up = np.ones((3, 12), dtype=np.uint16), np.ones((8, 3), dtype=np.uint16)
+s.load(1, down, up, 2.0)
+s.load(1, None, None)
+for slot in (-1, 2): assert "slot" in quiet(lambda: s.load(slot, down, up))
+for d, u in ((down[:, :11], up), (down, up[:7]), (down, up[:, :2]), (down.astype(np.float32), up), (np.ones((5, 12), dtype=np.uint16), np.ones((8, 5), dtype=np.uint16))): quiet(lambda: s.load(0, d, u))
+assert "matrices" in quiet(lambda: ctx.check(ctx.L.ps_hip_adapters_load(ctx.h, s.h, 0, None, None, 2, 1.0)))
+need = s.workspace(5)
+def go(x=a(), T=5, ids=a(), out=a(), ws=space, n=need, **k): return quiet(lambda: s.apply(x, T, ids, out, space=ws, space_bytes=n, **k))
+assert "x must be" in go(dtype=1)
+assert "tokens" in go(T=-1) and "tokens" in go(T=(1 << 22) + 1)
+for k in ({"x": None}, {"ids": None}, {"out": None}, {"x": a() + 2}): assert "missing" in go(**k)
+x = a()
+assert "same" in go(x=x, out=x)
+assert "overlap" in go(ldx=11) and "overlap" in go(ldo=7)
+for ws, n in ((None, need), (space, need - 1), (space + 8, need)): assert "workspace" in go(ws=ws, n=n)
+fake.fake_reset()
+s.apply(a(), 0, a(), a())
+assert count("hipLaunchKernel") == 0 and s.workspace(0) == 0
+other = hip.Ctx(1)
+assert "device" in refused(lambda: other.check(other.L.ps_hip_adapters_apply(other.h, s.h, 0, a(), 12, 5, a(), None, a(), 8, space, 1 << 20)))
+s.close()
+s.close()
+""")
+
+
+def test_adapters_give_their_memory_back(child):  # noqa: F811
+    """closed, and where the n-th allocation or copy of a set fails"""
+    child(MADE + """
+held = fake.fake_held()
+s = hip.Adapters(ctx, 80, 120, 5, 20)
+s.load(4, np.ones((17, 120), dtype=np.uint16), np.ones((80, 17), dtype=np.uint16), 2.0)
+assert fake.fake_held() > held and fake.fake_stray() == 0
+s.close()
+assert fake.fake_held() == held
+for n in (1, 2, 3, 4):
+    fail("hipMalloc", n)
+    refused(lambda: hip.Adapters(ctx, 80, 120, 5, 20))
+    assert fake.fake_held() == held, n
+s = hip.Adapters(ctx, 80, 120, 5, 20)
+fail("hipMemcpyAsync", 2)
+refused(lambda: s.load(0, np.ones((17, 120), dtype=np.uint16), np.ones((80, 17), dtype=np.uint16)))
+s.load(0, np.ones((17, 120), dtype=np.uint16), np.ones((80, 17), dtype=np.uint16))
+s.close()
+assert fake.fake_held() == held
+""")
+
+
+def test_launches_go_to_the_contexts_device_and_leave_the_callers_current(child):  # noqa: F811
+    child(MADE + """
+dev = C.c_int()
+other = hip.Ctx(1)  # (its device is current now)
+def current():
+    fake.hipGetDevice(C.byref(dev))
+    return dev.value
+assert current() == 1
+c, p, x, y, s = cache(), attn(), a(), a(), hip.sample_params(a())
+calls = [lambda: ctx.cache_attn(c, p, space, 1 << 20), lambda: ctx.cache_advance(c, x), lambda: ctx.cache_evict(c, hip.cache_evict_args(8), space, 1 << 20), lambda: ctx.sample(x, 100, 300, s, y)]
+for f in calls:
+    fake.hipSetDevice(1)
+    fake.fake_reset()
+    f()
+    assert count("hipLaunchKernel") >= 1 and current() == 1
+# what a failing launch says is the caller's to see
+fail("hipLaunchKernel")
+try: ctx.sample(x, 100, 300, s, y)
+except hip.PSHipError: pass
+else: raise AssertionError("a failed launch went unnoticed")
+""")
+
+
+def test_everything_of_a_step_is_captured(child):  # noqa: F811
+    """nothing but launches between the beginning and the end of a capture: no allocation, no copy, no memset, no wait"""
+    child(MADE + """
+s = hip.Adapters(ctx, 8, 12, 2, 4)
+fake.fake_reset()
+ctx.cache_attn(cache(), attn(weight_out=a(), tree=a()), space, 1 << 20)
+ctx.cache_attn(cache(dtype=30), attn(new=40, weight_out=a()), space, 1 << 20)
+ctx.cache_advance(cache(), a(), a(), 3)
+ctx.cache_evict(cache(), hip.cache_evict_args(8), space, 1 << 20)
+ctx.sample(a(), 100000, 2, hip.sample_params(a()), a(), space=space, space_bytes=1 << 20) if ctx.sample_workspace(100000, 2) <= 1 << 20 else None
+s.apply(a(), 500, a(), a(), space=space, space_bytes=1 << 20)
+assert count("hipLaunchKernel") > 10 and count("hipMemcpy") == count("hipMemset") == count("Synchronize") == count("hipEvent") == 0
+# (the lambdas allocate their buffers through the library: no other allocation)
+""")
