@@ -24,7 +24,7 @@ struct ev_args {
 };
 // weights as whole numbers of the same order, NaN lowest
 __device__ __forceinline__ unsigned order_of(float w) {
-    const unsigned u = __float_as_uint(w);
+    const unsigned u = __float_as_uint(w == 0.f ? 0.f : w); // (the two zeros are equal)
     if ((u & 0x7fffffffu) > 0x7f800000u) return 0u;
     return min((u & 0x80000000u) ? ~u : u | 0x80000000u, 0xfffffffeu);
 }

@@ -250,6 +250,22 @@ def test_eviction(ctx, hip, dtype, dim, n_ctx, n_kv, keep, recent, first, in_pla
         x.free()
 
 
+def test_eviction_takes_the_two_zeros_as_equal(ctx, hip):
+    n, keep, dim = 80, 30, 8
+    k, v = np.random.default_rng(8).standard_normal((2, 1, n, 1, dim)).astype(np.float32)
+    w = np.zeros((1, 1, n), dtype=np.float32)
+    w[0, 0, :40:3] = -0.0  # below it a slot at the end would stay for one of these
+    pos = np.arange(n, dtype=np.int32).reshape(1, 1, n)
+    d = [ctx.to_device(x) for x in (k, v, np.array([n], dtype=np.int32), pos, w)]
+    cache, args = hip.kv_cache(F32, d[0], d[1], d[2], 1, n, 1, dim, pos=d[3], weight=d[4]), hip.cache_evict_args(keep)
+    need = ctx.cache_evict_workspace(cache, args)
+    space = ctx.empty(need, np.uint8)
+    ctx.cache_evict(cache, args, space, need)
+    assert np.array_equal(d[0].numpy()[0, :keep], k[0, :keep]) and np.array_equal(d[3].numpy()[0, 0, :keep], np.arange(keep)) and d[2].numpy()[0] == keep
+    for x in d + [space]:
+        x.free()
+
+
 # ---------------------------------------------------------------------------------------------------------------------------- sampling
 def run_sample(ctx, hip, logits, dtype, rows_settings, stride=None):
     """logits: the type's bits [rows, n]; rows_settings: (temperature, top_k, top_p, min_p, u) arrays or None"""
