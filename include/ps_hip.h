@@ -558,7 +558,7 @@ typedef struct {
     const void *k_new, *v_new; /* [s * new_seq_stride + t * new_row_stride + g * dim + e], both or neither */
     int64_t q_seq_stride, q_row_stride, out_seq_stride, out_row_stride, new_seq_stride, new_row_stride; /* 0: rows one behind the other */
     const int32_t *count;   /* [n_seqs], or NULL: n_new each */
-    const int32_t *pos_new; /* [n_seqs][n_new] written to cache->pos for every kv head, or NULL */
+    const int32_t *pos_new; /* [n_seqs][n_new] written to cache->pos for every kv head, with k_new and v_new, or NULL */
     const uint8_t *tree;
     float *weight_out;
 } ps_cache_attn_params;

@@ -51,6 +51,7 @@ const char *wrong_attn(const ps_kv_cache *k, const ps_cache_attn_params *p) {
         p->out_row_stride * size % 16 || p->new_seq_stride * size % 16 || p->new_row_stride * size % 16)
         return "rows must be 16-byte aligned";
     if (p->pos_new && !k->pos) return "positions have no place in the cache";
+    if (p->pos_new && !p->k_new) return "positions come with new keys and values";
     return nullptr;
 }
 // rows one behind the other where a stride is 0

@@ -44,6 +44,7 @@ p = attn(); p.q = None
 assert "missing" in go(cache(), p)
 assert "together" in go(cache(), attn(k_new=a())) and "together" in go(cache(), attn(v_new=a()))
 assert "positions" in go(cache(pos=False), attn(pos_new=a()))
+assert "new keys" in go(cache(), attn(pos_new=a()))
 for i in range(6):
     assert "aligned" in go(cache(), attn(strides=[4 if i == j else 0 for j in range(6)])), i
 p = attn(); p.q += 4
