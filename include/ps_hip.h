@@ -594,7 +594,7 @@ typedef struct {
     const float *top_p, *min_p, *u;
 } ps_sample_params;
 size_t ps_hip_sample_workspace(ps_hip_ctx *ctx, int64_t n, int64_t rows);
-/* logits: [rows][n] of dtype PS_F32, PS_F16 or PS_BF16, rows `stride` numbers apart; ids int32 [rows]; prob [rows] the taken token's share of the candidates left, or NULL (device) */
+/* logits: [rows][n] of dtype PS_F32, PS_F16 or PS_BF16, rows `stride` numbers apart, fewer than 2^22 of them; ids int32 [rows]; prob [rows] the taken token's share of the candidates left, or NULL (device) */
 int ps_hip_sample(ps_hip_ctx *ctx, int dtype, const void *logits, int64_t n, int64_t rows, int64_t stride, const ps_sample_params *p, int32_t *ids, float *prob, void *workspace,
                   size_t workspace_bytes);
 

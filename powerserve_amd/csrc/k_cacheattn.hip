@@ -967,7 +967,7 @@ size_t psv_attn_space(int n_cu, const ps_kv_cache &c, const ps_cache_attn_params
     // more than 32 rows of a 16-bit cache: 128 rows a work-group
     const bool many = size == 2 && rows > 32;
     const long long groups = heads * (many ? (rows + ROWS - 1) / ROWS : (a.tiles + 1) / 2);
-    a.parts = (int)std::min<long long>({std::max<long long>(((many ? 1 : 3) * n_cu + groups - 1) / groups, many ? 1 : (c.n_ctx + 511) / 512), (c.n_ctx + 127) / 128, 64});
+    a.parts = (int)std::min<long long>({std::max<long long>(((many ? 1 : 3) * n_cu + groups - 1) / groups, many ? 1 : (c.n_ctx + 511) / 512), (c.n_ctx + 127) / 128, 64, std::max(1ll, ((1ll << 24) - 1) / groups)}); // (a launch's grid has fewer than 2^32 threads)
     a.plain = c.slot_stride >= 0 && c.slot_stride < (1 << 24);
     ps_carve ws{(char *)base};
     a.lse = ws.take<float>((size_t)(heads * rows));

@@ -21,6 +21,7 @@ struct on_device {
     int now;
 };
 bool aligned(const void *p, size_t to) { return ((uintptr_t)p & (to - 1)) == 0; }
+constexpr int64_t MOST_GROUPS = (1 << 24) - 1; // work-groups of 256 threads of a launch: a grid has fewer than 2^32 threads a direction
 int number_size(int dtype) { return dtype == PS_F32 ? 4 : dtype == PS_F16 || dtype == PS_BF16 ? 2 : 0; }
 
 // what is wrong with a cache, or NULL
@@ -43,7 +44,7 @@ const char *wrong_attn(const ps_kv_cache *k, const ps_cache_attn_params *p) {
     if (p->n_new < 0 || p->n_new > k->n_ctx) return "more new tokens than slots";
     if (!(std::fabs(p->scale) <= 1e30f)) return "the scale is not a number, or above 1e30";
     const int64_t heads = (int64_t)k->n_seqs * k->kv_heads, rows = (int64_t)p->n_new * (p->heads / k->kv_heads);
-    if (rows > (1 << 24) || rows * (p->heads / k->kv_heads) > UINT32_MAX || (int64_t)p->n_new * k->kv_heads * 32 > INT32_MAX || heads * ((rows + 15) / 16) * 64 > INT32_MAX || heads * ((k->n_ctx + 63) / 64) > INT32_MAX) return "too many rows";
+    if (rows > (1 << 24) || rows * (p->heads / k->kv_heads) > UINT32_MAX || (int64_t)p->n_new * k->kv_heads * 32 > INT32_MAX || heads * ((rows + 15) / 16) > MOST_GROUPS - 65536 || heads * ((k->n_ctx + 63) / 64) > MOST_GROUPS) return "too many rows or slots";
     if (!k->n_seqs || !p->n_new) return nullptr;
     if (!p->q || !p->out || p->q == p->out) return "q and out are missing or the same";
     if (!p->k_new != !p->v_new) return "new keys and values come together";
@@ -125,7 +126,7 @@ int ps_hip_cache_evict(ps_hip_ctx *c, const ps_kv_cache *k, const ps_cache_evict
 // ------------------------------------------------------------------ sampling
 static const char *wrong_sample(int64_t n, int64_t rows) {
     if (n < 1 || n > (1 << 24)) return "a row has 1 to 2^24 logits";
-    if (rows < 0 || rows > INT32_MAX) return "a number of rows that is not one";
+    if (rows < 0 || rows > MOST_GROUPS / 4) return "0 to 2^22 - 1 rows"; // (1024 threads each)
     return nullptr;
 }
 size_t ps_hip_sample_workspace(ps_hip_ctx *c, int64_t n, int64_t rows) {

@@ -53,6 +53,11 @@ need = ctx.cache_attn_workspace(cache(), attn())
 assert need > 0
 for ws, n in ((None, need), (space, need - 1), (space + 8, need), (space, 0)): assert "workspace" in go(cache(), attn(), ws, n)
 assert "many" in go(cache(S=60000, n_ctx=1 << 27), attn(new=1 << 20))
+assert "many" in go(cache(dtype=0, S=65535, G=8, n_ctx=4096, dim=8), attn(heads=8, new=100, weight_out=a()))  # 64 slots a work-group: more than 2^24 of them
+assert "many" in go(cache(S=65535, G=512, n_ctx=16, dim=8), attn(heads=512, new=1))
+c, p = cache(dtype=0, S=500, G=512, n_ctx=4096, dim=8), attn(heads=512, new=512)  # 8 parts of 512 slots, 16 work-groups of 32 rows each: a grid of more than 2^32 threads; there are 4
+heads, row_tiles, part = 500 * 512, 512 // 16, 16 * (8 + 2) * 4
+assert ctx.cache_attn_workspace(c, p) == heads * 512 * 4 + heads * row_tiles * 4 * part
 fake.fake_reset()
 ctx.cache_attn(cache(), attn(), space, need)
 assert count("hipLaunchKernel") > 0
@@ -90,6 +95,7 @@ u = hip.sample_params(a())
 def go(n=1000, rows=2, p=u, logits=a(), ids=a(), dtype=0, stride=None, ws=space, b=1 << 20): return quiet(lambda: ctx.sample(logits, n, rows, p, ids, dtype=dtype, stride=stride, space=ws, space_bytes=b))
 for n in (0, -5, (1 << 24) + 1): assert "logits" in go(n=n)
 assert "rows" in go(rows=-1) and "rows" in go(rows=1 << 31)
+assert "rows" in go(n=10, rows=1 << 22)  # 1024 threads each: a grid would pass 2^32 of them
 for dtype in (2, 26, 99): assert "F32" in go(dtype=dtype)
 assert "overlap" in go(stride=999)
 assert "random" in go(p=hip.sample_params(None))
