@@ -259,8 +259,8 @@ size_t psv_evict_space(const ps_kv_cache &c, const ps_cache_evict_params &p, voi
     // the keys of up to 32768 slots fit the LDS (128 KB): the passes behind the first read them there, else weights and positions again
     a.in_lds = c.n_ctx <= EV_LDS_KEYS;
     const size_t lds = a.in_lds ? (size_t)c.n_ctx * 4 : 0;
-    static unsigned long long seen = 0;
-    if (lds && ps_first_on_device(&seen)) (void)hipFuncSetAttribute((const void *)evict_choose_kernel, hipFuncAttributeMaxDynamicSharedMemorySize, EV_LDS_KEYS * 4);
+    static std::atomic<unsigned long long> done{0};
+    if (lds) ps_allow_lds((const void *)evict_choose_kernel, EV_LDS_KEYS * 4, done);
     hipLaunchKernelGGL(evict_choose_kernel, dim3((unsigned)c.kv_heads, (unsigned)c.n_seqs), dim3(EV_THREADS), lds, st, a);
     hipLaunchKernelGGL(evict_move_kernel, dim3((unsigned)std::max(1, (a.cap + EV_ROWS - 1) / EV_ROWS), (unsigned)c.kv_heads, (unsigned)c.n_seqs), dim3(256), 0, st, a);
     return ws.at;

@@ -650,13 +650,13 @@ __global__ __launch_bounds__(PICK) void sample_pick_kernel(const smp_args a) {
 template <class E>
 void launch(const smp_args &a, hipStream_t st) {
     const size_t lds = sizeof(pick_lds);
-    static unsigned long long seen[2] = {0, 0};
+    static std::atomic<unsigned long long> done[2];
     if (a.parts == 1) {
-        if (ps_first_on_device(&seen[0])) (void)hipFuncSetAttribute((const void *)sample_pick_kernel<E, true>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+        ps_allow_lds((const void *)sample_pick_kernel<E, true>, lds, done[0]);
         hipLaunchKernelGGL((sample_pick_kernel<E, true>), dim3((unsigned)a.rows), dim3(PICK), lds, st, a);
         return;
     }
-    if (ps_first_on_device(&seen[1])) (void)hipFuncSetAttribute((const void *)sample_pick_kernel<E, false>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+    ps_allow_lds((const void *)sample_pick_kernel<E, false>, lds, done[1]);
     hipLaunchKernelGGL((sample_top_kernel<E>), dim3((unsigned)a.parts, (unsigned)a.rows), dim3(256), 0, st, a);
     hipLaunchKernelGGL((sample_head_kernel<E>), dim3((unsigned)a.parts, (unsigned)a.rows), dim3(PICK), 0, st, a);
     hipLaunchKernelGGL((sample_pick_kernel<E, false>), dim3((unsigned)a.rows), dim3(PICK), lds, st, a);

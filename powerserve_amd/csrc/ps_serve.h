@@ -3,6 +3,8 @@
 #pragma once
 #include "ps_internal.h"
 
+#include <atomic>
+
 // Scratch memory in pieces of 256 bytes' alignment: the same steps give the size (base NULL) and the pieces.
 struct ps_carve {
     char *base;
@@ -13,6 +15,15 @@ struct ps_carve {
         return p;
     }
 };
+
+// More than 64 KB of LDS for a kernel's launches, once on each device.  Two contexts may come here at the same time: a device counts as done when it is, and both may do it.
+inline void ps_allow_lds(const void *kernel, size_t bytes, std::atomic<unsigned long long> &done) {
+    int dev = 0;
+    (void)hipGetDevice(&dev);
+    const unsigned long long bit = 1ull << (dev & 63);
+    if (done.load(std::memory_order_acquire) & bit) return;
+    if (hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) == hipSuccess) done.fetch_or(bit, std::memory_order_release);
+}
 
 size_t psv_attn_space(int n_cu, const ps_kv_cache &c, const ps_cache_attn_params &p, void *base, bool launch, hipStream_t st); // the bytes it takes; launch: enqueues
 void psv_advance(hipStream_t st, const ps_kv_cache &c, const int32_t *count, const int32_t *take, int n_take);
