@@ -208,6 +208,114 @@ def test_an_accepted_path_becomes_part_of_the_cache(ctx, hip, dtype):
     s.free()
 
 
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("n_new", [1, 5, 70])
+@pytest.mark.parametrize("scale", [-0.11, 0.0, 1e-3])
+def test_scales_of_every_kind(ctx, hip, dtype, n_new, scale):
+    rng = np.random.default_rng(n_new)
+    s = Step(ctx, hip, rng, dtype, 6, 2, 64, 500, [3, 0, 411], n_new)
+    s.args.scale = s.scale = float(np.float32(scale))
+    s.run().check()
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("n_new,heads,kv_heads,dim", [(7, 32, 8, 128), (5, 8, 2, 128), (8, 4, 1, 88), (17, 3, 3, 64), (1, 20, 1, 128), (32, 1, 1, 16), (33, 1, 1, 128)])
+@pytest.mark.parametrize("as_tree", [False, True])
+def test_two_tiles_of_rows(ctx, hip, dtype, n_new, heads, kv_heads, dim, as_tree):
+    rng = np.random.default_rng(n_new + dim)
+    Step(ctx, hip, rng, dtype, heads, kv_heads, dim, 700, [0, 640, 129], n_new, tree=random_tree(rng, 3, n_new) if as_tree else None).run().check()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("S", [255, 256, 257, 300])
+def test_many_sequences(ctx, hip, dtype, S):
+    rng = np.random.default_rng(S)
+    Step(ctx, hip, rng, dtype, 4, 2, 64, 300, rng.integers(0, 300, S), 1).run().check()
+
+
+@pytest.mark.parametrize("dtype", [F32, F16])
+@pytest.mark.parametrize("n_new", [1, 40])
+def test_one_long_sequence_and_among_short_ones(ctx, hip, dtype, n_new):
+    rng = np.random.default_rng(9)
+    Step(ctx, hip, rng, dtype, 2, 1, 64, 40000, [39900], n_new).run().check()
+    Step(ctx, hip, rng, dtype, 2, 1, 64, 20000, [0, 19900, 3], n_new).run().check()
+
+
+@pytest.mark.parametrize("dtype", [F32, F16])
+@pytest.mark.parametrize("n_new", [2, 50])
+def test_other_layouts_give_the_same_bits(ctx, hip, dtype, n_new):
+    """Heads before slots, rows of q, out, k_new and v_new with something between them, a workspace full of ones, another context: the same result to the bit, and nothing between the rows is touched."""
+    rng = np.random.default_rng(n_new)
+    S, H, G, D, n_ctx, pad = 3, 8, 2, 72, 400, 24
+    s = Step(ctx, hip, rng, dtype, H, G, D, n_ctx, [350, 0, 77], n_new)
+    s.run()
+    want = [s.d[n].numpy() for n in ("out", "weight_out", "k", "v")]
+    other = hip.Ctx(0)
+    kt, vt = (other.to_device(np.ascontiguousarray(x[:, :, 0].transpose(0, 2, 1, 3))) for x in (s.k, s.v))
+
+    def wider(x):
+        y = np.full((S, n_new + 1, x.shape[2] * D + pad), 3, dtype=x.dtype)
+        y[:, :n_new, :x.shape[2] * D] = x.reshape(S, n_new, -1)
+        return y
+
+    ow = wider(s.d["out"].numpy() * 0 + ref.pack(77.0, dtype))
+    dev = [other.to_device(x) for x in (wider(s.q), wider(s.kn), wider(s.vn), ow)]
+    n_kv, w, w_out = other.to_device(np.array([350, 0, 77], dtype=np.int32)), other.to_device(s.weight), other.to_device(np.full(s.weight.shape, -5.0, dtype=np.float32))
+    cache = hip.kv_cache(dtype, kt, vt, n_kv, S, n_ctx, G, D, weight=w, strides=(G * n_ctx * D, D, n_ctx * D))
+    q_row, n_row = H * D + pad, G * D + pad
+    args = hip.cache_attn_args(dev[0], dev[3], H, n_new, s.scale, k_new=dev[1], v_new=dev[2], weight_out=w_out,
+                               strides=((n_new + 1) * q_row, q_row, (n_new + 1) * q_row, q_row, (n_new + 1) * n_row, n_row))
+    need = other.cache_attn_workspace(cache, args)
+    space = other.to_device(np.full(need, 255, dtype=np.uint8))
+    other.cache_attn(cache, args, space, need)
+    got = dev[3].numpy()
+    same = lambda a, b: np.array_equal(np.ascontiguousarray(a).view(np.uint8), np.ascontiguousarray(b).view(np.uint8))  # noqa: E731
+    assert same(got[:, :n_new, :H * D].reshape(S, n_new, H, D), want[0])
+    assert (got[:, n_new:] == ow[:, n_new:]).all() and (got[:, :, H * D:] == ow[:, :, H * D:]).all()
+    assert same(w_out.numpy(), want[1]) and same(kt.numpy().transpose(0, 2, 1, 3), want[2][:, :, 0]) and same(vt.numpy().transpose(0, 2, 1, 3), want[3][:, :, 0])
+    for x in dev + [kt, vt, n_kv, w, w_out, space]:
+        x.free()
+    s.check()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("n_new", [1, 50])
+def test_offsets_past_32_bits(ctx, hip, dtype, n_new):
+    """Slots 8 MB apart, 600 of them, a step with eviction: the bits of the same slots one behind the other."""
+    rng = np.random.default_rng(n_new)
+    G, D, n_ctx, n0, keep = 2, 64, 620, 560, 400
+    s = Step(ctx, hip, rng, dtype, 4, G, D, n_ctx, [n0], n_new)
+    item, step = s.k.itemsize, 8 << 20
+    far = [ctx.empty((n_ctx * step,), np.uint8) for _ in range(2)]
+    for x, y in zip(far, (s.k, s.v)):
+        for j in range(n0):
+            row = np.ascontiguousarray(y[0, j, 0])
+            ctx.check(ctx.L.ps_hip_memcpy_h2d(ctx.h, x.ptr + j * step, row.ctypes.data_as(C.c_void_p), row.nbytes))
+    got = []
+    for k, v, strides in ((s.d["k"].ptr, s.d["v"].ptr, (n_ctx * G * D, G * D, D)), (far[0].ptr, far[1].ptr, (n_ctx * step // item, step // item, D))):
+        n_kv, w, pos, one = ctx.to_device(np.array([n0], dtype=np.int32)), ctx.to_device(s.weight), ctx.to_device(s.pos), ctx.to_device(np.array([n_new], dtype=np.int32))
+        cache = hip.kv_cache(dtype, k, v, n_kv, 1, n_ctx, G, D, pos=pos, weight=w, strides=strides)
+        args, evict = hip.cache_attn_args(s.d["q"], s.d["out"], 4, n_new, s.scale, k_new=s.d["kn"], v_new=s.d["vn"], weight_out=w), hip.cache_evict_args(keep, 30, 2)
+        need = [ctx.cache_attn_workspace(cache, args), ctx.cache_evict_workspace(cache, evict)]
+        space = [ctx.empty(b, np.uint8) for b in need]
+        ctx.cache_attn(cache, args, space[0], need[0])
+        ctx.cache_advance(cache, one)
+        ctx.cache_evict(cache, evict, space[1], need[1])
+        rows = np.empty((2, n0 + n_new, G * D), dtype=s.k.dtype)
+        for i, p in enumerate((k, v)):
+            for j in range(n0 + n_new):
+                ctx.check(ctx.L.ps_hip_memcpy_d2h(ctx.h, rows[i, j].ctypes.data_as(C.c_void_p), p + j * strides[1] * item, G * D * item))
+        got.append([s.d["out"].numpy(), w.numpy(), pos.numpy(), n_kv.numpy(), rows])
+        for x in [n_kv, w, pos, one] + space:
+            x.free()
+    for a, b in zip(*got):
+        assert np.array_equal(a.view(np.uint8), b.view(np.uint8))
+    assert got[0][3][0] == keep
+    for x in far:
+        x.free()
+    s.free()
+
+
 # ---------------------------------------------------------------------------------------------------------------------------- eviction
 @pytest.mark.parametrize("dtype,dim", [(F32, 8), (F16, 128), (BF16, 40)])
 @pytest.mark.parametrize("n_ctx,n_kv,keep,recent,first", [(300, [300, 0, 1, 65, 64, 299], 64, 16, 4), (70, [70, 69, 68], 69, 69, 0), (5000, [5000, 1025, 1024, 4097], 1024, 500, 0),
@@ -371,6 +479,18 @@ def test_sampling_at_the_borders(ctx, hip, rows):
     one(np.where(base > 0, np.float32(0.0), np.float32(-0.0)), 1.0, 3, 1.0, 0.0, 0.9)
 
 
+@pytest.mark.parametrize("rows", [1, 140])
+@pytest.mark.parametrize("n", [777, 30000])
+def test_sampling_with_settings_at_the_ends_of_their_types(ctx, hip, rows, n):
+    rng = np.random.default_rng(n)
+    base = 2 * rng.standard_normal((rows, n)).astype(np.float32)
+    for settings in ((np.inf, 0, 1.0, 0.0, 0.3), (1e-45, 0, 1.0, 0.0, 0.9), (3e38, 9, 0.7, 0.0, 0.6), (1.0, 2**31 - 1, 1.0, 0.0, 0.4), (1.0, -2**31, 0.999, 0.0, 0.4), (1.0, 1, 1e-40, 1e-40, 0.4),
+                     (-0.0, 3, 1.0, 0.0, 0.4), (1.0, 1014, 1.0, 0.0, 0.77), (1.0, 1015, 1.0, 0.0, 0.77), (0.5, 0, -1.0, -1.0, 0.5)):
+        check_sample(ctx, hip, base, F32, [np.full(rows, x) for x in settings])
+    wide = np.where(base > 0, np.float32(3.4e38), np.float32(-3.4e38))
+    check_sample(ctx, hip, wide, F32, [np.full(rows, x) for x in (1.0, 0, 1.0, 0.0, 0.6)])
+
+
 # ---------------------------------------------------------------------------------------------------------------------------- adapters
 def run_adapters(ctx, hip, rng, dtype, T, N, K, ranks, ids, pad=0, in_place=False, base=True):
     down = [ref.pack(rng.standard_normal((r, K)) / math.sqrt(K), BF16) for r in ranks]
@@ -426,6 +546,36 @@ def test_adapters_of_long_runs_strides_and_in_place(ctx, hip, dtype):
 def test_many_adapters_of_many_tokens(ctx, hip):
     rng = np.random.default_rng(2)
     run_adapters(ctx, hip, rng, BF16, 1500, 32, 64, [2] * 1100, rng.integers(0, 1100, 1500))
+
+
+def test_more_adapters_than_the_plan_counts_in_lds(ctx, hip):
+    rng = np.random.default_rng(12)
+    run_adapters(ctx, hip, rng, F32, 300, 12, 20, [1] * 8300, np.where(rng.random(300) < 0.5, 8299, rng.integers(0, 8301, 300)))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("T", [20, 90])
+def test_odd_numbers_of_a_token_stay_its_own(ctx, hip, dtype, T):
+    """Infinities and NaN in some tokens' x, and the largest numbers: the other tokens of the same adapter have the bits that they have without them."""
+    rng = np.random.default_rng(T)
+    a = hip.Adapters(ctx, 40, 100, 1, 24)
+    a.load(0, ref.pack(rng.standard_normal((24, 100)), BF16), ref.pack(rng.standard_normal((40, 24)), BF16), 0.5)
+    x = ref.pack(rng.standard_normal((T, 100)), dtype)
+    odd = x.copy()
+    odd[[3, 4, 17], [7, 99, 0]] = ref.pack([np.inf, NAN, -np.inf], dtype)
+    ids, need = ctx.to_device(np.zeros(T, dtype=np.int32)), a.workspace(T)
+    space, out = ctx.empty(need, np.uint8), ctx.empty((T, 40))
+    got = []
+    for y in (x, odd):
+        d = ctx.to_device(y)
+        a.apply(d, T, ids, out, dtype=dtype, space=space, space_bytes=need)
+        got.append(out.numpy())
+        d.free()
+    others = np.setdiff1d(np.arange(T), [3, 4, 17])
+    assert np.array_equal(got[0][others].view(np.uint32), got[1][others].view(np.uint32)) and not np.isfinite(got[1][[3, 4, 17]]).any() and np.isfinite(got[0]).all()
+    a.close()
+    for y in (ids, space, out):
+        y.free()
 
 
 def test_adapter_slots_change(ctx, hip):
@@ -531,4 +681,94 @@ def test_a_serving_step_together(ctx, hip, captured):
             assert n_now[s] == N[s] and np.array_equal(p_now[s, :, :N[s]], P[s, :, :N[s]])
             assert np.abs(w_now[s, :, :N[s]] - W[s, :, :N[s]]).max() < 1e-4
             assert tokens[s] == ref.sample(logits[i, s], 1.0, 30, 1.0, 0.0, float(u[i, s]))[0]
+    a.close()
+
+
+@pytest.mark.parametrize("dtype,n_new", [(F32, 1), (BF16, 1), (BF16, 24), (F16, 60), (F32, 60)])
+def test_captured_steps_are_replayed_with_other_lengths(ctx, hip, dtype, n_new):
+    """Two graphs of one step each, with a workspace of their own, replayed in turn over lengths that change in between, eager work between them: the bits of the eager call each time."""
+    rng = np.random.default_rng(n_new)
+    both = [Step(ctx, hip, rng, dtype, 8, 2, 64, 900, [800, 3, 410], n_new) for _ in range(2)]
+    go = [Graphs(ctx).capture(s.run) for s in both]
+    for n_kv in ([800, 3, 410], [0, 0, 0], [840, 1, 2], [5, 830, 128]):
+        new = np.array(n_kv, dtype=np.int32)
+        want = []
+        for s in both:
+            ctx.check(ctx.L.ps_hip_memcpy_h2d(ctx.h, s.d["n_kv"].ptr, new.ctypes.data_as(C.c_void_p), new.nbytes))
+            for n in ("k", "v"):  # (every slot is held by one of the steps: none is to be NaN)
+                x = np.nan_to_num(ref.unpack(getattr(s, n), dtype), nan=0.25)
+                x = np.ascontiguousarray(ref.pack(x, dtype))
+                ctx.check(ctx.L.ps_hip_memcpy_h2d(ctx.h, s.d[n].ptr, x.ctypes.data_as(C.c_void_p), x.nbytes))
+            s.run()
+            want.append([s.d[n].numpy() for n in ("out", "weight_out", "k", "v")])
+        for _ in range(2):
+            for s in both:  # (results that a replay has to write again)
+                x = np.zeros(s.weight.shape, dtype=np.float32)
+                ctx.check(ctx.L.ps_hip_memcpy_h2d(ctx.h, s.d["weight_out"].ptr, x.ctypes.data_as(C.c_void_p), x.nbytes))
+            for g in go:
+                assert g() == 0
+            ctx.sync()
+            for s, w in zip(both, want):
+                got = [s.d[n].numpy() for n in ("out", "weight_out", "k", "v")]
+                for i, n in enumerate(n_kv):
+                    e = n + n_new
+                    assert np.array_equal(got[0][i].view(np.uint8), w[0][i].view(np.uint8)) and np.array_equal(got[1][i, :, :e], w[1][i, :, :e])
+                assert np.array_equal(got[2].view(np.uint8), w[2].view(np.uint8)) and np.array_equal(got[3].view(np.uint8), w[3].view(np.uint8))
+    for s in both:
+        s.free()
+
+
+def test_sampling_eviction_and_adapters_captured_before_any_eager_call(ctx, hip):
+    """Captured as the first calls of their kinds in a new context, replayed with other numbers in the same places, sizes that take several kernels each."""
+    rng = np.random.default_rng(21)
+    mine = hip.Ctx(0)
+    rows, n, T, N, K = 3, 50000, 100, 64, 96
+    a = hip.Adapters(mine, N, K, 4, 16)
+    mats = [(ref.pack(rng.standard_normal((16, K)) / 10, BF16), ref.pack(rng.standard_normal((N, 16)), BF16)) for _ in range(4)]
+    for i, (d, u) in enumerate(mats):
+        a.load(i, d, u, 1.0)
+    up = mine.to_device
+    logits, u, ids, prob = up(np.zeros((rows, n), dtype=np.float32)), up(np.zeros(rows, dtype=np.float32)), mine.empty((rows,), np.int32), mine.empty((rows,))
+    x, who, out = up(np.zeros((T, K), dtype=np.float32)), up(np.zeros(T, dtype=np.int32)), mine.empty((T, N))
+    S, G, n_ctx, D, keep = 2, 2, 600, 8, 200
+    k, v, w, pos = (up(y) for y in (np.zeros((S, n_ctx, G, D), np.float32), np.zeros((S, n_ctx, G, D), np.float32), np.zeros((S, G, n_ctx), np.float32), np.zeros((S, G, n_ctx), np.int32)))
+    n_kv = up(np.zeros(S, dtype=np.int32))
+    cache, evict = hip.kv_cache(F32, k, v, n_kv, S, n_ctx, G, D, pos=pos, weight=w), hip.cache_evict_args(keep, 20, 2)
+    need = [mine.sample_workspace(n, rows), a.workspace(T), mine.cache_evict_workspace(cache, evict)]
+    space = [mine.empty(b, np.uint8) for b in need]
+
+    def step():
+        mine.sample(logits, n, rows, hip.sample_params(u=u), ids, prob=prob, space=space[0], space_bytes=need[0])
+        a.apply(x, T, who, out, space=space[1], space_bytes=need[1])
+        mine.cache_evict(cache, evict, space[2], need[2])
+
+    go = Graphs(mine).capture(step)
+
+    def put(d, y):
+        y = np.ascontiguousarray(y)
+        mine.check(mine.L.ps_hip_memcpy_h2d(mine.h, d.ptr, y.ctypes.data_as(C.c_void_p), y.nbytes))
+        return y
+
+    for i in range(4):
+        l = put(logits, (2 * rng.standard_normal((rows, n))).astype(np.float32))  # noqa: E741
+        uu, xx, ww = put(u, rng.random(rows).astype(np.float32)), put(x, rng.standard_normal((T, K)).astype(np.float32)), put(w, rng.random((S, G, n_ctx)).astype(np.float32))
+        kk, _, ii = put(k, rng.standard_normal((S, n_ctx, G, D)).astype(np.float32)), put(v, rng.standard_normal((S, n_ctx, G, D)).astype(np.float32)), put(who, rng.integers(-1, 4, T).astype(np.int32))
+        pp, nn = put(pos, np.argsort(rng.random((S, G, n_ctx)), -1).astype(np.int32)), put(n_kv, np.array([600, 150 + 40 * i], dtype=np.int32))
+        assert go() == 0
+        tokens, y, k2, w2 = ids.numpy(), out.numpy(), k.numpy(), w.numpy()
+        for r in range(rows):
+            want, _, near = ref.sample(l[r], 1.0, 0, 1.0, 0.0, float(uu[r]))
+            assert near < 2.0**-25 or tokens[r] == want
+        for t in range(T):
+            if ii[t] < 0:
+                assert (y[t] == 0).all()
+                continue
+            d, b = (ref.unpack(m, BF16) for m in mats[ii[t]])
+            size = np.abs(b) @ (np.abs(d) @ np.abs(xx[t]).astype(np.float64))
+            assert (np.abs(y[t] - b @ (d @ xx[t].astype(np.float64))) <= ((K + 3 * 16 + 32) * 2.0**-24 + 2.0**-22) * size).all()
+        for s in range(S):
+            for g in range(G):
+                take = ref.evict(int(nn[s]), keep, 20, 2, ww[s, g], pp[s, g]) if nn[s] > keep else np.arange(nn[s])
+                assert np.array_equal(k2[s, :len(take), g], kk[s, take, g]) and np.array_equal(w2[s, g, :len(take)], ww[s, g, take])
+        assert np.array_equal(n_kv.numpy(), np.minimum(nn, keep))
     a.close()
