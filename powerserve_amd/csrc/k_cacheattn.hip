@@ -42,8 +42,9 @@ struct ca_args {
     int parts, tiles, score_rows; // tiles of 16 rows
     int share, *chunks; // few rows of up to 256 sequences: work-groups that all their keys are shared out to, and keys of a part of each sequence; else 0, NULL
     int plain; // offsets within 32 slots fit 32 bits
-    int wparts;       // parts of the rows that the weights are summed in
-    float *wpart;     // [seq][kv head][part][slot]
+    int near;  // offsets within a sequence's q do
+    int wgroups;      // many rows: work-groups of a kv head that the weights' work is shared out to (0: one each 256 slots)
+    float *wpart;     // [seq][kv head][work-group + block of 256 slots][256]: sums of a work-group's rows of a block
 };
 struct ca_lens { int n0, cnt, len; };
 __device__ __forceinline__ int token_of(const ca_args &a, int row) { return a.by_R ? (int)__umulhi((unsigned)row, a.by_R) : row; }
@@ -60,6 +61,22 @@ __device__ __forceinline__ int chunk_of(const ca_args &a, int s, int len) {
     return max(128, ((len + a.parts - 1) / a.parts + 127) / 128 * 128);
 }
 __device__ __forceinline__ bool sees(const ca_args &a, int s, int t, int u) { return a.tree ? a.tree[((long long)s * a.T + t) * a.T + u] != 0 : u <= t; }
+// Which of the new tokens x .. x + 3 (below 0: held slots, which all see) token t sees, a bit each.  A tree's four bytes are one load, whatever their alignment, moved so that it stays in the row: a
+// byte after the other would be as many waits for the L2 in the last block of every sequence.
+__device__ __forceinline__ unsigned sees4(const ca_args &a, const ca_lens &L, int s, int t, int x) {
+    auto ones = [](int n) { return (1u << min(max(n, 0), 4)) - 1; };
+    if (!a.tree) return ones(min(t, L.cnt - 1) - x + 1);
+    const uint8_t *row = a.tree + ((long long)s * a.T + t) * a.T;
+    const int at = min(max(x, 0), max(a.T - 4, 0)), d = x - at;
+    unsigned v = 0;
+    if (a.T >= 4) __builtin_memcpy(&v, row + at, 4);
+    else
+        for (int i = 0; i < a.T; i++) v |= (unsigned)row[i] << 8 * i;
+    v = ((((v & 0x7f7f7f7fu) + 0x7f7f7f7fu) | v) & 0x80808080u) >> 7; // a byte that is not 0: 1
+    v = v * 0x10204080u >> 28;
+    v = d >= 0 ? v >> min(d, 4) : v << min(-d, 4) | ones(-d);
+    return v & ones(L.cnt - x);
+}
 
 template <class E> __device__ __forceinline__ pv_f4 mfma(const pv_u4 &x, const pv_u4 &y, const pv_f4 &c);
 template <> __device__ __forceinline__ pv_f4 mfma<BF16>(const pv_u4 &x, const pv_u4 &y, const pv_f4 &c) {
@@ -295,16 +312,20 @@ __global__ __launch_bounds__(256, E::SIZE == 4 ? 1 : 2) void cache_attn_kernel(c
         const bool edge = kb + 32 > min(L.n0, k1);
 #pragma unroll
         for (int r = 0; r < RT; r++) {
+            unsigned seen = 0;
+            if (edge)
+#pragma unroll
+                for (int u = 0; u < 2; u++) {
+                    const int j = kb + 16 * u + 4 * q4;
+                    seen |= (sees4(a, L, s, tok[r], j - L.n0) & ((1u << min(max(k1 - j, 0), 4)) - 1)) << 4 * u;
+                }
             float top = -INFINITY;
 #pragma unroll
             for (int u = 0; u < 2; u++)
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
                     float v = z[r][u][i] * a.sc2;
-                    if (edge) {
-                        const int j = kb + 16 * u + 4 * q4 + i;
-                        if (j >= k1 || (j >= L.n0 && !sees(a, s, tok[r], j - L.n0))) v = -INFINITY;
-                    }
+                    if (edge && !(seen >> (4 * u + i) & 1)) v = -INFINITY;
                     z[r][u][i] = v;
                     top = fmaxf(top, v);
                 }
@@ -533,11 +554,11 @@ __global__ __launch_bounds__(256) void cache_weight_kernel(const ca_args a) {
 #pragma unroll
             for (int u = 0; u < 4; u++) {
                 const pv_f4 z = dot<E, DP>(kf[u], qf);
+                const unsigned seen = kb + 64 <= L.n0 ? 15u : sees4(a, L, s, t, kb + 16 * u + 4 * q4 - L.n0);
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
-                    const int j = kb + 16 * u + 4 * q4 + i;
                     const float p = ls == INFINITY ? 0.f : ex<E>(z[i] * a.sc2 - ls);
-                    if (kb + 64 <= L.n0 || (j < L.len && (j < L.n0 || sees(a, s, t, j - L.n0)))) w[u][i] += p;
+                    w[u][i] += seen >> i & 1 ? p : 0.f;
                 }
             }
         }
@@ -582,27 +603,11 @@ __global__ __launch_bounds__(256) void cache_append_kernel(const ca_args a, int 
 // The weights go into the second product as one 16-bit number each (rounded like the result is: 2^-9 of a weight, bf16, to either side); their sum is taken before they are rounded.
 // What bounds it: the first operands of both products from LDS, 32 KB a wave and 64 keys beside 32 instructions of 32 clocks, and as many clocks of soft-max, which two work-groups a CU overlap.
 constexpr int ROWS = 128, KEYS = 64;
-// which of a lane's 16 keys of a tile its token sees, a bit each: key i is x0 + 8 (i / 4) + i % 4 behind the slots that were held.  (A tree: eight loads at once: 32 take registers that the tiles need, one at a time was 16 us of a small step.)
-__device__ __forceinline__ unsigned sees16(const ca_args &a, const ca_lens &L, int s, int tok, int x0) {
+// the same for a lane's 16 keys of a tile of 32, x + 8 (i / 4) + i % 4
+__device__ __forceinline__ unsigned sees16(const ca_args &a, const ca_lens &L, int s, int tok, int x) {
     unsigned bits = 0;
-    if (!a.tree) { // those up to its own: so many of each four
-        const int n = min(tok, L.cnt - 1) - x0 + 1;
 #pragma unroll
-        for (int q = 0; q < 4; q++) bits |= ((1u << min(max(n - 8 * q, 0), 4)) - 1) << 4 * q;
-        return bits;
-    }
-    const uint8_t *see = a.tree + ((long long)s * a.T + tok) * a.T;
-#pragma unroll 1
-    for (int h = 0; h < 16; h += 8) {
-        uint8_t v[8];
-#pragma unroll
-        for (int i = 0; i < 8; i++) v[i] = see[min(max(x0 + 2 * h + 8 * (i >> 2) + (i & 3), 0), L.cnt - 1)];
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const int x = x0 + 2 * h + 8 * (i >> 2) + (i & 3);
-            bits |= (x < 0 || (x < L.cnt && v[i]) ? 1u : 0u) << (h + i);
-        }
-    }
+    for (int q = 0; q < 4; q++) bits |= sees4(a, L, s, tok, x + 8 * q) << 4 * q;
     return bits;
 }
 template <class E, int DP>
@@ -777,25 +782,93 @@ __global__ __launch_bounds__(256, 2) void cache_rows_kernel(const ca_args a) {
     if (h == 0) a.lse[((long long)s * a.G + g) * a.T * a.R + row] = l == 0.f ? INFINITY : ms + log2f(l);
 }
 
-// The weights that slots receive from many rows of a 16-bit cache: 256 keys of a kv head (a wave 64 of them, in registers) against a part of the rows, 64 at a time through LDS.  Sums over rows run in
-// a lane's registers; the parts' sums are left side by side (one part: added to what there is).
+// which of 16 rows, row + 8 (i / 4) + i % 4, see new token x of a tree (below 0: a held slot, which all see), a bit each; rows behind the last repeat it
+__device__ __forceinline__ unsigned seen_by16(const ca_args &a, const ca_lens &L, int s, int row, int rows, int x) {
+    const uint8_t *see = a.tree + (long long)s * a.T * a.T + min(max(x, 0), L.cnt - 1);
+    uint8_t v[16];
+#pragma unroll
+    for (int i = 0; i < 16; i++) v[i] = see[(long long)token_of(a, min(row + 8 * (i >> 2) + (i & 3), rows - 1)) * a.T];
+    unsigned bits = 0;
+#pragma unroll
+    for (int i = 0; i < 16; i++) bits |= (x < 0 || (x < L.cnt && v[i]) ? 1u : 0u) << i;
+    return bits;
+}
+// The work of the weights of a kv head: blocks of 256 slots, each with the tiles of 64 rows that can see a slot of it, one behind the other.  Work-group w of `groups` has the tiles n w / groups ..,
+// so that all have as many whatever the lengths are; where it stands changes the group, the block or both, so that group + block is a place of its own for each pair that meets.
+constexpr int QT = 64;
+struct received {
+    long long n;  // tiles of all blocks
+    int tiles, held, groups; // of a block that all see; blocks that begin before the new tokens; work-groups that have any
+    const ca_args &a;
+    const ca_lens &L;
+    __device__ __forceinline__ int from(int b) const { return a.tree || b < held ? 0 : (b * 256 - L.n0) * a.R / QT; } // rows of tokens before a block's first slot see none of it
+    __device__ __forceinline__ received(const ca_args &a_, const ca_lens &L_) : a(a_), L(L_) {
+        tiles = (L.cnt * a.R + QT - 1) / QT;
+        const int blocks = (L.len + 255) / 256;
+        held = a.tree ? blocks : min((L.n0 + 255) / 256, blocks);
+        n = (long long)held * tiles;
+        for (int b = held; b < blocks; b++) n += tiles - from(b);
+        groups = (int)min((long long)a.wgroups, n);
+    }
+    __device__ __forceinline__ long long start(int w) const { return n * w / groups; }
+    __device__ __forceinline__ int group_of(long long tile) const { return (int)(((tile + 1) * groups + n - 1) / n) - 1; }
+};
+// The weights that slots receive from many rows of a 16-bit cache: 256 keys of a kv head (a wave 64 of them, in registers) against the rows that see any, 64 at a time through LDS.  S = Q K^T here: a
+// lane has a key, so that the sum over rows is its registers' and its other half's; the sums of the work-groups that share a block are left side by side.
 template <class E, int DP>
 __global__ __launch_bounds__(256, 2) void cache_receive_kernel(const ca_args a) {
-    constexpr int KS = DP / 16, QR = DP + 8, PER = DP / 8, QT = 64, ST = QT * PER / 256;
+    constexpr int KS = DP / 16, QR = DP + 8, PER = DP / 8, ST = QT * PER / 256;
     __shared__ __attribute__((aligned(16))) unsigned short ql[2][QT * QR];
-    __shared__ float lsl[2][QT];
+    __shared__ __attribute__((aligned(16))) float lsl[2][QT];
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, c = lane & 31, h = lane >> 5;
-    const int blocks = (a.n_ctx + 255) / 256;
     int id = blockIdx.x;
-    const int split = id % a.wparts; id /= a.wparts;
-    const int b = id % blocks; id /= blocks;
-    const int g = id % a.G, s = id / a.G;
+    const int heads = a.n_seqs * a.G, hs = id % heads, s = hs / a.G, g = hs - s * a.G; id /= heads; // (neighbours: kv heads, as above)
     const ca_lens L = lens_of(a, s);
-    if (b * 256 >= L.len) return;
-    const int kb = b * 256 + wave * 64, rows = L.cnt * a.R, tiles = (rows + QT - 1) / QT, per = (tiles + a.wparts - 1) / a.wparts;
-    // rows of tokens before the work-group's first key see none of its keys
-    const int from = a.tree || b * 256 < L.n0 ? 0 : (b * 256 - L.n0) * a.R / QT;
-    const int t0 = max(from, split * per), t1 = min(tiles, split * per + per);
+    const int rows = L.cnt * a.R;
+    const received work(a, L);
+    int b, t0, t1;
+    long long at = 0, end = 0, first = 0; // the tiles that are left, and the block's first
+    if (a.wgroups) {
+        if (id >= work.groups) return;
+        at = work.start(id);
+        end = work.start(id + 1);
+        b = (int)min(at / work.tiles, (long long)work.held);
+        first = (long long)b * work.tiles;
+        while (b >= work.held && first + work.tiles - work.from(b) <= at) { first += work.tiles - work.from(b); b++; }
+    } else {
+        b = id;
+        if (b * 256 >= L.len) return;
+    }
+    const float *lse = a.lse + ((long long)s * a.G + g) * a.T * a.R;
+    const char *qh = a.q + s * a.q_seq + (long long)g * a.R * a.dim * 2;
+    pv_u4 qs[ST];
+    float ls = 0.f;
+    auto fetch = [&](int tile) {
+#pragma unroll
+        for (int i = 0; i < ST; i++) {
+            const int x = tid + 256 * i, row = min(tile * QT + x / PER, rows - 1), tok = token_of(a, row), e = x % PER * 8;
+            if (a.near) qs[i] = *(const pv_u4 *)(qh + (unsigned)(tok * (int)a.q_row + (row - tok * a.R) * a.dim * 2 + (e < a.dim ? e * 2 : 0)));
+            else qs[i] = *(const pv_u4 *)(qh + tok * a.q_row + ((long long)(row - tok * a.R) * a.dim * 2 + (e < a.dim ? e * 2 : 0)));
+            if (e >= a.dim) qs[i] = (pv_u4){0, 0, 0, 0};
+        }
+        if (tid < QT) ls = tile * QT + tid < rows ? lse[tile * QT + tid] : INFINITY;
+    };
+    auto put = [&](int buf) {
+#pragma unroll
+        for (int i = 0; i < ST; i++) { const int x = tid + 256 * i; *(pv_u4 *)(ql[buf] + x / PER * QR + x % PER * 8) = qs[i]; }
+        if (tid < QT) lsl[buf][tid] = ls;
+    };
+#pragma unroll 1
+    do {
+    t0 = work.from(b);
+    t1 = work.tiles;
+    if (a.wgroups) {
+        const int skip = t0;
+        t0 = skip + (int)(at - first);
+        t1 = (int)min((long long)t1, skip + (end - first));
+        at = first = first + work.tiles - skip;
+    }
+    const int kb = b * 256 + wave * 64;
     pv_u4 kf[2][KS];
 #pragma unroll
     for (int u = 0; u < 2; u++) {
@@ -807,24 +880,7 @@ __global__ __launch_bounds__(256, 2) void cache_receive_kernel(const ca_args a) 
             if (e >= a.dim) kf[u][st] = (pv_u4){0, 0, 0, 0};
         }
     }
-    const float *lse = a.lse + ((long long)s * a.G + g) * a.T * a.R;
-    pv_u4 qs[ST];
-    float ls = 0.f;
-    auto fetch = [&](int tile) {
-#pragma unroll
-        for (int i = 0; i < ST; i++) {
-            const int x = tid + 256 * i, row = min(tile * QT + x / PER, rows - 1), tok = token_of(a, row), e = x % PER * 8;
-            qs[i] = *(const pv_u4 *)(a.q + s * a.q_seq + tok * a.q_row + (long long)(g * a.R + row - tok * a.R) * a.dim * 2 + (e < a.dim ? e * 2 : 0));
-            if (e >= a.dim) qs[i] = (pv_u4){0, 0, 0, 0};
-        }
-        if (tid < QT) ls = tile * QT + tid < rows ? lse[tile * QT + tid] : INFINITY;
-    };
-    auto put = [&](int buf) {
-#pragma unroll
-        for (int i = 0; i < ST; i++) { const int x = tid + 256 * i; *(pv_u4 *)(ql[buf] + x / PER * QR + x % PER * 8) = qs[i]; }
-        if (tid < QT) lsl[buf][tid] = ls;
-    };
-    float w[2][16] = {};
+    float w[2][2] = {};
     if (t0 < t1) { fetch(t0); put(0); }
     __syncthreads();
     int cur = 0;
@@ -833,62 +889,80 @@ __global__ __launch_bounds__(256, 2) void cache_receive_kernel(const ca_args a) 
         if (tile + 1 < t1) fetch(tile + 1);
 #pragma unroll 1
         for (int sub = 0; sub < QT / 32; sub++) {
-        const int r0 = tile * QT + 32 * sub;
-        const float mine = lsl[cur][32 * sub + c];
-        const int tok = token_of(a, min(r0 + c, rows - 1));
-        f16v z[2];
+            const int r0 = tile * QT + 32 * sub;
+            if (kb - L.n0 > (a.tree ? L.cnt : token_of(a, min(r0 + 31, rows - 1)))) continue; // these tokens all come before the wave's keys
+            f16v z[2];
 #pragma unroll
-        for (int u = 0; u < 2; u++) {
+            for (int i = 0; i < 16; i++) z[0][i] = z[1][i] = 0.f;
 #pragma unroll
-            for (int i = 0; i < 16; i++) z[u][i] = 0.f;
-        }
+            for (int st = 0; st < KS; st++) {
+                const pv_u4 q = *(const pv_u4 *)(ql[cur] + (32 * sub + c) * QR + 16 * st + 8 * h);
+                z[0] = mfma32<E>(q, kf[0][st], z[0]);
+                z[1] = mfma32<E>(q, kf[1][st], z[1]);
+            }
+            pv_f4 lr[4]; // of rows r0 + 8 (i / 4) + 4 h + i % 4
 #pragma unroll
-        for (int st = 0; st < KS; st++) {
-            const pv_u4 q = *(const pv_u4 *)(ql[cur] + (32 * sub + c) * QR + 16 * st + 8 * h);
-            z[0] = mfma32<E>(kf[0][st], q, z[0]);
-            z[1] = mfma32<E>(kf[1][st], q, z[1]);
-        }
-        if (kb + 64 <= (a.tree ? L.n0 : L.n0 + token_of(a, r0) + 1)) { // all see all
+            for (int x = 0; x < 4; x++) lr[x] = *(const pv_f4 *)(lsl[cur] + 32 * sub + 8 * x + 4 * h);
+            if (kb + 64 <= (a.tree ? L.n0 : L.n0 + token_of(a, r0) + 1)) { // all see all
 #pragma unroll
-            for (int u = 0; u < 2; u++)
+                for (int i = 0; i < 16; i++)
 #pragma unroll
-                for (int i = 0; i < 16; i++) w[u][i] += __builtin_amdgcn_exp2f(fmaf(z[u][i], a.sc2, -mine));
-        } else if (kb < L.len) {
+                    for (int u = 0; u < 2; u++) w[u][i & 1] += __builtin_amdgcn_exp2f(fmaf(z[u][i], a.sc2, -lr[i >> 2][i & 3]));
+            } else if (!a.tree) { // row r sees new token x where r >= x R
 #pragma unroll
-            for (int u = 0; u < 2; u++) {
-                const unsigned bits = mine == INFINITY ? 0 : sees16(a, L, s, tok, kb + 32 * u + 4 * h - L.n0);
+                for (int u = 0; u < 2; u++) {
+                    const int behind = min(max(kb + 32 * u + c - L.n0, 0), L.cnt) * a.R - r0 - 4 * h;
 #pragma unroll
-                for (int i = 0; i < 16; i++) {
-                    const float p = __builtin_amdgcn_exp2f(fmaf(z[u][i], a.sc2, -mine));
-                    w[u][i] += bits >> i & 1 ? p : 0.f;
+                    for (int i = 0; i < 16; i++) {
+                        const float p = __builtin_amdgcn_exp2f(fmaf(z[u][i], a.sc2, -lr[i >> 2][i & 3]));
+                        w[u][i & 1] += 8 * (i >> 2) + (i & 3) >= behind ? p : 0.f;
+                    }
+                }
+            } else if (kb < L.len) {
+#pragma unroll
+                for (int u = 0; u < 2; u++) {
+                    const int x = kb + 32 * u + c - L.n0; // the lane's key among the new ones
+                    const unsigned bits = seen_by16(a, L, s, r0 + 4 * h, rows, x);
+#pragma unroll
+                    for (int i = 0; i < 16; i++) {
+                        const float ls = lr[i >> 2][i & 3], p = __builtin_amdgcn_exp2f(fmaf(z[u][i], a.sc2, -ls));
+                        w[u][i & 1] += ls != INFINITY && (bits >> i & 1) ? p : 0.f;
+                    }
                 }
             }
-        }
         }
         if (tile + 1 < t1) put(cur ^ 1);
         __syncthreads();
     }
-    const long long at = ((long long)s * a.G + g) * a.n_ctx;
+    float v[2];
 #pragma unroll
-    for (int u = 0; u < 2; u++)
-#pragma unroll
-        for (int i = 0; i < 16; i++) {
-            float v = w[u][i];
-#pragma unroll
-            for (int x = 1; x < 32; x <<= 1) v += __shfl_xor(v, x, 64);
-            const int j = kb + 32 * u + 8 * (i >> 2) + 4 * h + (i & 3);
-            if (c != 0 || j >= L.len) continue;
-            if (a.wparts > 1) a.wpart[(((long long)s * a.G + g) * a.wparts + split) * a.n_ctx + j] = v;
-            else a.weight_out[at + j] = j < L.n0 && a.weight ? a.weight[at + j] + v : v;
-        }
+    for (int u = 0; u < 2; u++) {
+        v[u] = w[u][0] + w[u][1];
+        v[u] += __shfl_xor(v[u], 32, 64);
+    }
+    const int j = kb + lane;
+    const float sum = h ? v[1] : v[0];
+    if (a.wgroups) a.wpart[(hs * (a.wgroups + (a.n_ctx + 255ll) / 256) + id + b) * 256 + wave * 64 + lane] = sum;
+    else if (j < L.len) {
+        const long long to = (long long)hs * a.n_ctx + j;
+        a.weight_out[to] = j < L.n0 && a.weight ? a.weight[to] + sum : sum;
+    }
+    b++;
+    } while (at < end);
 }
-__global__ __launch_bounds__(256) void cache_gather_kernel(const ca_args a) { // the parts' sums, in order
-    const int j = blockIdx.x * 256 + threadIdx.x, g = blockIdx.y, s = blockIdx.z;
+__global__ __launch_bounds__(256) void cache_gather_kernel(const ca_args a) { // the sums of a block's work-groups, in order
+    const int b = blockIdx.x, j = b * 256 + threadIdx.x, g = blockIdx.y, s = blockIdx.z;
     const ca_lens L = lens_of(a, s);
     if (j >= L.len) return;
     const long long head = (long long)s * a.G + g, at = head * a.n_ctx + j;
+    const received work(a, L);
     float v = 0.f;
-    for (int p = 0; p < a.wparts; p++) v += a.wpart[(head * a.wparts + p) * a.n_ctx + j];
+    if (work.n) {
+        long long first = (long long)min(b, work.held) * work.tiles;
+        for (int x = work.held; x < b; x++) first += work.tiles - work.from(x);
+        const int w0 = work.group_of(first), w1 = work.group_of(first + work.tiles - work.from(b) - 1);
+        for (int w = w0; w <= w1; w++) v += a.wpart[(head * (a.wgroups + (a.n_ctx + 255ll) / 256) + w + b) * 256 + threadIdx.x];
+    }
     a.weight_out[at] = j < L.n0 && a.weight ? a.weight[at] + v : v;
 }
 
@@ -943,8 +1017,8 @@ void launch_attn(const ca_args &a, bool many, hipStream_t st) {
             hipLaunchKernelGGL((cache_rows_kernel<E, DP>), dim3((unsigned)(heads * a.parts * ((a.T * a.R + ROWS - 1) / ROWS))), dim3(256), 0, st, a);
             if (a.parts > 1) hipLaunchKernelGGL((cache_join_kernel<E>), dim3((unsigned)(heads * a.tiles)), dim3(256), 0, st, a);
             if (!a.weight_out) return;
-            hipLaunchKernelGGL((cache_receive_kernel<E, DP>), dim3((unsigned)(heads * ((a.n_ctx + 255) / 256) * a.wparts)), dim3(256), 0, st, a);
-            if (a.wparts > 1) hipLaunchKernelGGL(cache_gather_kernel, dim3((unsigned)((a.n_ctx + 255) / 256), (unsigned)a.G, (unsigned)a.n_seqs), dim3(256), 0, st, a);
+            hipLaunchKernelGGL((cache_receive_kernel<E, DP>), dim3((unsigned)(heads * (a.wgroups ? a.wgroups : (a.n_ctx + 255) / 256))), dim3(256), 0, st, a);
+            if (a.wgroups) hipLaunchKernelGGL(cache_gather_kernel, dim3((unsigned)((a.n_ctx + 255) / 256), (unsigned)a.G, (unsigned)a.n_seqs), dim3(256), 0, st, a);
             return;
         }
     }
@@ -968,6 +1042,7 @@ size_t psv_attn_space(int n_cu, const ps_kv_cache &c, const ps_cache_attn_params
     const bool many = size == 2 && rows > 32;
     const long long groups = heads * (many ? (rows + ROWS - 1) / ROWS : (a.tiles + 1) / 2);
     a.parts = (int)std::min<long long>({std::max<long long>(((many ? 1 : 3) * n_cu + groups - 1) / groups, many ? 1 : (c.n_ctx + 511) / 512), (c.n_ctx + 127) / 128, 64, std::max(1ll, ((1ll << 24) - 1) / groups)}); // (a launch's grid has fewer than 2^32 threads)
+    a.near = p.q_row_stride >= 0 && p.q_row_stride < (1 << 28) && (p.n_new + 1ll) * (p.q_row_stride + (long long)R * c.dim) < (1 << 29);
     a.plain = c.slot_stride >= 0 && c.slot_stride < (1 << 24);
     ps_carve ws{(char *)base};
     a.lse = ws.take<float>((size_t)(heads * rows));
@@ -978,11 +1053,12 @@ size_t psv_attn_space(int n_cu, const ps_kv_cache &c, const ps_cache_attn_params
         a.chunks = ws.take<int>(c.n_seqs);
     }
     if (p.weight_out && a.tiles <= 2) a.score = ws.take<float>((size_t)(heads * c.n_ctx * a.score_rows));
-    a.wparts = 1;
-    if (many && p.weight_out) { // parts of the rows until the chip is full twice, 128 rows at least
-        const long long blocks = heads * ((c.n_ctx + 255) / 256);
-        a.wparts = (int)std::max<long long>(1, std::min<long long>({(4 * n_cu + blocks - 1) / blocks, (rows + 127) / 128, 16}));
-        if (a.wparts > 1) a.wpart = ws.take<float>((size_t)(heads * a.wparts * c.n_ctx));
+    if (many && p.weight_out) { // up to 256 rows of slots enough to fill the chip: a block's rows are few; else the blocks' rows, which a sequence's length and the causal mask make unequal, are shared out
+        const long long blocks = (c.n_ctx + 255) / 256;
+        if (rows > 4 * QT || heads * blocks < 2 * n_cu) {
+            a.wgroups = (int)((2 * n_cu + heads - 1) / heads);
+            a.wpart = ws.take<float>((size_t)(heads * (a.wgroups + blocks) * 256));
+        }
     }
     if (!launch) return ws.at;
     a.k = (char *)c.k; a.v = (char *)c.v; a.out = (char *)p.out; a.q = (const char *)p.q; a.k_new = (const char *)p.k_new; a.v_new = (const char *)p.v_new;
