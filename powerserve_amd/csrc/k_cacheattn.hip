@@ -94,9 +94,9 @@ template <class E> __device__ __forceinline__ pv_f2 wide2(unsigned u) {
     if constexpr (__is_same(E, BF16)) return (pv_f2){__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u)};
     else { const h2 h = __builtin_bit_cast(h2, u); return (pv_f2){(float)h[0], (float)h[1]}; }
 }
-template <class E> __device__ __forceinline__ bool odd16(unsigned u) { // infinities or NaN among two 16-bit numbers
-    constexpr unsigned m = __is_same(E, BF16) ? 0x7f80u : 0x7c00u;
-    return (u & m) == m || (u >> 16 & m) == m;
+template <class E> __device__ __forceinline__ unsigned odd_bits(unsigned u) { // not 0: infinities or NaN among two 16-bit numbers (an exponent of ones and one more is the sign's bit)
+    constexpr unsigned m = __is_same(E, BF16) ? 0x7f807f80u : 0x7c007c00u, one = __is_same(E, BF16) ? 0x00800080u : 0x04000400u;
+    return ((u & m) + one) & 0x80008000u;
 }
 // the infinities and NaN of two 16-bit numbers alone, or the others alone
 template <class E> __device__ __forceinline__ unsigned without_odd(unsigned u) {
@@ -290,7 +290,7 @@ __global__ __launch_bounds__(256, E::SIZE == 4 ? 1 : 2) void cache_attn_kernel(c
 #pragma unroll
                 for (int x = 0; x < 4; x++) {
                     if constexpr (E::SIZE == 2) {
-                        if (odd16<E>(vf[i][x])) { odd = true; vf[i][x] = without_odd<E>(vf[i][x]); }
+                        if (odd_bits<E>(vf[i][x])) { odd = true; vf[i][x] = without_odd<E>(vf[i][x]); }
                     } else if (odd32(__uint_as_float(vf[i][x]))) { odd = true; vf[i][x] = 0u; }
                 }
             }
@@ -670,10 +670,15 @@ __global__ __launch_bounds__(256, 2) void cache_rows_kernel(const ca_args a) {
 #pragma unroll
         for (int i = 0; i < ST; i++) {
             const int x = tid + 256 * i, r = x / PER, e = x % PER * 8;
-            if (kb + KEYS > L.n0 && kb + r >= L.n0) { // a new token's infinities and NaN stay out of the products
+            if (kb + KEYS > L.n0) { // a new token's infinities and NaN stay out of the products
+                unsigned any = 0;
 #pragma unroll
-                for (int y = 0; y < 4; y++)
-                    if (odd16<E>(vs[i][y])) { odd = true; vs[i][y] = without_odd<E>(vs[i][y]); }
+                for (int y = 0; y < 4; y++) any |= odd_bits<E>(vs[i][y]);
+                if (any && kb + r >= L.n0) {
+                    odd = true;
+#pragma unroll
+                    for (int y = 0; y < 4; y++) vs[i][y] = without_odd<E>(vs[i][y]);
+                }
             }
             *(pv_u4 *)(kl[buf] + r * KR + e) = ks[i];
             *(pv_u4 *)(vl[buf] + r * VR + e) = vs[i];
@@ -693,6 +698,14 @@ __global__ __launch_bounds__(256, 2) void cache_rows_kernel(const ca_args a) {
         for (int st = 0; st < KS; st++)
 #pragma unroll
             for (int u = 0; u < 2; u++) z[u] = mfma32<E>(*(const pv_u4 *)(kl[cur] + (32 * u + c) * KR + 16 * st + 8 * h), qf[st], z[u]);
+        // keys are loaded six products ahead, not two as the compiler has them (2048 tokens behind 2047: 152 us, 149 so)
+        __builtin_amdgcn_sched_group_barrier(0x100, 6, 0);
+#pragma unroll
+        for (int i = 0; i < 2 * KS - 6; i++) {
+            __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        }
+        __builtin_amdgcn_sched_group_barrier(0x8, 6, 0);
         if (kb + KEYS > (a.tree ? L.n0 : L.n0 + first + 1)) {
 #pragma unroll
             for (int u = 0; u < 2; u++) {
