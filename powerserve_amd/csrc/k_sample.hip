@@ -43,17 +43,17 @@ struct smp_args {
 struct F16 { typedef _Float16 T; };
 struct BF16 { typedef __bf16 T; };
 struct F32 { typedef float T; };
-template <int N> __device__ __forceinline__ float at(const float (&l)[N], int e) { // of registers
-    float v = l[0];
+// One of a few registers.  (A chain of choices among the l[i] would be made a load of an array in memory: 33 rows of 151936 bf16 numbers, the second pass 31 us, 21 so.)
+template <int N> __device__ __forceinline__ float at(const float (&l)[N], int e) {
+    unsigned v = 0;
 #pragma unroll
-    for (int i = 1; i < N; i++) v = e == i ? l[i] : v;
-    return v;
+    for (int i = 0; i < N; i++) v |= e == i ? __float_as_uint(l[i]) : 0u;
+    return __uint_as_float(v);
 }
 __device__ __forceinline__ bool candidate(float l) { return l > -INFINITY; } // (NaN is none)
-// f(numbers, index of the first) for the pieces of 16 bytes of the numbers lo .. hi of a row, four loads of a thread in flight.  What lies before the first whole piece and behind the last goes in
-// a piece each, filled up with minus infinity.  ROLLED: one piece after the other in one place of the code -- a part of a row is a few pieces a thread, and what that costs is fetching instructions
-// (a row's second pass over 64 parts: 11 us unrolled, 8 so); a whole row's passes run unrolled.
-template <class E, int THREADS, bool ROLLED, class F>
+// f(numbers, index of the first) for the pieces of 16 bytes of the numbers lo .. hi of a row: a piece is worked on with the next three and the one that takes its place on their way.  What lies before
+// the first whole piece and behind the last goes in a piece each, filled up with minus infinity.
+template <class E, int THREADS, class F>
 __device__ __forceinline__ void each(const typename E::T *row, int lo, int hi, F f) {
     typedef typename E::T T;
     constexpr int PER = 16 / sizeof(T);
@@ -71,18 +71,7 @@ __device__ __forceinline__ void each(const typename E::T *row, int lo, int hi, F
         __builtin_memcpy(x, &v, 16);
         give(x, head + u * PER);
     };
-    if constexpr (ROLLED) {
-        for (int i = tid; i < body; i += 4 * THREADS) {
-            pv_u4 v[4];
-#pragma unroll
-            for (int j = 0; j < 4; j++) v[j] = p[min(i + j * THREADS, body - 1)];
-#pragma unroll 1
-            for (int u = i; u < body && u < i + 4 * THREADS; u += THREADS) {
-                piece(v[0], u);
-                v[0] = v[1]; v[1] = v[2]; v[2] = v[3];
-            }
-        }
-    } else if (tid < body) { // a piece is worked on with the next three and the one that takes its place on their way
+    if (tid < body) {
         pv_u4 v[4];
 #pragma unroll
         for (int j = 0; j < 4; j++) v[j] = p[min(tid + j * THREADS, body - 1)];
@@ -247,7 +236,7 @@ __global__ __launch_bounds__(256) void sample_top_kernel(const smp_args a) {
     int lo, hi;
     part_of(a, blockIdx.x, lo, hi);
     float m = -INFINITY;
-    each<E, 256, false>(row, lo, hi, [&](const auto &l, int) {
+    each<E, 256>(row, lo, hi, [&](const auto &l, int) {
 #pragma unroll
         for (float x : l) m = fmaxf(m, x);
     });
@@ -257,9 +246,9 @@ __global__ __launch_bounds__(256) void sample_top_kernel(const smp_args a) {
     if (threadIdx.x % lanes == 0) a.top[r * 1024 + blockIdx.x * (256 / lanes) + threadIdx.x / lanes] = m;
 }
 // the second pass over lo .. hi: at or above the bound into the head (room for `most`; n counts on); where the others count, all into the bins
-template <class E, bool ROLLED>
+template <class E>
 __device__ __forceinline__ void second_pass(const typename E::T *row, int lo, int hi, const row_of &w, const passes &ps, u64 *head, int *n, int most, unsigned *cnt, u64 *sum, const double *table) {
-    each<E, PICK, ROLLED>(row, lo, hi, [&](const auto &l, int first) {
+    each<E, PICK>(row, lo, hi, [&](const auto &l, int first) {
         constexpr int PER = sizeof(l) / 4;
         float m = l[0];
 #pragma unroll
@@ -303,7 +292,7 @@ __global__ __launch_bounds__(PICK) void sample_head_kernel(const smp_args a) {
     __syncthreads();
     int lo, hi;
     part_of(a, blockIdx.x, lo, hi);
-    second_pass<E, true>(row, lo, hi, w, ps, list, &n_list, PART_HEAD, cnt, sum, table);
+    second_pass<E>(row, lo, hi, w, ps, list, &n_list, PART_HEAD, cnt, sum, table);
     __syncthreads();
     // side by side with the other parts': sums between work-groups of different XCDs would be atomics at the memory (33 rows of 16 parts: 35 us of 47)
     const long long part = r * a.parts + blockIdx.x;
@@ -362,7 +351,7 @@ struct picker {
     template <class F> __device__ __forceinline__ void each_of_bin(int b, F f) {
         float lo, hi;
         range_of(b, lo, hi);
-        each<E, PICK, false>(row, 0, a.n, [&](const auto &l, int first) {
+        each<E, PICK>(row, 0, a.n, [&](const auto &l, int first) {
             unsigned some = 0;
 #pragma unroll
             for (int e = 0; e < (int)(sizeof(l) / 4); e++) some |= (l[e] >= lo && l[e] <= hi ? 1u : 0u) << e;
@@ -547,7 +536,7 @@ __global__ __launch_bounds__(PICK) void sample_pick_kernel(const smp_args a) {
     float mine = -INFINITY, top;
     passes ps;
     if constexpr (OWN)
-        each<E, PICK, false>(row, 0, a.n, [&](const auto &l, int) {
+        each<E, PICK>(row, 0, a.n, [&](const auto &l, int) {
 #pragma unroll
             for (float x : l) mine = fmaxf(mine, x);
         });
@@ -577,7 +566,7 @@ __global__ __launch_bounds__(PICK) void sample_pick_kernel(const smp_args a) {
     if (threadIdx.x < 4) { s.n[threadIdx.x] = 0; s.place[threadIdx.x] = NB; s.n_head = s.n_few = 0; }
     __syncthreads();
     if constexpr (OWN) {
-        second_pass<E, false>(row, 0, a.n, w, ps, s.head, &s.n_head, HEAD, cnt, sum, s.table);
+        second_pass<E>(row, 0, a.n, w, ps, s.head, &s.n_head, HEAD, cnt, sum, s.table);
         __syncthreads();
     } else { // the parts' heads one behind the other, a wave a part
         const int lane = threadIdx.x & 63;
@@ -604,7 +593,7 @@ __global__ __launch_bounds__(PICK) void sample_pick_kernel(const smp_args a) {
         in_head = 0;
         if (!ps.tail) {
             const passes all{NAN, true, true}; // (nothing is at or above it)
-            second_pass<E, true>(row, 0, a.n, w, all, s.head, &s.n[0], 0, cnt, sum, s.table);
+            second_pass<E>(row, 0, a.n, w, all, s.head, &s.n[0], 0, cnt, sum, s.table);
         }
     } else if (!ps.tail) {
         for (int i = threadIdx.x; i < s.n_head; i += PICK) add_to_bins(w, from_order(~(unsigned)(s.head[i] >> 32)), cnt, sum, s.table, true);
