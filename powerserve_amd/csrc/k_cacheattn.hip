@@ -3,9 +3,9 @@
 //   new tokens.  Weight of a slot = the sum over rows of its soft-max weights.
 //   cache_attn_kernel     16 RT rows of one kv head against a part of its keys; the waves of a work-group share the part (blocks of 32 keys in turn), join in LDS, and leave sum, maximum and
 //                         unnormed result of the part -- or the result itself where there is one part.  New rows go into the cache on the way.
-//   cache_join_kernel     the parts of a row together; a row's log-sum of weights is left for
-//   cache_score_kernel    up to 32 rows: a slot's weights from the scores, which cache_attn_kernel leaves beside its result
-//   cache_rows_kernel, cache_receive_kernel, cache_gather_kernel   the same for more rows of a 16-bit cache, cache_weight_kernel of an fp32 one: the scores are made again for the weights
+//   cache_join_kernel     the parts of a row together; up to 32 rows, beside that: a slot's weights from the scores, which cache_attn_kernel leaves beside its result
+//   cache_append_kernel, cache_rows_kernel, cache_receive_kernel, cache_gather_kernel   the same for more rows of a 16-bit cache, cache_weight_kernel of an fp32 one: the scores are made again for the
+//                         weights
 // S^T = K Q^T, so that a lane has one row and maximum and sum run over its own registers and two lane moves; the second product O^T = V^T P^T takes its 32 keys in any order that both operands
 // share, so a lane's weights are its piece of the operand as they are.  16-bit values pass through LDS, a wave's own stretch, and come back transposed (ds_read_b64_tr_b16: 4 keys x 16 numbers).
 // Lengths are read on the device; a part is ceil(length / parts) keys, so that a fixed grid serves any length.
@@ -43,6 +43,7 @@ struct ca_args {
     int share, *chunks; // few rows of up to 256 sequences: work-groups that all their keys are shared out to, and keys of a part of each sequence; else 0, NULL
     int plain; // offsets within 32 slots fit 32 bits
     int near;  // offsets within a sequence's q do
+    int scorers;      // few rows: work-groups of a kv head that make its weights from scores
     int wgroups;      // many rows: work-groups of a kv head that the weights' work is shared out to (0: one each 256 slots)
     float *wpart;     // [seq][kv head][work-group + block of 256 slots][256]: sums of a work-group's rows of a block
 };
@@ -446,80 +447,109 @@ __global__ __launch_bounds__(256, E::SIZE == 4 ? 1 : 2) void cache_attn_kernel(c
     }
 }
 
-// a row's parts: 16 lanes a row, 16 rows a work-group
+// Row r of a tile from the maxima and sums of its n parts, by four lanes 16 apart: the sum, its logarithm for the weights, and what each part's result is multiplied with (f: LDS, or NULL)
+template <class E> __device__ __forceinline__ float row_sum(const ca_args &a, const float *part, int n, int r, int lane4, float (*f)[16], float &lse) {
+    const long long step = 16 * (a.dim + 2);
+    const float *m = part + 16 * a.dim + r, *l = m + 16;
+    float top = -INFINITY, sum = 0.f;
+#pragma unroll 4
+    for (int i = lane4; i < n; i += 4) top = fmaxf(top, m[i * step]);
+    top = fmaxf(top, __shfl_xor(top, 16, 64));
+    top = fmaxf(top, __shfl_xor(top, 32, 64));
+    const float ms = top == -INFINITY ? 0.f : top;
+#pragma unroll 4
+    for (int i = lane4; i < n; i += 4) {
+        const float v = m[i * step], x = ex<E>(v - ms);
+        sum = fmaf(l[i * step], x, sum);
+        if (f) f[i][r] = v == -INFINITY ? 0.f : x; // (no result is left there)
+    }
+    sum += __shfl_xor(sum, 16, 64);
+    sum += __shfl_xor(sum, 32, 64);
+    lse = sum == 0.f ? INFINITY : ms + lg<E>(sum);
+    return sum;
+}
+// The first `joins` work-groups: a tile's parts together, 16 lanes a row; where it has fewer rows the others take parts of them.  Behind them, up to 32 rows: the weights from the scores that the
+// attention has left, a thread a key, `scorers` work-groups a kv head, which work the rows' sums out for themselves instead of waiting for them (32 sequences of up to 8191, one launch behind the
+// other: 16.5 us, 10.3 so; the number of work-groups, empty ones among them, is what it costs: 2 n_cu of them 17.5, 4 n_cu 12, one each 256 slots 17.5).
 template <class E>
-__global__ __launch_bounds__(256) void cache_join_kernel(const ca_args a) {
-    __shared__ float f[64][16]; // what a part's result is multiplied with
-    __shared__ float total[16];
-    int id = blockIdx.x;
+__global__ __launch_bounds__(256) void cache_join_kernel(const ca_args a, unsigned joins) {
+    __shared__ float f[64][16], total[16], lse[32];
+    __shared__ __attribute__((aligned(16))) float acc[16][132];
+    const int tid = threadIdx.x, lane = tid & 63, c = lane & 15;
+    unsigned id = blockIdx.x;
+    if (id >= joins) {
+        id -= joins;
+        const int s = (int)(id / a.scorers) / a.G, j0 = (int)(id % a.scorers) * 256;
+        const long long head = id / a.scorers;
+        const ca_lens L = lens_of(a, s);
+        if (j0 >= L.len) return;
+        const int rows = L.cnt * a.R, pitch = a.score_rows;
+        if (tid < 128) {
+            const int tile = tid >> 6, row = tile * 16 + c;
+            float x = INFINITY;
+            if (tile * 16 < rows) {
+                if (a.parts > 1) {
+                    const int chunk = chunk_of(a, s, L.len);
+                    row_sum<E>(a, a.part + (head * a.tiles + tile) * a.parts * (16 * (a.dim + 2)), (L.len + chunk - 1) / chunk, c, lane >> 4, nullptr, x);
+                } else if (row < rows) x = a.lse[head * a.T * a.R + row];
+            }
+            if (lane < 16) lse[row] = row < rows ? x : INFINITY;
+        }
+        __syncthreads();
+#pragma unroll 2
+        for (int j = j0 + tid; j < L.len; j += a.scorers * 256) {
+            const long long at = head * a.n_ctx + j;
+            float w = 0.f;
+            for (int row = 0; row < rows; row += 4) {
+                const pv_f4 z = *(const pv_f4 *)(a.score + at * pitch + row);
+#pragma unroll
+                for (int i = 0; i < 4; i++) w += lse[row + i] == INFINITY ? 0.f : ex<E>(z[i] - lse[row + i]);
+            }
+            a.weight_out[at] = j < L.n0 && a.weight ? a.weight[at] + w : w;
+        }
+        return;
+    }
     const int tile = id % a.tiles; id /= a.tiles;
-    const int g = id % a.G, s = id / a.G, rr = threadIdx.x >> 4, row = tile * 16 + rr;
+    const int g = id % a.G, s = id / a.G;
     const ca_lens L = lens_of(a, s);
-    if (tile * 16 >= L.cnt * a.R) return;
-    const int chunk = chunk_of(a, s, L.len), n = (L.len + chunk - 1) / chunk, t = token_of(a, row), hd = g * a.R + row - t * a.R;
+    const int rows = min(16, L.cnt * a.R - tile * 16);
+    if (rows <= 0) return;
+    const int chunk = chunk_of(a, s, L.len), n = (L.len + chunk - 1) / chunk;
     const long long step = 16 * (a.dim + 2);
     const float *part = a.part + (((long long)s * a.G + g) * a.tiles + tile) * a.parts * step;
-    if (threadIdx.x < 64) { // four lanes a row
-        const int r = threadIdx.x & 15, first = threadIdx.x >> 4;
-        float top = -INFINITY, sum = 0.f;
-        for (int i = first; i < n; i += 4) top = fmaxf(top, part[i * step + 16 * a.dim + r]);
-        top = fmaxf(top, __shfl_xor(top, 16, 64));
-        top = fmaxf(top, __shfl_xor(top, 32, 64));
-        const float ms = top == -INFINITY ? 0.f : top;
-        for (int i = first; i < n; i += 4) {
-            const float m = part[i * step + 16 * a.dim + r], x = ex<E>(m - ms);
-            sum = fmaf(part[i * step + 16 * a.dim + 16 + r], x, sum);
-            f[i][r] = m == -INFINITY ? 0.f : x; // (no result is left there)
-        }
-        sum += __shfl_xor(sum, 16, 64);
-        sum += __shfl_xor(sum, 32, 64);
-        if (first == 0) {
-            total[r] = sum;
-            if (tile * 16 + r < L.cnt * a.R) a.lse[((long long)s * a.G + g) * a.T * a.R + tile * 16 + r] = sum == 0.f ? INFINITY : ms + lg<E>(sum);
+    if (tid < 64) {
+        float x;
+        const float sum = row_sum<E>(a, part, n, c, lane >> 4, f, x);
+        if (lane < 16) {
+            total[c] = sum;
+            if (c < rows) a.lse[((long long)s * a.G + g) * a.T * a.R + tile * 16 + c] = x;
         }
     }
     __syncthreads();
-    if (row >= L.cnt * a.R) return;
-    const float inv = total[rr] == 0.f ? 0.f : 1.f / total[rr];
-    for (int e = (threadIdx.x & 15) * 4; e < a.dim; e += 64) {
+    const int nr = rows > 8 ? 16 : rows > 4 ? 8 : rows > 2 ? 4 : rows, groups = 16 / nr, slot = tid >> 4, rr = slot % nr, first = slot / nr;
+    const bool has = rr < rows && first < groups;
+    for (int e = c * 4; e < a.dim; e += 64) {
         pv_f4 v = {0.f, 0.f, 0.f, 0.f};
+        if (has)
 #pragma unroll 4
-        for (int i = 0; i < n; i++) {
-            const float w = f[i][rr];
-            const pv_f4 x = *(const pv_f4 *)(part + i * step + rr * a.dim + e);
+            for (int i = first; i < n; i += groups) {
+                const float w = f[i][rr];
+                const pv_f4 x = *(const pv_f4 *)(part + i * step + rr * a.dim + e);
 #pragma unroll
-            for (int y = 0; y < 4; y++) v[y] = w == 0.f ? v[y] : fmaf(x[y], w, v[y]);
-        }
+                for (int y = 0; y < 4; y++) v[y] = w == 0.f ? v[y] : fmaf(x[y], w, v[y]);
+            }
+        *(pv_f4 *)&acc[slot][e] = v;
+    }
+    __syncthreads();
+    if (slot >= rows) return;
+    const int row = tile * 16 + slot, t = token_of(a, row), hd = g * a.R + row - t * a.R;
+    const float inv = total[slot] == 0.f ? 0.f : 1.f / total[slot];
+    for (int e = c * 4; e < a.dim; e += 64) {
+        pv_f4 v = *(const pv_f4 *)&acc[slot][e];
+        for (int x = 1; x < groups; x++) v += *(const pv_f4 *)&acc[x * nr + slot][e];
         char *dst = a.out + s * a.o_seq + t * a.o_row + ((long long)hd * a.dim + e) * E::SIZE;
         if constexpr (E::SIZE == 2) *(pv_u2 *)dst = (pv_u2){round2<E>(v[0] * inv, v[1] * inv), round2<E>(v[2] * inv, v[3] * inv)};
         else *(pv_f4 *)dst = (pv_f4){v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv};
-    }
-}
-
-// the weights of few rows from the scores that the attention has left, a thread a key
-constexpr int SCORE_KEYS = 1024;
-template <class E>
-__global__ __launch_bounds__(256) void cache_score_kernel(const ca_args a) {
-    const int blocks = (a.n_ctx + SCORE_KEYS - 1) / SCORE_KEYS;
-    int id = blockIdx.x;
-    const int b = id % blocks; id /= blocks;
-    const int g = id % a.G, s = id / a.G;
-    const ca_lens L = lens_of(a, s);
-    if (b * SCORE_KEYS >= L.len) return;
-    const long long head = (long long)s * a.G + g;
-    const int rows = L.cnt * a.R, pitch = a.score_rows, end = min(L.len, (b + 1) * SCORE_KEYS);
-    __shared__ float lse[32];
-    if (threadIdx.x < 32) lse[threadIdx.x] = (int)threadIdx.x < rows ? a.lse[head * a.T * a.R + threadIdx.x] : INFINITY;
-    __syncthreads();
-    for (int j = b * SCORE_KEYS + threadIdx.x; j < end; j += 256) {
-        const long long at = head * a.n_ctx + j;
-        float w = 0.f;
-        for (int row = 0; row < rows; row += 4) {
-            const pv_f4 z = *(const pv_f4 *)(a.score + at * pitch + row);
-#pragma unroll
-            for (int i = 0; i < 4; i++) w += lse[row + i] == INFINITY ? 0.f : ex<E>(z[i] - lse[row + i]);
-        }
-        a.weight_out[at] = j < L.n0 && a.weight ? a.weight[at] + w : w;
     }
 }
 
@@ -1028,7 +1058,7 @@ void launch_attn(const ca_args &a, bool many, hipStream_t st) {
             const int row_bytes = a.dim * 2, pieces = a.T * a.G * (row_bytes / 16);
             if (a.k_new) hipLaunchKernelGGL(cache_append_kernel, dim3((unsigned)((pieces + 255) / 256), (unsigned)a.n_seqs), dim3(256), 0, st, a, row_bytes);
             hipLaunchKernelGGL((cache_rows_kernel<E, DP>), dim3((unsigned)(heads * a.parts * ((a.T * a.R + ROWS - 1) / ROWS))), dim3(256), 0, st, a);
-            if (a.parts > 1) hipLaunchKernelGGL((cache_join_kernel<E>), dim3((unsigned)(heads * a.tiles)), dim3(256), 0, st, a);
+            if (a.parts > 1) hipLaunchKernelGGL((cache_join_kernel<E>), dim3((unsigned)(heads * a.tiles)), dim3(256), 0, st, a, (unsigned)(heads * a.tiles));
             if (!a.weight_out) return;
             hipLaunchKernelGGL((cache_receive_kernel<E, DP>), dim3((unsigned)(heads * (a.wgroups ? a.wgroups : (a.n_ctx + 255) / 256))), dim3(256), 0, st, a);
             if (a.wgroups) hipLaunchKernelGGL(cache_gather_kernel, dim3((unsigned)((a.n_ctx + 255) / 256), (unsigned)a.G, (unsigned)a.n_seqs), dim3(256), 0, st, a);
@@ -1039,10 +1069,10 @@ void launch_attn(const ca_args &a, bool many, hipStream_t st) {
     const unsigned grid = (unsigned)(a.share ? a.share + heads * ((a.tiles + 1) / 2) : heads * a.parts * ((a.tiles + 1) / 2)); // (shared out: a sequence's last part may be a short one)
     if (a.tiles > 1) hipLaunchKernelGGL((cache_attn_kernel<E, DP, 2>), dim3(grid), dim3(256), 0, st, a);
     else hipLaunchKernelGGL((cache_attn_kernel<E, DP, 1>), dim3(grid), dim3(256), 0, st, a);
-    if (a.parts > 1) hipLaunchKernelGGL((cache_join_kernel<E>), dim3((unsigned)(heads * a.tiles)), dim3(256), 0, st, a);
-    if (!a.weight_out) return;
-    if (a.tiles <= 2) hipLaunchKernelGGL((cache_score_kernel<E>), dim3((unsigned)(heads * ((a.n_ctx + SCORE_KEYS - 1) / SCORE_KEYS))), dim3(256), 0, st, a);
-    else if constexpr (E::SIZE == 4) hipLaunchKernelGGL((cache_weight_kernel<E, DP>), dim3((unsigned)(heads * ((a.n_ctx + 63) / 64))), dim3(256), 0, st, a);
+    const unsigned joins = a.parts > 1 ? (unsigned)(heads * a.tiles) : 0, scores = a.weight_out && a.tiles <= 2 ? (unsigned)(heads * a.scorers) : 0;
+    if (joins + scores) hipLaunchKernelGGL((cache_join_kernel<E>), dim3(joins + scores), dim3(256), 0, st, a, joins);
+    if (!a.weight_out || a.tiles <= 2) return;
+    if constexpr (E::SIZE == 4) hipLaunchKernelGGL((cache_weight_kernel<E, DP>), dim3((unsigned)(heads * ((a.n_ctx + 63) / 64))), dim3(256), 0, st, a);
 }
 } // namespace
 
@@ -1065,6 +1095,7 @@ size_t psv_attn_space(int n_cu, const ps_kv_cache &c, const ps_cache_attn_params
         a.share = 4 * n_cu;
         a.chunks = ws.take<int>(c.n_seqs);
     }
+    a.scorers = (int)std::max<long long>(1, std::min<long long>((c.n_ctx + 255) / 256, 8 * n_cu / heads));
     if (p.weight_out && a.tiles <= 2) a.score = ws.take<float>((size_t)(heads * c.n_ctx * a.score_rows));
     if (many && p.weight_out) { // up to 256 rows of slots enough to fill the chip: a block's rows are few; else the blocks' rows, which a sequence's length and the causal mask make unequal, are shared out
         const long long blocks = (c.n_ctx + 255) / 256;

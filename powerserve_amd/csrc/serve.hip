@@ -44,7 +44,7 @@ const char *wrong_attn(const ps_kv_cache *k, const ps_cache_attn_params *p) {
     if (p->n_new < 0 || p->n_new > k->n_ctx) return "more new tokens than slots";
     if (!(std::fabs(p->scale) <= 1e30f)) return "the scale is not a number, or above 1e30";
     const int64_t heads = (int64_t)k->n_seqs * k->kv_heads, rows = (int64_t)p->n_new * (p->heads / k->kv_heads);
-    if (rows > (1 << 24) || rows * (p->heads / k->kv_heads) > UINT32_MAX || (int64_t)p->n_new * k->kv_heads * 32 > INT32_MAX || heads * ((rows + 15) / 16) > MOST_GROUPS - 65536 || heads * ((k->n_ctx + 63) / 64) > MOST_GROUPS) return "too many rows or slots";
+    if (rows > (1 << 24) || rows * (p->heads / k->kv_heads) > UINT32_MAX || (int64_t)p->n_new * k->kv_heads * 32 > INT32_MAX || heads * ((rows + 15) / 16) > MOST_GROUPS / 2 - 65536 || heads * ((k->n_ctx + 63) / 64) > MOST_GROUPS) return "too many rows or slots";
     if (!k->n_seqs || !p->n_new) return nullptr;
     if (!p->q || !p->out || p->q == p->out) return "q and out are missing or the same";
     if (!p->k_new != !p->v_new) return "new keys and values come together";
