@@ -232,6 +232,7 @@ __global__ __launch_bounds__(256) void adapt_up_kernel(const ad_args a) {
         for (int i = tid; i < r16 * 8; i += 256) { // two ranks of a token
             const int t = i & 15, r = (i >> 4) * 2;
             float v[2] = {0.f, 0.f};
+#pragma unroll 4
             for (int p = 0; p < a.parts; p++) {
                 const float *h = a.h + (((long long)p * gridDim.x + b) * a.RP + r) * TILE + t;
                 v[0] += h[0];
@@ -297,8 +298,8 @@ __global__ __launch_bounds__(256) void adapt_up_kernel(const ad_args a) {
 size_t psv_adapt_space(const ps_adapters &s, int x_dtype, const void *x, int64_t ldx, int T, const int32_t *ids, const float *base_out, float *out, int64_t ldo, void *base, bool launch, hipStream_t st) {
     ad_args a{};
     const int most = T <= ADAPT_SELF ? T : std::min<int64_t>(T, (int64_t)s.n_slots + 1 + T / TILE); // tiles there can be
-    // parts of K so that the tiles of a batch of one adapter each fill the chip: 128 numbers of K a wave at least
-    a.parts = (int)std::max<int64_t>(1, std::min<int64_t>({(2 * s.n_cu + most - 1) / most, s.KP / 512, 16}));
+    // parts of K so that the tiles of a batch of one adapter each fill the chip four times, 64 numbers of K a wave at least (64 adapters of rank 64, K 4096: 13 parts, 10.3 us; 7 parts, 13.8)
+    a.parts = (int)std::max<int64_t>(1, std::min<int64_t>({(4 * s.n_cu + most - 1) / most, s.KP / 256, 16}));
     ps_carve ws{(char *)base};
     a.h = ws.take<float>((size_t)a.parts * most * s.RP * TILE);
     int32_t *count = nullptr;
