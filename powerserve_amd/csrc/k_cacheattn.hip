@@ -190,7 +190,7 @@ __global__ __launch_bounds__(256, E::SIZE == 4 ? 1 : 2) void cache_attn_kernel(c
     }
     int id = blockIdx.x;
     if (id >= items) return;
-    const int rb = id % blocks; id /= blocks;
+    const int rb = blocks - 1 - id % blocks; id /= blocks; // (the rows with the most causal keys first)
     int g, s, split, chunk;
     if (a.share) {
         g = id % a.G; id /= a.G;
@@ -209,8 +209,11 @@ __global__ __launch_bounds__(256, E::SIZE == 4 ? 1 : 2) void cache_attn_kernel(c
     }
     const ca_lens L = lens_of(a, s);
     chunk = a.share ? chunk_at[s] : chunk_of(a, s, L.len);
-    const int k0 = split * chunk, k1 = min(L.len, k0 + chunk);
-    if (L.cnt == 0 || k0 >= L.len || rb * RT * 16 >= L.cnt * a.R) return;
+    const int k0 = split * chunk, rows_ = L.cnt * a.R;
+    if (L.cnt == 0 || k0 >= L.len || rb * RT * 16 >= rows_) return;
+    // the last row block sees all keys, and takes the new ones into the cache; the others stop where none of their rows sees any (scores that are asked for are asked for whole)
+    const bool last = (rb + 1) * RT * 16 >= rows_;
+    const int k1 = min(min(L.len, k0 + chunk), last || a.tree || a.score ? L.len : L.n0 + token_of(a, rb * RT * 16 + RT * 16 - 1) + 1);
     const char *kb_ = a.k + s * a.seq + g * a.head, *vb_ = a.v + s * a.seq + g * a.head;
     const char *kn = a.k_new ? a.k_new + s * a.new_seq + (long long)g * a.dim * E::SIZE : nullptr, *vn = a.k_new ? a.v_new + s * a.new_seq + (long long)g * a.dim * E::SIZE : nullptr;
     auto row_at = [&](const char *held, const char *fresh, int j) { return fresh && j >= L.n0 ? fresh + (j - L.n0) * a.new_row : held + j * a.slot; };
@@ -268,7 +271,7 @@ __global__ __launch_bounds__(256, E::SIZE == 4 ? 1 : 2) void cache_attn_kernel(c
     if (k0 + wave * 32 < k1) fetch(k0 + wave * 32);
     for (int kb = k0 + wave * 32; kb < k1; kb += 128) {
         if (kb + 32 > L.n0) { // new tokens among the keys
-            if (kn && rb == 0) {
+            if (kn && last) {
 #pragma unroll
                 for (int u = 0; u < 2; u++) {
                     const int j = kb + 16 * u + c;
@@ -287,7 +290,7 @@ __global__ __launch_bounds__(256, E::SIZE == 4 ? 1 : 2) void cache_attn_kernel(c
                 const int r = E::SIZE == 2 ? i * RPI + vr : 16 * (i / (4 * (DP / 64))) + 4 * q4 + i / (DP / 64) % 4, e = E::SIZE == 2 ? vc : 64 * (i % (DP / 64)) + 4 * c;
                 const int j = kb + r;
                 if (j < L.n0 || j >= k1 || e >= a.dim) continue;
-                if (vn && rb == 0) *(pv_u4 *)(a.v + s * a.seq + g * a.head + j * a.slot + e * E::SIZE) = vf[i];
+                if (vn && last) *(pv_u4 *)(a.v + s * a.seq + g * a.head + j * a.slot + e * E::SIZE) = vf[i];
 #pragma unroll
                 for (int x = 0; x < 4; x++) {
                     if constexpr (E::SIZE == 2) {
@@ -553,34 +556,72 @@ __global__ __launch_bounds__(256) void cache_join_kernel(const ca_args a, unsign
     }
 }
 
-// fp32 caches, more rows: 64 keys of a kv head; the waves take the 16-row tiles in turn
+// The work of the weights of a kv head: blocks of B slots, each with the tiles of 64 rows that can see a slot of it, one behind the other.  Work-group w of `groups` has the tiles n w / groups ..,
+// so that all have as many whatever the lengths are; where it stands changes the group, the block or both, so that group + block is a place of its own for each pair that meets.
+constexpr int QT = 64;
+template <int B> struct received {
+    long long n;  // tiles of all blocks
+    int tiles, held, groups; // of a block that all see; blocks that begin before the new tokens; work-groups that have any
+    const ca_args &a;
+    const ca_lens &L;
+    __device__ __forceinline__ int from(int b) const { return a.tree || b < held ? 0 : (b * B - L.n0) * a.R / QT; } // rows of tokens before a block's first slot see none of it
+    __device__ __forceinline__ received(const ca_args &a_, const ca_lens &L_) : a(a_), L(L_) {
+        tiles = (L.cnt * a.R + QT - 1) / QT;
+        const int blocks = (L.len + B - 1) / B;
+        held = a.tree ? blocks : min((L.n0 + B - 1) / B, blocks);
+        n = (long long)held * tiles;
+        for (int b = held; b < blocks; b++) n += tiles - from(b);
+        groups = (int)min((long long)a.wgroups, n);
+    }
+    // the block that tile `at` is in, and the first tile of it
+    __device__ __forceinline__ int block_of(long long at, long long &first) const {
+        int b = (int)min(at / tiles, (long long)held);
+        first = (long long)b * tiles;
+        while (b >= held && first + tiles - from(b) <= at) { first += tiles - from(b); b++; }
+        return b;
+    }
+    __device__ __forceinline__ long long start(int w) const { return n * w / groups; }
+    __device__ __forceinline__ int group_of(long long tile) const { return (int)(((tile + 1) * groups + n - 1) / n) - 1; }
+};
+// fp32 caches, more rows: 64 keys of a kv head against the rows that see any, the waves 16 of 64 rows each
 template <class E, int DP>
 __global__ __launch_bounds__(256) void cache_weight_kernel(const ca_args a) {
-    constexpr int NS = STEPS<E, DP>, KEYS = 64;
+    constexpr int NS = STEPS<E, DP>;
     __shared__ float red[4][64];
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, c = lane & 15, q4 = lane >> 4;
-    const int blocks = (a.n_ctx + KEYS - 1) / KEYS;
     int id = blockIdx.x;
-    const int b = id % blocks; id /= blocks;
-    const int g = id % a.G, s = id / a.G;
+    const int heads = a.n_seqs * a.G, hs = id % heads, s = hs / a.G, g = hs - s * a.G; id /= heads;
     const ca_lens L = lens_of(a, s);
-    if (b * KEYS >= L.len) return;
-    const int kb = b * KEYS;
-    const float *w_in = a.weight ? a.weight + ((long long)s * a.G + g) * a.n_ctx : nullptr;
-    float *w_out = a.weight_out + ((long long)s * a.G + g) * a.n_ctx;
-    pv_u4 kf[4][NS];
-    float w[4][4] = {};
-    if (kb < L.len) {
+    const int rows = L.cnt * a.R;
+    const received<64> work(a, L);
+    int b = id;
+    long long at = 0, end = 0, first = 0; // the tiles that are left, and the block's first
+    if (a.wgroups) {
+        if (id >= work.groups) return;
+        at = work.start(id);
+        end = work.start(id + 1);
+        b = work.block_of(at, first);
+    } else if (b * 64 >= L.len) return;
+    const float *lse = a.lse + (long long)hs * a.T * a.R;
+#pragma unroll 1
+    do {
+        int t0 = work.from(b), t1 = work.tiles;
+        if (a.wgroups) {
+            const int skip = t0;
+            t0 = skip + (int)(at - first);
+            t1 = (int)min((long long)t1, skip + (end - first));
+            at = first = first + work.tiles - skip;
+        }
+        const int kb = b * 64;
+        pv_u4 kf[4][NS];
+        float w[4][4] = {};
 #pragma unroll
         for (int u = 0; u < 4; u++) get_row<E, DP>(kf[u], a.k + s * a.seq + g * a.head + min(kb + 16 * u + c, L.len - 1) * a.slot, q4, a.dim);
-        const int rows = L.cnt * a.R;
-        const float *lse = a.lse + ((long long)s * a.G + g) * a.T * a.R;
-        for (int tile = wave; tile * 16 < rows; tile += 4) {
-            const int row = min(tile * 16 + c, rows - 1), t = token_of(a, row);
-            if (!a.tree && token_of(a, min(tile * 16 + 15, rows - 1)) < kb - L.n0) continue; // all these tokens come before these keys
+        for (int r0 = t0 * QT + wave * 16; r0 < min(t1 * QT, rows); r0 += QT) {
+            const int row = min(r0 + c, rows - 1), t = token_of(a, row);
             pv_u4 qf[NS];
             get_row<E, DP>(qf, a.q + s * a.q_seq + t * a.q_row + (long long)(g * a.R + row - t * a.R) * a.dim * E::SIZE, q4, a.dim);
-            const float ls = tile * 16 + c < rows ? lse[row] : INFINITY;
+            const float ls = r0 + c < rows ? lse[row] : INFINITY;
 #pragma unroll
             for (int u = 0; u < 4; u++) {
                 const pv_f4 z = dot<E, DP>(kf[u], qf);
@@ -592,20 +633,27 @@ __global__ __launch_bounds__(256) void cache_weight_kernel(const ca_args a) {
                 }
             }
         }
-    }
 #pragma unroll
-    for (int u = 0; u < 4; u++)
+        for (int u = 0; u < 4; u++)
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
+            for (int i = 0; i < 4; i++) {
 #pragma unroll
-            for (int x = 1; x < 16; x <<= 1) w[u][i] += __shfl_xor(w[u][i], x, 64);
-            if (c == 0) red[wave][16 * u + 4 * q4 + i] = w[u][i];
+                for (int x = 1; x < 16; x <<= 1) w[u][i] += __shfl_xor(w[u][i], x, 64);
+                if (c == 0) red[wave][16 * u + 4 * q4 + i] = w[u][i];
+            }
+        __syncthreads();
+        const int j = kb + lane;
+        if (wave == 0) {
+            const float sum = (red[0][lane] + red[1][lane]) + (red[2][lane] + red[3][lane]);
+            if (a.wgroups) a.wpart[(hs * (a.wgroups + (a.n_ctx + 63ll) / 64) + id + b) * 64 + lane] = sum;
+            else if (j < L.len) {
+                const long long to = (long long)hs * a.n_ctx + j;
+                a.weight_out[to] = j < L.n0 && a.weight ? a.weight[to] + sum : sum;
+            }
         }
-    __syncthreads();
-    const int j = kb + lane;
-    if (j >= L.len || wave) return;
-    const float sum = (red[0][lane] + red[1][lane]) + (red[2][lane] + red[3][lane]);
-    w_out[j] = j < L.n0 && w_in ? w_in[j] + sum : sum;
+        __syncthreads();
+        b++;
+    } while (at < end);
 }
 
 typedef float f16v __attribute__((ext_vector_type(16)));
@@ -836,26 +884,6 @@ __device__ __forceinline__ unsigned seen_by16(const ca_args &a, const ca_lens &L
     for (int i = 0; i < 16; i++) bits |= (x < 0 || (x < L.cnt && v[i]) ? 1u : 0u) << i;
     return bits;
 }
-// The work of the weights of a kv head: blocks of 256 slots, each with the tiles of 64 rows that can see a slot of it, one behind the other.  Work-group w of `groups` has the tiles n w / groups ..,
-// so that all have as many whatever the lengths are; where it stands changes the group, the block or both, so that group + block is a place of its own for each pair that meets.
-constexpr int QT = 64;
-struct received {
-    long long n;  // tiles of all blocks
-    int tiles, held, groups; // of a block that all see; blocks that begin before the new tokens; work-groups that have any
-    const ca_args &a;
-    const ca_lens &L;
-    __device__ __forceinline__ int from(int b) const { return a.tree || b < held ? 0 : (b * 256 - L.n0) * a.R / QT; } // rows of tokens before a block's first slot see none of it
-    __device__ __forceinline__ received(const ca_args &a_, const ca_lens &L_) : a(a_), L(L_) {
-        tiles = (L.cnt * a.R + QT - 1) / QT;
-        const int blocks = (L.len + 255) / 256;
-        held = a.tree ? blocks : min((L.n0 + 255) / 256, blocks);
-        n = (long long)held * tiles;
-        for (int b = held; b < blocks; b++) n += tiles - from(b);
-        groups = (int)min((long long)a.wgroups, n);
-    }
-    __device__ __forceinline__ long long start(int w) const { return n * w / groups; }
-    __device__ __forceinline__ int group_of(long long tile) const { return (int)(((tile + 1) * groups + n - 1) / n) - 1; }
-};
 // The weights that slots receive from many rows of a 16-bit cache: 256 keys of a kv head (a wave 64 of them, in registers) against the rows that see any, 64 at a time through LDS.  S = Q K^T here: a
 // lane has a key, so that the sum over rows is its registers' and its other half's; the sums of the work-groups that share a block are left side by side.
 template <class E, int DP>
@@ -868,16 +896,14 @@ __global__ __launch_bounds__(256, 2) void cache_receive_kernel(const ca_args a) 
     const int heads = a.n_seqs * a.G, hs = id % heads, s = hs / a.G, g = hs - s * a.G; id /= heads; // (neighbours: kv heads, as above)
     const ca_lens L = lens_of(a, s);
     const int rows = L.cnt * a.R;
-    const received work(a, L);
+    const received<256> work(a, L);
     int b, t0, t1;
     long long at = 0, end = 0, first = 0; // the tiles that are left, and the block's first
     if (a.wgroups) {
         if (id >= work.groups) return;
         at = work.start(id);
         end = work.start(id + 1);
-        b = (int)min(at / work.tiles, (long long)work.held);
-        first = (long long)b * work.tiles;
-        while (b >= work.held && first + work.tiles - work.from(b) <= at) { first += work.tiles - work.from(b); b++; }
+        b = work.block_of(at, first);
     } else {
         b = id;
         if (b * 256 >= L.len) return;
@@ -993,18 +1019,19 @@ __global__ __launch_bounds__(256, 2) void cache_receive_kernel(const ca_args a) 
     b++;
     } while (at < end);
 }
+template <int B>
 __global__ __launch_bounds__(256) void cache_gather_kernel(const ca_args a) { // the sums of a block's work-groups, in order
-    const int b = blockIdx.x, j = b * 256 + threadIdx.x, g = blockIdx.y, s = blockIdx.z;
+    const int j = blockIdx.x * 256 + threadIdx.x, b = j / B, g = blockIdx.y, s = blockIdx.z;
     const ca_lens L = lens_of(a, s);
     if (j >= L.len) return;
     const long long head = (long long)s * a.G + g, at = head * a.n_ctx + j;
-    const received work(a, L);
+    const received<B> work(a, L);
     float v = 0.f;
     if (work.n) {
         long long first = (long long)min(b, work.held) * work.tiles;
         for (int x = work.held; x < b; x++) first += work.tiles - work.from(x);
         const int w0 = work.group_of(first), w1 = work.group_of(first + work.tiles - work.from(b) - 1);
-        for (int w = w0; w <= w1; w++) v += a.wpart[(head * (a.wgroups + (a.n_ctx + 255ll) / 256) + w + b) * 256 + threadIdx.x];
+        for (int w = w0; w <= w1; w++) v += a.wpart[(head * (a.wgroups + (a.n_ctx + B - 1ll) / B) + w + b) * B + j % B];
     }
     a.weight_out[at] = j < L.n0 && a.weight ? a.weight[at] + v : v;
 }
@@ -1061,7 +1088,7 @@ void launch_attn(const ca_args &a, bool many, hipStream_t st) {
             if (a.parts > 1) hipLaunchKernelGGL((cache_join_kernel<E>), dim3((unsigned)(heads * a.tiles)), dim3(256), 0, st, a, (unsigned)(heads * a.tiles));
             if (!a.weight_out) return;
             hipLaunchKernelGGL((cache_receive_kernel<E, DP>), dim3((unsigned)(heads * (a.wgroups ? a.wgroups : (a.n_ctx + 255) / 256))), dim3(256), 0, st, a);
-            if (a.wgroups) hipLaunchKernelGGL(cache_gather_kernel, dim3((unsigned)((a.n_ctx + 255) / 256), (unsigned)a.G, (unsigned)a.n_seqs), dim3(256), 0, st, a);
+            if (a.wgroups) hipLaunchKernelGGL((cache_gather_kernel<256>), dim3((unsigned)((a.n_ctx + 255) / 256), (unsigned)a.G, (unsigned)a.n_seqs), dim3(256), 0, st, a);
             return;
         }
     }
@@ -1072,7 +1099,10 @@ void launch_attn(const ca_args &a, bool many, hipStream_t st) {
     const unsigned joins = a.parts > 1 ? (unsigned)(heads * a.tiles) : 0, scores = a.weight_out && a.tiles <= 2 ? (unsigned)(heads * a.scorers) : 0;
     if (joins + scores) hipLaunchKernelGGL((cache_join_kernel<E>), dim3(joins + scores), dim3(256), 0, st, a, joins);
     if (!a.weight_out || a.tiles <= 2) return;
-    if constexpr (E::SIZE == 4) hipLaunchKernelGGL((cache_weight_kernel<E, DP>), dim3((unsigned)(heads * ((a.n_ctx + 63) / 64))), dim3(256), 0, st, a);
+    if constexpr (E::SIZE == 4) {
+        hipLaunchKernelGGL((cache_weight_kernel<E, DP>), dim3((unsigned)(heads * (a.wgroups ? a.wgroups : (a.n_ctx + 63) / 64))), dim3(256), 0, st, a);
+        if (a.wgroups) hipLaunchKernelGGL((cache_gather_kernel<64>), dim3((unsigned)((a.n_ctx + 255) / 256), (unsigned)a.G, (unsigned)a.n_seqs), dim3(256), 0, st, a);
+    }
 }
 } // namespace
 
@@ -1097,11 +1127,11 @@ size_t psv_attn_space(int n_cu, const ps_kv_cache &c, const ps_cache_attn_params
     }
     a.scorers = (int)std::max<long long>(1, std::min<long long>((c.n_ctx + 255) / 256, 8 * n_cu / heads));
     if (p.weight_out && a.tiles <= 2) a.score = ws.take<float>((size_t)(heads * c.n_ctx * a.score_rows));
-    if (many && p.weight_out) { // up to 256 rows of slots enough to fill the chip: a block's rows are few; else the blocks' rows, which a sequence's length and the causal mask make unequal, are shared out
-        const long long blocks = (c.n_ctx + 255) / 256;
+    if (a.tiles > 2 && p.weight_out) { // up to 256 rows of slots enough to fill the chip: a block's rows are few; else the blocks' rows, which a sequence's length and the causal mask make unequal, are shared out
+        const long long block = many ? 256 : 64, blocks = (c.n_ctx + block - 1) / block;
         if (rows > 4 * QT || heads * blocks < 2 * n_cu) {
-            a.wgroups = (int)((2 * n_cu + heads - 1) / heads);
-            a.wpart = ws.take<float>((size_t)(heads * (a.wgroups + blocks) * 256));
+            a.wgroups = (int)(((many ? 2 : 4) * n_cu + heads - 1) / heads);
+            a.wpart = ws.take<float>((size_t)(heads * (a.wgroups + blocks) * block));
         }
     }
     if (!launch) return ws.at;
