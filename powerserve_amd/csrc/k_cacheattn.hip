@@ -95,12 +95,14 @@ template <class E> __device__ __forceinline__ pv_f2 wide2(unsigned u) {
     if constexpr (__is_same(E, BF16)) return (pv_f2){__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u)};
     else { const h2 h = __builtin_bit_cast(h2, u); return (pv_f2){(float)h[0], (float)h[1]}; }
 }
-template <class E> __device__ __forceinline__ unsigned odd_bits(unsigned u) { // not 0: infinities or NaN among two 16-bit numbers (an exponent of ones and one more is the sign's bit)
+template <class E> __device__ __forceinline__ unsigned odd_bits(unsigned u) { // not 0: infinities or NaN among the numbers of 32 bits (an exponent of ones and one more is the sign's bit)
+    if constexpr (E::SIZE == 4) return ((u & 0x7f800000u) + 0x00800000u) & 0x80000000u;
     constexpr unsigned m = __is_same(E, BF16) ? 0x7f807f80u : 0x7c007c00u, one = __is_same(E, BF16) ? 0x00800080u : 0x04000400u;
     return ((u & m) + one) & 0x80008000u;
 }
-// the infinities and NaN of two 16-bit numbers alone, or the others alone
+// the others of them alone
 template <class E> __device__ __forceinline__ unsigned without_odd(unsigned u) {
+    if constexpr (E::SIZE == 4) return odd_bits<E>(u) ? 0u : u;
     constexpr unsigned m = __is_same(E, BF16) ? 0x7f80u : 0x7c00u;
     return ((u & m) == m ? 0u : u & 0xffffu) | ((u >> 16 & m) == m ? 0u : u & 0xffff0000u);
 }
@@ -211,9 +213,9 @@ __global__ __launch_bounds__(256, E::SIZE == 4 ? 1 : 2) void cache_attn_kernel(c
     chunk = a.share ? chunk_at[s] : chunk_of(a, s, L.len);
     const int k0 = split * chunk, rows_ = L.cnt * a.R;
     if (L.cnt == 0 || k0 >= L.len || rb * RT * 16 >= rows_) return;
-    // the last row block sees all keys, and takes the new ones into the cache; the others stop where none of their rows sees any (scores that are asked for are asked for whole)
+    // row blocks but the last stop where none of their rows sees any key
     const bool last = (rb + 1) * RT * 16 >= rows_;
-    const int k1 = min(min(L.len, k0 + chunk), last || a.tree || a.score ? L.len : L.n0 + token_of(a, rb * RT * 16 + RT * 16 - 1) + 1);
+    const int k1 = min(min(L.len, k0 + chunk), last || a.tree ? L.len : L.n0 + token_of(a, rb * RT * 16 + RT * 16 - 1) + 1);
     const char *kb_ = a.k + s * a.seq + g * a.head, *vb_ = a.v + s * a.seq + g * a.head;
     const char *kn = a.k_new ? a.k_new + s * a.new_seq + (long long)g * a.dim * E::SIZE : nullptr, *vn = a.k_new ? a.v_new + s * a.new_seq + (long long)g * a.dim * E::SIZE : nullptr;
     auto row_at = [&](const char *held, const char *fresh, int j) { return fresh && j >= L.n0 ? fresh + (j - L.n0) * a.new_row : held + j * a.slot; };
@@ -242,7 +244,7 @@ __global__ __launch_bounds__(256, E::SIZE == 4 ? 1 : 2) void cache_attn_kernel(c
     constexpr int ES = E::SIZE;
     const unsigned ko = c * (unsigned)a.slot + q4 * 16, vo = ES == 2 ? vr * (unsigned)a.slot + vc * 2 : 4 * q4 * (unsigned)a.slot + c * 16;
     auto fetch = [&](int kb) {
-        if (RT == 1 && kb + 32 <= L.n0 && kb + 32 <= k1 && a.plain && a.dim == DP) { // slots that were held: one place a wave, and an offset a lane
+        if ((RT == 1 || ES == 4) && kb + 32 <= (kn ? min(L.n0, k1) : k1) && a.plain && a.dim == DP) { // slots of the cache: one place a wave, and an offset a lane
             const char *kt = kb_ + kb * a.slot, *vt = vb_ + kb * a.slot;
 #pragma unroll
             for (int u = 0; u < 2; u++)
@@ -271,7 +273,7 @@ __global__ __launch_bounds__(256, E::SIZE == 4 ? 1 : 2) void cache_attn_kernel(c
     if (k0 + wave * 32 < k1) fetch(k0 + wave * 32);
     for (int kb = k0 + wave * 32; kb < k1; kb += 128) {
         if (kb + 32 > L.n0) { // new tokens among the keys
-            if (kn && last) {
+            if (kn) {
 #pragma unroll
                 for (int u = 0; u < 2; u++) {
                     const int j = kb + 16 * u + c;
@@ -285,19 +287,22 @@ __global__ __launch_bounds__(256, E::SIZE == 4 ? 1 : 2) void cache_attn_kernel(c
                     }
                 }
             }
+            unsigned any = 0;
 #pragma unroll
-            for (int i = 0; i < VI; i++) {
-                const int r = E::SIZE == 2 ? i * RPI + vr : 16 * (i / (4 * (DP / 64))) + 4 * q4 + i / (DP / 64) % 4, e = E::SIZE == 2 ? vc : 64 * (i % (DP / 64)) + 4 * c;
-                const int j = kb + r;
-                if (j < L.n0 || j >= k1 || e >= a.dim) continue;
-                if (vn && last) *(pv_u4 *)(a.v + s * a.seq + g * a.head + j * a.slot + e * E::SIZE) = vf[i];
+            for (int i = 0; i < VI; i++)
 #pragma unroll
-                for (int x = 0; x < 4; x++) {
-                    if constexpr (E::SIZE == 2) {
+                for (int x = 0; x < 4; x++) any |= odd_bits<E>(vf[i][x]);
+            if (any || vn)
+#pragma unroll
+                for (int i = 0; i < VI; i++) {
+                    const int r = E::SIZE == 2 ? i * RPI + vr : 16 * (i / (4 * (DP / 64))) + 4 * q4 + i / (DP / 64) % 4, e = E::SIZE == 2 ? vc : 64 * (i % (DP / 64)) + 4 * c;
+                    const int j = kb + r;
+                    if (j < L.n0 || j >= k1 || e >= a.dim) continue;
+                    if (vn) *(pv_u4 *)(a.v + s * a.seq + g * a.head + j * a.slot + e * E::SIZE) = vf[i];
+#pragma unroll
+                    for (int x = 0; x < 4; x++)
                         if (odd_bits<E>(vf[i][x])) { odd = true; vf[i][x] = without_odd<E>(vf[i][x]); }
-                    } else if (odd32(__uint_as_float(vf[i][x]))) { odd = true; vf[i][x] = 0u; }
                 }
-            }
         }
         pv_u4 vk[VI];
         if constexpr (E::SIZE == 2) {
@@ -1078,12 +1083,15 @@ __global__ __launch_bounds__(256) void cache_count_kernel(int32_t *n_kv, const i
 }
 
 template <class E, int DP>
-void launch_attn(const ca_args &a, bool many, hipStream_t st) {
+void launch_attn(ca_args a, bool many, hipStream_t st) {
     const long long heads = (long long)a.n_seqs * a.G;
+    if (a.tiles > 2 && a.k_new) { // more than 32 rows: the new rows go into the cache first, and everything is read from there
+        const int row_bytes = a.dim * E::SIZE, pieces = a.T * a.G * (row_bytes / 16);
+        hipLaunchKernelGGL(cache_append_kernel, dim3((unsigned)((pieces + 255) / 256), (unsigned)a.n_seqs), dim3(256), 0, st, a, row_bytes);
+        a.k_new = a.v_new = nullptr;
+    }
     if constexpr (E::SIZE == 2) {
         if (many) {
-            const int row_bytes = a.dim * 2, pieces = a.T * a.G * (row_bytes / 16);
-            if (a.k_new) hipLaunchKernelGGL(cache_append_kernel, dim3((unsigned)((pieces + 255) / 256), (unsigned)a.n_seqs), dim3(256), 0, st, a, row_bytes);
             hipLaunchKernelGGL((cache_rows_kernel<E, DP>), dim3((unsigned)(heads * a.parts * ((a.T * a.R + ROWS - 1) / ROWS))), dim3(256), 0, st, a);
             if (a.parts > 1) hipLaunchKernelGGL((cache_join_kernel<E>), dim3((unsigned)(heads * a.tiles)), dim3(256), 0, st, a, (unsigned)(heads * a.tiles));
             if (!a.weight_out) return;
