@@ -109,22 +109,8 @@ __global__ __launch_bounds__(EV_THREADS) void evict_choose_kernel(const ev_args 
     const long long since = (long long)newest_ - a.recent; // positions above it are recent
     auto key_from = [&](int pos, float weight) { return pos < a.first || pos > since ? 0xffffffffu : order_of(weight); };
     auto key = [&](int j) { return a.in_lds ? keys[j] : key_from(p[j], w[j]); };
-    // The first digit's histogram, and the keys into LDS.  Weights of 0 (most of a soft-max's) and protected slots are many of one key each: a thread counts its own, they would be additions to one
-    // place of the LDS one behind the other (16384 slots, a third of them 0: 10 us).
-    constexpr unsigned ZERO = 0x80000000u, KEPT = 0xffffffffu;
-    int zeros = 0, kept_ = 0;
-    auto count = [&](unsigned k, int shift, int bits) {
-        if (k == ZERO) zeros++;
-        else if (k == KEPT) kept_++;
-        else atomicAdd(&hist[k >> shift & ((1u << bits) - 1)], 1u);
-    };
-    auto settle = [&](int shift, int bits) { // what the threads have counted into the histogram
-        zeros = wave_sums(zeros);
-        kept_ = wave_sums(kept_);
-        if (lane == 63 && zeros) atomicAdd(&hist[ZERO >> shift & ((1u << bits) - 1)], (unsigned)zeros);
-        if (lane == 63 && kept_) atomicAdd(&hist[KEPT >> shift & ((1u << bits) - 1)], (unsigned)kept_);
-        zeros = kept_ = 0;
-    };
+    // the first digit's histogram, and the keys into LDS
+    auto count = [&](unsigned k, int shift, int bits) { atomicAdd(&hist[k >> shift & ((1u << bits) - 1)], 1u); };
     for (int base = 4 * tid; base < n; base += AT_ONCE) {
         if (!once)
 #pragma unroll
@@ -155,7 +141,6 @@ __global__ __launch_bounds__(EV_THREADS) void evict_choose_kernel(const ev_args 
                 const unsigned x = key(j);
                 if ((x & mask) == found) count(x, shift, bits);
             }
-        settle(shift, bits);
         __syncthreads();
         // from the largest digit down: thread t has digits 2047 - 2 t and 2046 - 2 t
         const int hi = (int)hist[2047 - 2 * tid], lo = (int)hist[2046 - 2 * tid];
