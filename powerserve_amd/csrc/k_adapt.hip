@@ -6,6 +6,8 @@
 //   adapt_up_kernel    the parts' sums together, then 64 columns a wave of base + scale up h
 // A factor that is not bfloat16 -- x in fp32, h -- goes in as three bfloat16 numbers that add up to it, 24 bits together: every product is exact and every sum fp32.  Both matrices
 // together are read once per tile and step; what bounds a decode step is that read, a prompt the pass over base and out.
+// Measured: 253 tokens of 64 adapters of rank 64, 4096 to 14336, bf16: plan 6, down 10 us (34 MB), up 28 us for 146 MB, 5.2 TB/s (a large copy: 5.0); 2048 tokens of four, rank 16, 4096 to 4096: plan 5, down 9 us,
+// up 18 us for 67 MB, 3.7 TB/s; 4 tokens: 5 + 5 us, latency.
 #include "ps_serve.h"
 
 #include <algorithm>

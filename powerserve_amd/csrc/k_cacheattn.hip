@@ -9,6 +9,9 @@
 // S^T = K Q^T, so that a lane has one row and maximum and sum run over its own registers and two lane moves; the second product O^T = V^T P^T takes its 32 keys in any order that both operands
 // share, so a lane's weights are its piece of the operand as they are.  16-bit values pass through LDS, a wave's own stretch, and come back transposed (ds_read_b64_tr_b16: 4 keys x 16 numbers).
 // Lengths are read on the device; a part is ceil(length / parts) keys, so that a fixed grid serves any length.
+// Measured, dim 128, 32 query heads of 8, bf16: one token of 32 sequences that hold 17 to 8191 slots, with weights, 51 + 10 us, 187 MB of keys and values at 3.7 TB/s (a plain read of 1 GiB: 4.0) -- memory
+// bounds it; 2048 tokens behind 2047, 138 + 88 us for 103 and 52 GFLOP, 750 and 590 TFLOP/s (the library's product of 8192^3: 1130) -- the vector units' soft-max beside the matrix units, which two
+// waves a SIMD overlap in part; one token behind 100 in fp32 (14 heads of 2, dim 64), 8 + 4 us: latency of lengths, keys, sums and two launches.
 #include "ps_serve.h"
 
 #include <algorithm>
@@ -150,6 +153,8 @@ __device__ __forceinline__ pv_f4 dot(const frame<E, DP> &k, const frame<E, DP> &
 
 constexpr int VPAD = 16; // numbers behind a value row in LDS: four rows of eight banks side by side
 
+// The next block's keys and values are on their way while one is worked on; two work-groups a CU (three or four leave no registers for that: slower).  fp32 runs on v_mfma_f32_16x16x4, 1024 tokens behind 1000
+// at 52 TFLOP/s (the library's product: 153): one wave a SIMD, whose loads and soft-max nothing overlaps.
 template <class E, int DP, int RT>
 __global__ __launch_bounds__(256, E::SIZE == 4 ? 1 : 2) void cache_attn_kernel(const ca_args a) {
     constexpr int NS = STEPS<E, DP>, ND = DP / 16, OP = DP + 4, VR = DP + VPAD;
@@ -588,7 +593,7 @@ template <int B> struct received {
     __device__ __forceinline__ long long start(int w) const { return n * w / groups; }
     __device__ __forceinline__ int group_of(long long tile) const { return (int)(((tile + 1) * groups + n - 1) / n) - 1; }
 };
-// fp32 caches, more rows: 64 keys of a kv head against the rows that see any, the waves 16 of 64 rows each
+// fp32 caches, more rows: 64 keys of a kv head against the rows that see any, the waves 16 of 64 rows each (1024 tokens behind 1000, 14 heads of 2, dim 64: 65 us, 43 TFLOP/s; a work-group a block: 251)
 template <class E, int DP>
 __global__ __launch_bounds__(256) void cache_weight_kernel(const ca_args a) {
     constexpr int NS = STEPS<E, DP>;
@@ -684,7 +689,8 @@ __global__ __launch_bounds__(256) void cache_append_kernel(const ca_args a, int 
 // Many rows of a 16-bit cache: 128 of a kv head against a part of its keys, a wave 32 of them against all, 64 keys at a time through two LDS stages that the four waves fill.  The products are
 // v_mfma_f32_32x32x16: S^T = K Q^T with the queries in registers (a lane: one row, 16 keys a tile), O^T = V^T P^T with the weights as they come, values transposed on their way out of LDS.
 // The weights go into the second product as one 16-bit number each (rounded like the result is: 2^-9 of a weight, bf16, to either side); their sum is taken before they are rounded.
-// What bounds it: the first operands of both products from LDS, 32 KB a wave and 64 keys beside 32 instructions of 32 clocks, and as many clocks of soft-max, which two work-groups a CU overlap.
+// What bounds it: a wave and 64 keys take 32 matrix instructions of 32 clocks, 32 KB of operands from LDS and some 230 vector instructions; two waves a SIMD overlap them in part, at the 2.0 GHz that the card holds
+// under it (2048 tokens behind 2047: 138 us, 750 TFLOP/s).  Work-groups of eight waves read a tile for twice the rows, and their sizes even out worse (168 us there; 8192 tokens 5 % faster).
 constexpr int ROWS = 128, KEYS = 64;
 // the same for a lane's 16 keys of a tile of 32, x + 8 (i / 4) + i % 4
 __device__ __forceinline__ unsigned sees16(const ca_args &a, const ca_lens &L, int s, int tok, int x) {
@@ -890,7 +896,8 @@ __device__ __forceinline__ unsigned seen_by16(const ca_args &a, const ca_lens &L
     return bits;
 }
 // The weights that slots receive from many rows of a 16-bit cache: 256 keys of a kv head (a wave 64 of them, in registers) against the rows that see any, 64 at a time through LDS.  S = Q K^T here: a
-// lane has a key, so that the sum over rows is its registers' and its other half's; the sums of the work-groups that share a block are left side by side.
+// lane has a key, so that the sum over rows is its registers' and its other half's (S^T: 32 sums a lane and 160 moves between lanes, 8 us of 24 of a small step); the sums of the work-groups that share a block are
+// left side by side.  What bounds it: 96 vector instructions, 32 of them 2^x, beside 16 matrix instructions.
 template <class E, int DP>
 __global__ __launch_bounds__(256, 2) void cache_receive_kernel(const ca_args a) {
     constexpr int KS = DP / 16, QR = DP + 8, PER = DP / 8, ST = QT * PER / 256;

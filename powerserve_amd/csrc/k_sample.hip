@@ -9,6 +9,8 @@
 //   high temperature) every digit is a pass over the row.
 //   Weights e^-z -- of z in 64 bits, e^-(bin / 32) from a table times a polynomial of what is left, below 1/32 -- are added as whole multiples of 2^-scale of the largest one: any order of
 //   work gives the same sums, and what a weight is off by, 2^-28 of it to either side alike, moves one draw in millions to a neighbour, where 32-bit sums would move one in some thousands.
+// Measured: one row of 128256 in fp32, 3 + 7 + 10 us, the latency of the passes and of a stage's steps; 33 rows of 151936 in bf16, 5 + 21 + 17, the second pass's 64-bit arithmetic and its additions to the LDS; 256
+// such rows of fp32 in one launch, 116 us: 15 the first pass (131 MB), 30 the second where the head alone counts and 55 where all do, 14 for each place that lies behind the head, 1 for one in it.
 //   sample_top_kernel   the first pass over a part of a row
 //   sample_head_kernel  the second pass over a part
 //   sample_pick_kernel  the stages; with few parts of a row (many rows) it makes both passes itself
