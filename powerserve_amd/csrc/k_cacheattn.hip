@@ -43,7 +43,7 @@ struct ca_args {
     float *score; // [seq][kv head][slot][score_rows]: scores of few rows for the weights, or NULL
     float *lse;  // [seq][kv head][T R] logarithm, in the scores' units, of the sum of weights (+inf: no weights)
     int parts, tiles, score_rows; // tiles of 16 rows
-    int share, *chunks; // few rows of up to 256 sequences: work-groups that all their keys are shared out to, and keys of a part of each sequence; else 0, NULL
+    int share, *chunks; // 2 to 256 sequences in parts: work-groups that all their keys are shared out to, and keys of a part of each sequence; else 0, NULL
     int plain; // offsets within 32 slots fit 32 bits
     int near;  // offsets within a sequence's q do
     int scorers;      // few rows: work-groups of a kv head that make its weights from scores
@@ -153,6 +153,49 @@ __device__ __forceinline__ pv_f4 dot(const frame<E, DP> &k, const frame<E, DP> &
 
 constexpr int VPAD = 16; // numbers behind a value row in LDS: four rows of eight banks side by side
 
+// Parts of a step's work, all of much the same size: the keys of all sequences shared out, so that one long sequence among short ones does not keep a few work-groups busy and none is started for
+// slots that nobody holds.  Every work-group of 256 threads finds the same plan from the lengths (a thread a sequence), and what it has of it; false: nothing.
+__device__ __forceinline__ bool shared_part(const ca_args &a, int id, int blocks, int &rb, int &g, int &s, int &split, int &chunk) {
+    __shared__ int before[257], chunk_at[256], sums[4];
+    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+    const ca_lens mine = tid < a.n_seqs ? lens_of(a, tid) : ca_lens{0, 0, 0};
+    const int len = mine.cnt ? mine.len : 0;
+    int x = len;
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) x += __shfl_xor(x, o, 64);
+    if (lane == 0) sums[wave] = x;
+    __syncthreads();
+    const long long all = (long long)sums[0] + sums[1] + sums[2] + sums[3], even = (all * a.G * blocks + a.share - 1) / a.share;
+    const int keys = max(128, (int)((max(even, (long long)((len + a.parts - 1) / a.parts)) + 127) / 128 * 128));
+    chunk_at[tid] = keys;
+    if (id == 0 && tid < a.n_seqs) a.chunks[tid] = keys;
+    x = len ? (len + keys - 1) / keys : 0;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const int y = __shfl_up(x, o, 64);
+        if (lane >= o) x += y;
+    }
+    __syncthreads();
+    if (lane == 63) sums[wave] = x;
+    __syncthreads();
+    for (int i = 0; i < wave; i++) x += sums[i];
+    before[tid + 1] = x;
+    if (tid == 0) before[0] = 0;
+    __syncthreads();
+    if (id >= before[256] * a.G * blocks) return false;
+    rb = id % blocks; id /= blocks;
+    g = id % a.G; id /= a.G;
+    int lo = 0, hi = a.n_seqs - 1; // the last sequence whose parts begin at id or before
+    while (lo < hi) {
+        const int m = (lo + hi + 1) / 2;
+        if (before[m] <= id) lo = m;
+        else hi = m - 1;
+    }
+    s = lo;
+    split = id - before[s];
+    chunk = chunk_at[s];
+    return true;
+}
 // The next block's keys and values are on their way while one is worked on; two work-groups a CU (three or four leave no registers for that: slower).  fp32 runs on v_mfma_f32_16x16x4, 1024 tokens behind 1000
 // at 52 TFLOP/s (the library's product: 153): one wave a SIMD, whose loads and soft-max nothing overlaps.
 template <class E, int DP, int RT>
@@ -163,59 +206,19 @@ __global__ __launch_bounds__(256, E::SIZE == 4 ? 1 : 2) void cache_attn_kernel(c
     __shared__ float lm[4][16], ll[4][16];
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, c = lane & 15, q4 = lane >> 4;
     const int blocks = (a.tiles + RT - 1) / RT;
-    // Parts of a step's work, all of much the same size: the keys of all sequences shared out, so that one long sequence among short ones does not keep a few work-groups busy and none is started
-    // for slots that nobody holds.  Every work-group finds the same plan from the lengths (a thread a sequence).
-    __shared__ int before[257], chunk_at[256];
-    int items = a.n_seqs * a.G * a.parts * blocks;
+    int rb, g, s, split, chunk;
     if (a.share) {
-        __shared__ int sums[4];
-        const ca_lens mine = tid < a.n_seqs ? lens_of(a, tid) : ca_lens{0, 0, 0};
-        const int len = mine.cnt ? mine.len : 0;
-        int x = len;
-#pragma unroll
-        for (int o = 32; o > 0; o >>= 1) x += __shfl_xor(x, o, 64);
-        if (lane == 0) sums[wave] = x;
-        __syncthreads();
-        const long long all = (long long)sums[0] + sums[1] + sums[2] + sums[3], even = (all * a.G * blocks + a.share - 1) / a.share;
-        const int chunk = (int)((max(even, (long long)((len + a.parts - 1) / a.parts)) + 127) / 128 * 128), n = len ? (len + max(chunk, 128) - 1) / max(chunk, 128) : 0;
-        chunk_at[tid] = max(chunk, 128);
-        if (blockIdx.x == 0 && tid < a.n_seqs) a.chunks[tid] = max(chunk, 128);
-        x = n;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const int y = __shfl_up(x, o, 64);
-            if (lane >= o) x += y;
-        }
-        __syncthreads();
-        if (lane == 63) sums[wave] = x;
-        __syncthreads();
-        for (int i = 0; i < wave; i++) x += sums[i];
-        before[tid + 1] = x;
-        if (tid == 0) before[0] = 0;
-        __syncthreads();
-        items = before[256] * a.G * blocks;
-    }
-    int id = blockIdx.x;
-    if (id >= items) return;
-    const int rb = blocks - 1 - id % blocks; id /= blocks; // (the rows with the most causal keys first)
-    int g, s, split, chunk;
-    if (a.share) {
-        g = id % a.G; id /= a.G;
-        int lo = 0, hi = a.n_seqs - 1; // the last sequence whose parts begin at id or before
-        while (lo < hi) {
-            const int m = (lo + hi + 1) / 2;
-            if (before[m] <= id) lo = m;
-            else hi = m - 1;
-        }
-        s = lo;
-        split = id - before[s];
+        if (!shared_part(a, blockIdx.x, blocks, rb, g, s, split, chunk)) return;
     } else {
+        int id = blockIdx.x;
+        rb = id % blocks; id /= blocks;
         split = id % a.parts; id /= a.parts;
         g = id % a.G;
         s = id / a.G;
     }
+    rb = blocks - 1 - rb; // (the rows with the most causal keys first)
     const ca_lens L = lens_of(a, s);
-    chunk = a.share ? chunk_at[s] : chunk_of(a, s, L.len);
+    if (!a.share) chunk = chunk_of(a, s, L.len);
     const int k0 = split * chunk, rows_ = L.cnt * a.R;
     if (L.cnt == 0 || k0 >= L.len || rb * RT * 16 >= rows_) return;
     // row blocks but the last stop where none of their rows sees any key
@@ -705,12 +708,20 @@ __global__ __launch_bounds__(256, 2) void cache_rows_kernel(const ca_args a) {
     __shared__ __attribute__((aligned(16))) unsigned short kl[2][KEYS * KR], vl[2][KEYS * VR];
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, c = lane & 31, h = lane >> 5;
     const int rows_all = a.T * a.R, blocks = (rows_all + ROWS - 1) / ROWS;
-    int id = blockIdx.x;
-    // neighbours are kv heads, so that a head's keys stay in one XCD's L2; the rows with the most causal keys first, those with the fewest from the middle on: a CU's two work-groups add up alike
-    const int heads = a.n_seqs * a.G, hs = id % heads, s = hs / a.G, g = hs - s * a.G; id /= heads;
-    const int split = id % a.parts, p = id / a.parts, half = (blocks + 1) / 2, rb = p < half ? blocks - 1 - p : p - half;
+    int rb, g, s, split, chunk;
+    if (a.share) {
+        if (!shared_part(a, blockIdx.x, blocks, rb, g, s, split, chunk)) return;
+    } else {
+        // neighbours are kv heads, so that a head's keys stay in one XCD's L2; the rows with the most causal keys first, those with the fewest from the middle on: a CU's two work-groups add up alike
+        const int heads = a.n_seqs * a.G, hs = blockIdx.x % heads, id = blockIdx.x / heads, p = id / a.parts, half = (blocks + 1) / 2;
+        s = hs / a.G;
+        g = hs - s * a.G;
+        split = id % a.parts;
+        rb = p < half ? blocks - 1 - p : p - half;
+    }
     const ca_lens L = lens_of(a, s);
-    const int rows = L.cnt * a.R, chunk = chunk_of(a, s, L.len), k0 = split * chunk, k1 = min(L.len, k0 + chunk);
+    if (!a.share) chunk = chunk_of(a, s, L.len);
+    const int rows = L.cnt * a.R, k0 = split * chunk, k1 = min(L.len, k0 + chunk);
     if (rb * ROWS >= rows || k0 >= L.len) return;
     const int r0 = rb * ROWS + wave * 32, row = min(r0 + c, rows - 1), tok = token_of(a, row), first = token_of(a, min(r0, rows - 1));
     const int kend = a.tree ? k1 : min(k1, L.n0 + token_of(a, min(rb * ROWS + ROWS - 1, rows - 1)) + 1); // behind the last key that a row of the work-group sees
@@ -1099,7 +1110,8 @@ void launch_attn(ca_args a, bool many, hipStream_t st) {
     }
     if constexpr (E::SIZE == 2) {
         if (many) {
-            hipLaunchKernelGGL((cache_rows_kernel<E, DP>), dim3((unsigned)(heads * a.parts * ((a.T * a.R + ROWS - 1) / ROWS))), dim3(256), 0, st, a);
+            const long long blocks = (a.T * a.R + ROWS - 1) / ROWS;
+            hipLaunchKernelGGL((cache_rows_kernel<E, DP>), dim3((unsigned)(a.share ? a.share + heads * blocks : heads * a.parts * blocks)), dim3(256), 0, st, a);
             if (a.parts > 1) hipLaunchKernelGGL((cache_join_kernel<E>), dim3((unsigned)(heads * a.tiles)), dim3(256), 0, st, a, (unsigned)(heads * a.tiles));
             if (!a.weight_out) return;
             hipLaunchKernelGGL((cache_receive_kernel<E, DP>), dim3((unsigned)(heads * (a.wgroups ? a.wgroups : (a.n_ctx + 255) / 256))), dim3(256), 0, st, a);
@@ -1126,18 +1138,21 @@ size_t psv_attn_space(int n_cu, const ps_kv_cache &c, const ps_cache_attn_params
     const long long heads = (long long)c.n_seqs * c.kv_heads, rows = (long long)p.n_new * R;
     ca_args a{};
     a.tiles = (int)((rows + 15) / 16);
-    // more than 32 rows of a 16-bit cache: 128 rows a work-group
+    // more than 32 rows of a 16-bit cache: 128 rows a work-group (one side and the other, with weights, bf16, 32 heads of 8, dim 128: 4 sequences of 1801 to 4001, 20 rows 40 and 43 us, 32 rows 44 and 44; 32 sequences
+    // of up to 8100, 20 rows 90 and 102, 32 rows 104 and 102)
     const bool many = size == 2 && rows > 32;
     const long long groups = heads * (many ? (rows + ROWS - 1) / ROWS : (a.tiles + 1) / 2);
-    a.parts = (int)std::min<long long>({std::max<long long>(((many ? 1 : 3) * n_cu + groups - 1) / groups, many ? 1 : (c.n_ctx + 511) / 512), (c.n_ctx + 127) / 128, 64, std::max(1ll, ((1ll << 24) - 1) / groups)}); // (a launch's grid has fewer than 2^32 threads)
+    // parts of the keys: until the chip is full (few rows: three times, or 512 keys each); 1024 keys each where several sequences have one work-group's rows, so that the longest does not keep the others
+    // waiting (32 sequences of up to 8100, 48 rows: 230 us in one part each, 110 so)
+    a.parts = (int)std::min<long long>({std::max<long long>(((many ? 1 : 3) * n_cu + groups - 1) / groups, !many ? (c.n_ctx + 511) / 512 : rows <= ROWS && c.n_seqs > 1 ? (c.n_ctx + 1023) / 1024 : 1), (c.n_ctx + 127) / 128, 64, std::max(1ll, ((1ll << 24) - 1) / groups)}); // (a launch's grid has fewer than 2^32 threads)
     a.near = p.q_row_stride >= 0 && p.q_row_stride < (1 << 28) && (p.n_new + 1ll) * (p.q_row_stride + (long long)R * c.dim) < (1 << 29);
     a.plain = c.slot_stride >= 0 && c.slot_stride < (1 << 24);
     ps_carve ws{(char *)base};
     a.lse = ws.take<float>((size_t)(heads * rows));
     if (a.parts > 1) a.part = ws.take<float>((size_t)(heads * a.tiles * a.parts * 16 * (c.dim + 2)));
     a.score_rows = (int)((rows + 3) / 4 * 4);
-    if (!many && a.parts > 1 && c.n_seqs > 1 && c.n_seqs <= 256) {
-        a.share = 4 * n_cu;
+    if (a.parts > 1 && c.n_seqs > 1 && c.n_seqs <= 256) {
+        a.share = (many ? 2 : 4) * n_cu;
         a.chunks = ws.take<int>(c.n_seqs);
     }
     a.scorers = (int)std::max<long long>(1, std::min<long long>((c.n_ctx + 255) / 256, 8 * n_cu / heads));

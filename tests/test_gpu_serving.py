@@ -233,6 +233,16 @@ def test_many_sequences(ctx, hip, dtype, S):
     Step(ctx, hip, rng, dtype, 4, 2, 64, 300, rng.integers(0, 300, S), 1).run().check()
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("S", [2, 61, 256, 257])
+def test_drafted_tokens_of_many_sequences(ctx, hip, dtype, S):
+    """more than 32 rows each, lengths far apart, some without a token"""
+    rng = np.random.default_rng(S)
+    n_kv = (1090 * rng.random(S) ** 3).astype(int)
+    n_kv[0] = 1091
+    Step(ctx, hip, rng, dtype, 8, 2, 32, 1100, n_kv, 9, count=np.where(np.arange(S) % 5 == 4, 0, 9), tree=random_tree(rng, S, 9)).run().check()
+
+
 @pytest.mark.parametrize("dtype", [F32, F16])
 @pytest.mark.parametrize("n_new", [1, 40])
 def test_one_long_sequence_and_among_short_ones(ctx, hip, dtype, n_new):
