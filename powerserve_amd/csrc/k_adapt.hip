@@ -1,7 +1,7 @@
 // Low-rank adapters of many requests beside a shared projection (ps_hip_adapters_apply): out[t] = base[t] + scale_a up_a (down_a x[t]), a = ids[t].
 //   The tokens of one adapter are taken 16 at a time (a tile), wherever they stand in the batch, so that its matrices are read once for all of them and the products run on
 //   v_mfma_f32_16x16x32_bf16.
-//   adapt_plan_kernel  the tokens sorted by adapter and the tiles, for batches of more than ADAPT_SELF tokens; in smaller ones every work-group finds its tile from the ids itself
+//   adapt_plan_kernel  the tokens sorted by adapter and the tiles, for large batches; in small ones every work-group finds its tile from the ids itself
 //   adapt_down_kernel  h = down x: a tile against a part of K, four waves a quarter each; the parts' sums are left side by side
 //   adapt_up_kernel    the parts' sums together, then 64 columns a wave of base + scale up h
 // A factor that is not bfloat16 -- x in fp32, h -- goes in as three bfloat16 numbers that add up to it, 24 bits together: every product is exact and every sum fp32.  Both matrices
@@ -15,7 +15,10 @@
 namespace {
 typedef __bf16 b8 __attribute__((ext_vector_type(8)));
 typedef __bf16 b2 __attribute__((ext_vector_type(2)));
-constexpr int TILE = 16, ADAPT_SELF = 64; // 253 tokens of 64 adapters: 57 us without a plan, 50 with one; 4 of 3: 11 and 17
+constexpr int TILE = 16;
+// Without a plan a launch is saved, and there are work-groups for every token, most of which find that their tile begins elsewhere: up to 256 tokens (a thread each) and 2^19 results.  K 2048, rank 16, a quarter as
+// many adapters as tokens, without and with: 16 x 14336 11.1 and 13.6 us, 64 x 4096 11.4 and 14.1, 32 x 14336 14.6 and 14.2, 128 x 4096 14.4 and 15.4, 253 x 2048 15.1 and 16.3, 64 x 14336 23.0 and 16.6.
+inline bool plans_itself(int64_t T, int64_t N) { return T <= 256 && T * N <= 1 << 19; }
 struct ad_args {
     const uint16_t *down, *up;
     const int32_t *rank, *ids;
@@ -48,7 +51,7 @@ __device__ __forceinline__ int adapter_of(const ad_args &a, int t) { // -1: none
     const int i = a.ids[t];
     return i >= 0 && i < a.n_slots && a.rank[i] > 0 ? i : -1;
 }
-// The work-group's tile: its adapter (-2: no such tile), its tokens in tok[16].  Without a plan tile b belongs to token b where that is the first, 17th, 33rd .. of its adapter (T <= 64, a thread a
+// The work-group's tile: its adapter (-2: no such tile), its tokens in tok[16].  Without a plan tile b belongs to token b where that is the first, 17th, 33rd .. of its adapter (a thread a
 // token).
 __device__ __forceinline__ int tile_of(const ad_args &a, int b, int *tok, int *n, int *sh) {
     const int tid = threadIdx.x;
@@ -299,13 +302,14 @@ __global__ __launch_bounds__(256) void adapt_up_kernel(const ad_args a) {
 
 size_t psv_adapt_space(const ps_adapters &s, int x_dtype, const void *x, int64_t ldx, int T, const int32_t *ids, const float *base_out, float *out, int64_t ldo, void *base, bool launch, hipStream_t st) {
     ad_args a{};
-    const int most = T <= ADAPT_SELF ? T : std::min<int64_t>(T, (int64_t)s.n_slots + 1 + T / TILE); // tiles there can be
+    const bool plan = !plans_itself(T, s.N);
+    const int most = !plan ? T : std::min<int64_t>(T, (int64_t)s.n_slots + 1 + T / TILE); // tiles there can be
     // parts of K so that the tiles of a batch of one adapter each fill the chip four times, 64 numbers of K a wave at least (64 adapters of rank 64, K 4096: 13 parts, 10.3 us; 7 parts, 13.8)
     a.parts = (int)std::max<int64_t>(1, std::min<int64_t>({(4 * s.n_cu + most - 1) / most, s.KP / 256, 16}));
     ps_carve ws{(char *)base};
     a.h = ws.take<float>((size_t)a.parts * most * s.RP * TILE);
     int32_t *count = nullptr;
-    if (T > ADAPT_SELF) {
+    if (plan) {
         a.order = ws.take<int32_t>((size_t)T);
         a.tiles = ws.take<int32_t>(1 + 3 * (size_t)most);
         count = ws.take<int32_t>((size_t)s.n_slots + 1);
@@ -315,7 +319,7 @@ size_t psv_adapt_space(const ps_adapters &s, int x_dtype, const void *x, int64_t
     a.N = s.N; a.K = s.K; a.KP = s.KP; a.RP = s.RP; a.ldx = ldx; a.ldo = ldo; a.n_slots = s.n_slots; a.T = T;
     const int size = x_dtype == PS_F32 ? 4 : 2;
     a.vec = ((uintptr_t)x % 16 == 0 && ldx * size % 16 == 0 ? 1 : 0) | ((uintptr_t)out % 16 == 0 && (uintptr_t)base_out % 16 == 0 && ldo % 4 == 0 && s.N % 4 == 0 ? 2 : 0);
-    if (T > ADAPT_SELF) hipLaunchKernelGGL(adapt_plan_kernel, dim3(1), dim3(1024), s.n_slots + 1 <= PLAN_LDS ? (size_t)(s.n_slots + 1) * 4 : 0, st, a, count);
+    if (plan) hipLaunchKernelGGL(adapt_plan_kernel, dim3(1), dim3(1024), s.n_slots + 1 <= PLAN_LDS ? (size_t)(s.n_slots + 1) * 4 : 0, st, a, count);
     if (x_dtype == PS_F32) hipLaunchKernelGGL(adapt_down_kernel<true>, dim3(most, a.parts), dim3(256), 0, st, a);
     else hipLaunchKernelGGL(adapt_down_kernel<false>, dim3(most, a.parts), dim3(256), 0, st, a);
     // 256 columns a work-group until the chip is full four times, then more
