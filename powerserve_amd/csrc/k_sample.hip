@@ -153,7 +153,7 @@ __device__ __forceinline__ void make_table(double *table, double *sh, int thread
     __syncthreads();
 }
 __device__ __forceinline__ void part_of(const smp_args &a, int part, int &lo, int &hi) {
-    const int per = ((a.n + a.parts - 1) / a.parts + 63) / 64 * 64;
+    const int per = ((a.n + a.parts - 1) / a.parts + 7) / 8 * 8;
     lo = min(a.n, part * per);
     hi = min(a.n, lo + per);
 }
@@ -195,7 +195,7 @@ __device__ __forceinline__ void row_bound(const smp_args &a, long long r, float 
     for (int x = 32; x > 0; x >>= 1) { lo = min(lo, (unsigned)__shfl_xor((int)lo, x, 64)); hi = max(hi, (unsigned)__shfl_xor((int)hi, x, 64)); }
     if (threadIdx.x < 256) { d.cnt[threadIdx.x] = 0; d.sum[threadIdx.x] = 0; }
     if (threadIdx.x == 0) { d.out[0] = ~0ull; d.out[1] = 0; }
-    __syncthreads();
+    const int some = __syncthreads_count(mine > -INFINITY); // groups with a candidate: short parts and masked stretches leave others empty
     if ((threadIdx.x & 63) == 0) { atomicMin(&d.out[0], (u64)lo); atomicMax(&d.out[1], (u64)hi); }
     __syncthreads();
     lo = (unsigned)d.out[0];
@@ -203,7 +203,7 @@ __device__ __forceinline__ void row_bound(const smp_args &a, long long r, float 
     top = from_order(~lo);
     const int k = row_settings(a, r, top).k, first = 31 - __clz(lo ^ hi); // (-1: all are equal)
     ps = passes_of(k, 0.f);
-    const u64 goal = (u64)(ps.tail ? QUANTILE : k);
+    const u64 goal = (u64)(ps.tail ? max(1, min(QUANTILE, some - (1024 - QUANTILE))) : k);
     unsigned mask = first >= 31 ? 0 : ~0u << (first + 1), found = lo & mask;
     u64 before = 0;
     int shift = max(0, first - 7);
@@ -556,12 +556,13 @@ __global__ __launch_bounds__(PICK) void sample_pick_kernel(const smp_args a) {
     for (int b = threadIdx.x; b <= NB; b += PICK) {
         unsigned c = 0;
         u64 x = 0;
-        if (!OWN && ps.tail)
+        if (!OWN && ps.tail) {
 #pragma unroll 8
-            for (int q = 0; q < a.parts; q++) {
-                if (ps.counts) c += a.cnt[(r * a.parts + q) * (NB + 1) + b];
-                x += a.sum[(r * a.parts + q) * (NB + 1) + b];
-            }
+            for (int q = 0; q < a.parts; q++) x += a.sum[(r * a.parts + q) * (NB + 1) + b];
+            if (ps.counts) // (loops of their own: a condition between the loads would wait for each)
+#pragma unroll 8
+                for (int q = 0; q < a.parts; q++) c += a.cnt[(r * a.parts + q) * (NB + 1) + b];
+        }
         cnt[b] = c;
         sum[b] = x;
     }
@@ -656,10 +657,11 @@ void launch(const smp_args &a, hipStream_t st) {
 
 size_t psv_sample_space(int n_cu, int dtype, const void *logits, int64_t n, int64_t rows, int64_t stride, const ps_sample_params *p, int32_t *ids, float *prob, void *base, bool launch_, hipStream_t st) {
     smp_args a{};
-    // a row alone where there is a row for half the CUs; else 4, 8 .. 64 parts (1024 groups of a row in all) of at least 1024 logits, as many as the chip takes at once
+    // a row alone where there is a row for half the CUs; else 4, 8 .. 64 parts (1024 groups of a row in all) of at least a piece of 16 bytes a thread, as many as the chip takes at once
+    const int64_t least = dtype == PS_F32 ? 1024 : 2048;
     a.parts = 1;
-    if (rows * 2 <= n_cu && n >= 4096)
-        for (a.parts = 4; a.parts < 64 && a.parts * 2 * rows <= 2 * n_cu && a.parts * 2 * 1024 <= n;) a.parts *= 2;
+    if (rows * 2 <= n_cu && n >= 4 * least)
+        for (a.parts = 4; a.parts < 64 && a.parts * 2 * rows <= 2 * n_cu && a.parts * 2 * least <= n;) a.parts *= 2;
     ps_carve ws{(char *)base};
     if (a.parts > 1) {
         a.top = ws.take<float>((size_t)rows * 1024);

@@ -433,6 +433,18 @@ def test_sampling_with_all_settings(ctx, hip, dtype, rows, n):
     check_sample(ctx, hip, logits, dtype, settings, stride=n + rows % 3)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("rows,n", [(6, 27424), (2, 16385), (1, 8200), (9, 8191), (130, 8193)])
+@pytest.mark.parametrize("masked", [0.0, 0.97])
+def test_sampling_of_short_parts_and_masked_rows(ctx, hip, dtype, rows, n, masked):
+    """parts of a row with fewer numbers than threads, and vocabularies most of which a grammar forbids"""
+    rng = np.random.default_rng(n + dtype)
+    logits = 2.5 * rng.standard_normal((rows, n))
+    logits[rng.random((rows, n)) < masked] = -np.inf
+    settings = [rng.choice([0.6, 1.0, 1.3], rows), rng.choice([0, 40, 5000], rows), rng.choice([1.0, 0.9], rows), rng.choice([0.0, 0.01], rows), rng.random(rows)]
+    check_sample(ctx, hip, ref.pack(logits, dtype), dtype, settings, stride=n + 1)
+
+
 @pytest.mark.parametrize("rows", [2, 200])
 def test_sampling_without_settings(ctx, hip, rows):
     rng = np.random.default_rng(rows)
