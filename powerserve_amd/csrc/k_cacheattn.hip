@@ -596,7 +596,7 @@ template <int B> struct received {
     __device__ __forceinline__ long long start(int w) const { return n * w / groups; }
     __device__ __forceinline__ int group_of(long long tile) const { return (int)(((tile + 1) * groups + n - 1) / n) - 1; }
 };
-// fp32 caches, more rows: 64 keys of a kv head against the rows that see any, the waves 16 of 64 rows each (1024 tokens behind 1000, 14 heads of 2, dim 64: 65 us, 43 TFLOP/s; a work-group a block: 251)
+// fp32 caches, more rows: 64 keys of a kv head against the rows that see any, the waves 16 of 64 rows each (1024 tokens behind 1000, 14 heads of 2, dim 64: 53 us, 52 TFLOP/s; a work-group a block: 251)
 template <class E, int DP>
 __global__ __launch_bounds__(256) void cache_weight_kernel(const ca_args a) {
     constexpr int NS = STEPS<E, DP>;
@@ -1054,6 +1054,7 @@ __global__ __launch_bounds__(256) void cache_gather_kernel(const ca_args a) { //
         long long first = (long long)min(b, work.held) * work.tiles;
         for (int x = work.held; x < b; x++) first += work.tiles - work.from(x);
         const int w0 = work.group_of(first), w1 = work.group_of(first + work.tiles - work.from(b) - 1);
+#pragma unroll 8
         for (int w = w0; w <= w1; w++) v += a.wpart[(head * (a.wgroups + (a.n_ctx + B - 1ll) / B) + w + b) * B + j % B];
     }
     a.weight_out[at] = j < L.n0 && a.weight ? a.weight[at] + v : v;
@@ -1160,7 +1161,7 @@ size_t psv_attn_space(int n_cu, const ps_kv_cache &c, const ps_cache_attn_params
     if (a.tiles > 2 && p.weight_out) { // up to 256 rows of slots enough to fill the chip: a block's rows are few; else the blocks' rows, which a sequence's length and the causal mask make unequal, are shared out
         const long long block = many ? 256 : 64, blocks = (c.n_ctx + block - 1) / block;
         if (rows > 4 * QT || heads * blocks < 2 * n_cu) {
-            a.wgroups = (int)(((many ? 2 : 4) * n_cu + heads - 1) / heads);
+            a.wgroups = (int)((2 * n_cu + heads - 1) / heads); // (two a CU: half as many, 2048 tokens behind 2047: 87 -> 129 us; twice as many in fp32, 1024 behind 1000: 53 -> 65)
             a.wpart = ws.take<float>((size_t)(heads * (a.wgroups + blocks) * block));
         }
     }
