@@ -196,10 +196,10 @@ __device__ __forceinline__ bool shared_part(const ca_args &a, int id, int blocks
     chunk = chunk_at[s];
     return true;
 }
-// The next block's keys and values are on their way while one is worked on; two work-groups a CU (three or four leave no registers for that: slower).  fp32 runs on v_mfma_f32_16x16x4, 1024 tokens behind 1000
-// at 52 TFLOP/s (the library's product: 153): one wave a SIMD, whose loads and soft-max nothing overlaps.
+// The next block's keys and values are on their way while one is worked on; two work-groups a CU (three or four leave no registers for that: slower).  fp32 runs on v_mfma_f32_16x16x4: 1024 tokens behind
+// 1000, dim 64 57 TFLOP/s, dim 128, whose registers leave one work-group a CU, 52 (the library's product: 153).
 template <class E, int DP, int RT>
-__global__ __launch_bounds__(256, E::SIZE == 4 ? 1 : 2) void cache_attn_kernel(const ca_args a) {
+__global__ __launch_bounds__(256, E::SIZE == 4 && DP == 128 ? 1 : 2) void cache_attn_kernel(const ca_args a) {
     constexpr int NS = STEPS<E, DP>, ND = DP / 16, OP = DP + 4, VR = DP + VPAD;
     constexpr int VBYTES = E::SIZE == 2 ? 4 * 32 * VR * 2 : 0, OBYTES = 4 * 16 * OP * 4;
     __shared__ __attribute__((aligned(16))) char lds[VBYTES > OBYTES ? VBYTES : OBYTES];
@@ -598,7 +598,7 @@ template <int B> struct received {
 };
 // fp32 caches, more rows: 64 keys of a kv head against the rows that see any, the waves 16 of 64 rows each (1024 tokens behind 1000, 14 heads of 2, dim 64: 53 us, 52 TFLOP/s; a work-group a block: 251)
 template <class E, int DP>
-__global__ __launch_bounds__(256) void cache_weight_kernel(const ca_args a) {
+__global__ __launch_bounds__(256, 2) void cache_weight_kernel(const ca_args a) {
     constexpr int NS = STEPS<E, DP>;
     __shared__ float red[4][64];
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, c = lane & 15, q4 = lane >> 4;
