@@ -226,6 +226,16 @@ def test_two_tiles_of_rows(ctx, hip, dtype, n_new, heads, kv_heads, dim, as_tree
     Step(ctx, hip, rng, dtype, heads, kv_heads, dim, 700, [0, 640, 129], n_new, tree=random_tree(rng, 3, n_new) if as_tree else None).run().check()
 
 
+@pytest.mark.parametrize("dtype", [F32, F16])
+@pytest.mark.parametrize("n_new", [2, 3, 4, 6])
+@pytest.mark.parametrize("heads,kv_heads", [(4, 2), (40, 2)])
+def test_small_trees_of_any_bytes(ctx, hip, dtype, n_new, heads, kv_heads):
+    """rows of fewer than four bytes, and bytes that are not 0 and not 1"""
+    rng = np.random.default_rng(n_new)
+    tree = random_tree(rng, 5, n_new) * rng.choice(np.array([1, 2, 127, 128, 255], dtype=np.uint8), (5, n_new, n_new))
+    Step(ctx, hip, rng, dtype, heads, kv_heads, 64, 400, [0, 61, 399, 30, 254], n_new, count=[n_new, n_new - 1, n_new, 1, n_new], tree=tree).run().check()
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("S", [255, 256, 257, 300])
 def test_many_sequences(ctx, hip, dtype, S):
