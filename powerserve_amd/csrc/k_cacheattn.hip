@@ -39,7 +39,7 @@ struct ca_args {
     const uint8_t *tree;
     const float *weight;
     float *weight_out;
-    float *part; // [seq][kv head][16 rows][part]: 16 x dim results, 16 maxima, 16 sums
+    float *part; // [seq][kv head][16 rows][part]: 16 x dim results, the 16 scores that their weights are taken against, 16 sums
     float *score; // [seq][kv head][slot][score_rows]: scores of few rows for the weights, or NULL
     float *lse;  // [seq][kv head][T R] logarithm, in the scores' units, of the sum of weights (+inf: no weights)
     int parts, tiles, score_rows; // tiles of 16 rows
@@ -117,6 +117,13 @@ template <class E> __device__ __forceinline__ float ex(float x) {
         const float y = x * 1.44269504f, lo = fmaf(x, 1.44269504f, -y) + x * 1.92596299e-8f, e = __builtin_amdgcn_exp2f(y);
         return x < -104.f ? 0.f : fmaf(e, lo * 0.693147181f, e);
     }
+}
+// The score that a row's weights are taken against, from its largest: e^(score - this).  It cancels in the result and in the sums' logarithm.  fp16 weights are up to 2^15 instead of 1 (65504 is the largest
+// number), so that one keeps its 11 bits down to 2^-29 of the largest, and its second number to 2^-40 of it: thousands of small weights beside an attention sink are the result where the sink's value is
+// small.  From 2^20 on, where a float's steps are an eighth and more, the largest itself.
+template <class E> __device__ __forceinline__ float against(float top) {
+    if constexpr (__is_same(E, F16)) return fabsf(top) < 1048576.f ? top - 15.f : top;
+    else return top;
 }
 template <class E> __device__ __forceinline__ float lg(float x) { return E::SIZE == 2 ? log2f(x) : logf(x); }
 __device__ __forceinline__ bool odd32(float v) { return (__float_as_uint(v) & 0x7f800000u) == 0x7f800000u; }
@@ -356,7 +363,7 @@ __global__ __launch_bounds__(256, E::SIZE == 4 && DP == 128 ? 1 : 2) void cache_
             }
             top = fmaxf(top, __shfl_xor(top, 16, 64));
             top = fmaxf(top, __shfl_xor(top, 32, 64));
-            const float mn = fmaxf(m[r], top), ms = mn == -INFINITY ? 0.f : mn, al = ex<E>(m[r] - ms);
+            const float mn = fmaxf(m[r], against<E>(top)), ms = mn == -INFINITY ? 0.f : mn, al = ex<E>(m[r] - ms);
             float p[8], sum = 0.f;
 #pragma unroll
             for (int u = 0; u < 2; u++)
@@ -372,8 +379,8 @@ __global__ __launch_bounds__(256, E::SIZE == 4 && DP == 128 ? 1 : 2) void cache_
 #pragma unroll
                 for (int i = 0; i < 4; i++) o[r][d][i] *= al;
             if constexpr (E::SIZE == 2) {
-                // the weights as two 16-bit numbers each: what the second product rounds off is 2^-17 (bf16; fp16 2^-23) of a weight, not the 2^-9 that would stand beside the result's own
-                // rounding; these products are not what bounds a pass over the cache
+                // the weights as two 16-bit numbers each: what the second product rounds off is 2^-17 (bf16; fp16 2^-23, and 2^-40 of the row's largest where that is more) of a weight, not the 2^-9 that
+                // would stand beside the result's own rounding; these products are not what bounds a pass over the cache
                 pv_u4 hi, lo;
 #pragma unroll
                 for (int x = 0; x < 4; x++) {
@@ -817,7 +824,7 @@ __global__ __launch_bounds__(256, 2) void cache_rows_kernel(const ca_args a) {
         float top = fmaxf(z[0][0], z[1][0]); // (of scores before the scale, which is above 0 here)
 #pragma unroll
         for (int i = 1; i < 16; i++) top = fmaxf(fmaxf(z[0][i], z[1][i]), top);
-        top = fmaxf(top, __shfl_xor(top, 32, 64)) * sc;
+        top = against<E>(fmaxf(top, __shfl_xor(top, 32, 64)) * sc);
         if (__any(top > mx)) { // most blocks behind the first few raise no maximum
             const float mn = fmaxf(mx, top), ms = mn == -INFINITY ? 0.f : mn, al = __builtin_amdgcn_exp2f(mx - ms);
             l *= al;

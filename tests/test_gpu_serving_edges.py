@@ -1,0 +1,62 @@
+"""The operators of a serving step of many sequences on the GPU where their numbers are few, far apart or infinite, and along paths that ordinary sizes do not take (plain forms in 64 bits: tests/serving_ref.py)."""
+import numpy as np
+import pytest
+
+import serving_ref as ref
+from serving_ref import BF16, F16, F32
+from test_gpu_serving import NAN, Step, random_tree
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def hip():
+    from powerserve_amd import hip as h
+    return h
+
+
+def again(step, *names):
+    """Arrays of a step that were changed behind its making, to the device."""
+    for n in names:
+        step.d[n].free()
+        step.d[n] = step.ctx.to_device(getattr(step, n))
+    step.cache.k, step.cache.v, step.args.q = (step.d[n].ptr for n in ("k", "v", "q"))
+    if step.append:
+        step.args.k_new, step.args.v_new = step.d["kn"].ptr, step.d["vn"].ptr
+    return step
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("n_new", [1, 4, 60])
+def test_a_token_that_takes_almost_all_of_the_weight_and_the_many_that_share_the_rest(ctx, hip, dtype, n_new):
+    """An attention sink: one slot 10 to 24 above the others, whose value is zero, so that the result is what thousands of small weights leave."""
+    rng = np.random.default_rng(n_new)
+    H, G, D = 8, 2, 64
+    s = Step(ctx, hip, rng, dtype, H, G, D, 4200, [4100, 900], n_new)
+    above = np.array([10.0, 14.0, 16.0, 18.0, 12.0, 17.0, 20.0, 24.0])  # of each query head
+    q, kn, vn, k, v = (ref.unpack(getattr(s, n), dtype) for n in ("q", "kn", "vn", "k", "v"))
+    q *= 0.3
+    q[..., 0] = above / 4 / s.scale
+    for x in (k, kn):
+        x[..., 0] = 0
+    for x in (v, vn):
+        x[:] = np.abs(x)
+    k[:, 0, 0] = 0
+    k[:, 0, 0, :, 0] = 4
+    v[:, 0, 0] = 0
+    s.q, s.kn, s.vn, s.k, s.v = (ref.pack(x, dtype) for x in (q, kn, vn, k, v))
+    again(s, "q", "kn", "vn", "k", "v").run().check()
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("n_new", [1, 60])
+@pytest.mark.parametrize("sign", [1, -1])
+def test_scores_whose_steps_are_coarse(ctx, hip, dtype, n_new, sign):
+    """Scores of millions, a float's steps an eighth to a half: no weight passes its type's largest number."""
+    rng = np.random.default_rng(n_new)
+    s = Step(ctx, hip, rng, dtype, 8, 2, 64, 500, [400, 60, 0], n_new, weights=False)
+    s.q, s.k, s.kn = (ref.pack(np.abs(ref.unpack(x, dtype)) * y, dtype) for x, y in ((s.q, sign * 400), (s.k, 30), (s.kn, 30)))  # (one sign, so that none is near zero)
+    s.args.scale = s.scale = 8.0
+    again(s, "q", "k", "kn").run()
+    assert np.isfinite(ref.unpack(s.d["out"].numpy(), dtype)).all()
+    s.check()
