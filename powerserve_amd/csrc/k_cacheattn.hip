@@ -456,6 +456,26 @@ __global__ __launch_bounds__(256, E::SIZE == 4 && DP == 128 ? 1 : 2) void cache_
                         if (odd32(x)) v[i] += x;
                     }
                 }
+            // An infinite value is NaN by now where it met a weight's second number, which may be 0 or below it, or a weight or a factor too small for its type: what the infinities and NaN that the row
+            // sees add up to, where the row's weights are numbers and there are any
+            if (sum == sum && (v[0] != v[0] || v[1] != v[1] || v[2] != v[2] || v[3] != v[3])) {
+                pv_f4 x = {0.f, 0.f, 0.f, 0.f};
+                auto add = [&](int j) {
+                    const char *src = row_at(vb_, vn, j) + e * E::SIZE;
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const float y = number<E>(src + i * E::SIZE);
+                        x[i] += odd32(y) ? y : 0.f;
+                    }
+                };
+#pragma unroll 4
+                for (int j = k0; j < min(k1, L.n0); j++) add(j);
+                for (int j = max(k0, L.n0); j < k1; j++)
+                    if (sees(a, s, t, j - L.n0)) add(j);
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    if (v[i] != v[i] && x[i] != 0.f) v[i] = x[i];
+            }
             if (a.parts > 1) *(pv_f4 *)(part + rr * a.dim + e) = v;
             else {
                 char *dst = a.out + s * a.o_seq + t * a.o_row + ((long long)hd * a.dim + e) * E::SIZE;
@@ -484,7 +504,7 @@ template <class E> __device__ __forceinline__ float row_sum(const ca_args &a, co
     for (int i = lane4; i < n; i += 4) {
         const float v = m[i * step], x = ex<E>(v - ms);
         sum = fmaf(l[i * step], x, sum);
-        if (f) f[i][r] = v == -INFINITY ? 0.f : x; // (no result is left there)
+        if (f) f[i][r] = v == -INFINITY ? 0.f : fmaxf(x, 1e-45f); // (an infinite result counts however small its part's weights are)
     }
     sum += __shfl_xor(sum, 16, 64);
     sum += __shfl_xor(sum, 32, 64);
@@ -875,6 +895,30 @@ __global__ __launch_bounds__(256, 2) void cache_rows_kernel(const ca_args a) {
                     const float x = number<E>(src + e * 2);
                     if (odd32(x)) o[m][i] += x;
                 }
+        }
+    // infinite values that met a weight or a factor of 0, as in cache_attn_kernel
+    unsigned long long nan = 0;
+#pragma unroll
+    for (int m = 0; m < MD; m++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) nan |= (o[m][i] != o[m][i] ? 1ull : 0ull) << (16 * m + i);
+    if (nan && l == l)
+#pragma unroll 1
+        for (int x = 0; x < 16 * MD; x++) { // (one at a time: all together would not fit the registers)
+            const int e = 32 * (x >> 4) + 8 * (x >> 2 & 3) + 4 * h + (x & 3);
+            const bool here = (nan >> x & 1) && e < a.dim;
+            float sum = 0.f;
+            if (here) {
+                auto value = [&](int j) { const float y = number<E>(vb_ + j * a.slot + e * 2); return odd32(y) ? y : 0.f; };
+#pragma unroll 8
+                for (int j = k0; j < min(kend, L.n0); j++) sum += value(j);
+                for (int j = max(k0, L.n0); j < kend; j++)
+                    if (sees(a, s, tok, j - L.n0)) sum += value(j);
+            }
+#pragma unroll
+            for (int m = 0; m < MD; m++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) o[m][i] = here && sum != 0.f && x == 16 * m + i ? sum : o[m][i];
         }
     const float ms = mx == -INFINITY ? 0.f : mx;
     if (a.parts > 1) {

@@ -60,3 +60,50 @@ def test_scores_whose_steps_are_coarse(ctx, hip, dtype, n_new, sign):
     again(s, "q", "k", "kn").run()
     assert np.isfinite(ref.unpack(s.d["out"].numpy(), dtype)).all()
     s.check()
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("n_new,n_kv", [(1, [40, 1, 3000]), (6, [40, 5, 3000]), (60, [40, 9, 3000])])
+def test_infinite_values_of_held_slots(ctx, hip, dtype, n_new, n_kv):
+    """A value that is infinite is that in the result, whether its slot is held or new; two of different signs, or a NaN, are NaN; where one slot alone is seen too."""
+    rng = np.random.default_rng(n_new)
+    s = Step(ctx, hip, rng, dtype, 8, 2, 64, 3100, n_kv, n_new, weights=False)
+    v, vn = ref.unpack(s.v, dtype), ref.unpack(s.vn, dtype)
+    for i, n in enumerate(n_kv):
+        for e, x in ((5, np.inf), (6, -np.inf), (7, NAN), (8, np.inf)):
+            v[i, n // 2, 0, :, e] = x
+        v[i, n - 1, 0, :, 8] = -np.inf if n > 1 else np.inf
+    vn[:, -1, :, 9] = np.inf  # beside a new one
+    s.v, s.vn = ref.pack(v, dtype), ref.pack(vn, dtype)
+    again(s, "v", "vn").run().check()
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_a_single_slot_of_infinite_values(ctx, hip, dtype):
+    rng = np.random.default_rng(1)
+    s = Step(ctx, hip, rng, dtype, 4, 2, 64, 40, [1, 1], 1, tree=np.zeros((2, 1, 1)), weights=False)
+    v = ref.unpack(s.v, dtype)
+    v[0, 0, 0, :, ::2] = np.inf
+    v[1, 0, 0, :, 1::2] = -np.inf
+    s.v = ref.pack(v, dtype)
+    again(s, "v").run().check()
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("n_new", [1, 60])
+def test_infinite_values_of_the_smallest_weights(ctx, hip, dtype, n_new):
+    """Slots 100 to 200 below another one, whose weights no float holds, in its block, in its part and in others: infinite is what an infinite value is times any weight."""
+    rng = np.random.default_rng(n_new)
+    D = 64
+    s = Step(ctx, hip, rng, dtype, 4, 2, D, 3100, [3000, 200, 3000], n_new, weights=False)
+    q, kn, k, v = (ref.unpack(getattr(s, n), dtype) for n in ("q", "kn", "k", "v"))
+    q[..., 0] = 30
+    kn[..., 0] = k[..., 0] = 0
+    for i, at in enumerate((10, 150, 2900)):
+        k[i, at, 0, :, 0] = (100, 150, 200)[i] / 30 / s.scale
+    for i, n in enumerate(s.n0):
+        for e, j in enumerate((0, 11, 40, 120, 199, 2000)):
+            if j < n:
+                v[i, j, 0, :, e] = np.inf if e % 2 else -np.inf
+    s.q, s.kn, s.k, s.v = (ref.pack(x, dtype) for x in (q, kn, k, v))
+    again(s, "q", "kn", "k", "v").run().check()
