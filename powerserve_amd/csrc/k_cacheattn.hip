@@ -718,8 +718,9 @@ __global__ __launch_bounds__(256) void cache_append_kernel(const ca_args a, int 
 
 // Many rows of a 16-bit cache: 128 of a kv head against a part of its keys, a wave 32 of them against all, 64 keys at a time through two LDS stages that the four waves fill.  The products are
 // v_mfma_f32_32x32x16: S^T = K Q^T with the queries in registers (a lane: one row, 16 keys a tile), O^T = V^T P^T with the weights as they come, values transposed on their way out of LDS.
-// The weights go into the second product as one 16-bit number each (rounded like the result is: 2^-9 of a weight, bf16, to either side); their sum is taken before they are rounded.
-// What bounds it: a wave and 64 keys take 32 matrix instructions of 32 clocks, 32 KB of operands from LDS and some 230 vector instructions; two waves a SIMD overlap them in part, at the 2.0 GHz that the card holds
+// The weights go into the second product as two 16-bit numbers each, as in cache_attn_kernel, so that a token's result is as exact among many new tokens as among few; one number each, 2^-9 of a weight off
+// (bf16), would take a third fewer matrix instructions (2048 tokens behind 2047, all launches: 214 us instead of 248).  Their sum is taken before they are rounded.
+// What bounds it: a wave and 64 keys take 48 matrix instructions of 32 clocks, 32 KB of operands from LDS and some 300 vector instructions; two waves a SIMD overlap them in part, at the 2.0 GHz that the card holds
 // under it (2048 tokens behind 2047: 138 us, 750 TFLOP/s).  Work-groups of eight waves read a tile for twice the rows, and their sizes even out worse (168 us there; 8192 tokens 5 % faster).
 constexpr int ROWS = 128, KEYS = 64;
 // the same for a lane's 16 keys of a tile of 32, x + 8 (i / 4) + i % 4
@@ -855,7 +856,7 @@ __global__ __launch_bounds__(256, 2) void cache_rows_kernel(const ca_args a) {
             mx = mn;
         }
         const float ms = mx == -INFINITY ? 0.f : mx;
-        pv_u4 pk[4];
+        pv_u4 pk[4], pl[4]; // the weights as two 16-bit numbers each
         float sum = 0.f;
 #pragma unroll
         for (int u = 0; u < 2; u++)
@@ -863,7 +864,10 @@ __global__ __launch_bounds__(256, 2) void cache_rows_kernel(const ca_args a) {
             for (int i = 0; i < 16; i += 2) {
                 const float p0 = __builtin_amdgcn_exp2f(fmaf(z[u][i], sc, -ms)), p1 = __builtin_amdgcn_exp2f(fmaf(z[u][i + 1], sc, -ms));
                 sum += p0 + p1;
-                pk[2 * u + (i >> 3)][(i >> 1) & 3] = round2<E>(p0, p1);
+                const unsigned hi = round2<E>(p0, p1);
+                const pv_f2 w = wide2<E>(hi);
+                pk[2 * u + (i >> 3)][(i >> 1) & 3] = hi;
+                pl[2 * u + (i >> 3)][(i >> 1) & 3] = round2<E>(p0 - w[0], p1 - w[1]);
             }
         l += sum;
         const unsigned short *base = vl[cur] + (4 * h + ((lane & 15) >> 2)) * VR + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
@@ -874,7 +878,9 @@ __global__ __launch_bounds__(256, 2) void cache_rows_kernel(const ca_args a) {
             for (int m = 0; m < MD; m++) {
                 const s4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)(base + 16 * k * VR + 32 * m)), y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)(base + (16 * k + 8) * VR + 32 * m));
                 const pv_u2 xx = __builtin_bit_cast(pv_u2, x), yy = __builtin_bit_cast(pv_u2, y);
-                o[m] = mfma32<E>((pv_u4){xx[0], xx[1], yy[0], yy[1]}, pk[k], o[m]);
+                const pv_u4 v = {xx[0], xx[1], yy[0], yy[1]};
+                o[m] = mfma32<E>(v, pk[k], o[m]);
+                o[m] = mfma32<E>(v, pl[k], o[m]);
             }
         if (more) put(kb + KEYS, cur ^ 1);
         __syncthreads();
@@ -882,44 +888,41 @@ __global__ __launch_bounds__(256, 2) void cache_rows_kernel(const ca_args a) {
     odd = __syncthreads_or(odd);
     l += __shfl_xor(l, 32, 64);
     if (r0 + c >= rows) return;
-    if (odd)
-        for (int j = max(k0, L.n0); j < kend; j++) {
-            if (!sees(a, s, tok, j - L.n0)) continue;
-            const char *src = vb_ + j * a.slot;
-#pragma unroll
-            for (int m = 0; m < MD; m++)
-#pragma unroll
-                for (int i = 0; i < 16; i++) {
-                    const int e = 32 * m + 8 * (i >> 2) + 4 * h + (i & 3);
-                    if (e >= a.dim) continue;
-                    const float x = number<E>(src + e * 2);
-                    if (odd32(x)) o[m][i] += x;
-                }
-        }
-    // infinite values that met a weight or a factor of 0, as in cache_attn_kernel
+    // the infinities and NaN of new tokens; and results that are NaN where an infinite value met a weight's second number, or a weight or a factor of 0, as in cache_attn_kernel
     unsigned long long nan = 0;
 #pragma unroll
     for (int m = 0; m < MD; m++)
 #pragma unroll
         for (int i = 0; i < 16; i++) nan |= (o[m][i] != o[m][i] ? 1ull : 0ull) << (16 * m + i);
-    if (nan && l == l)
+    if (l != l) nan = 0;
+    if (odd || nan) {
+#pragma unroll
+        for (int m = 0; m < MD; m++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) o[m][i] = nan >> (16 * m + i) & 1 ? 0.f : o[m][i];
 #pragma unroll 1
         for (int x = 0; x < 16 * MD; x++) { // (one at a time: all together would not fit the registers)
             const int e = 32 * (x >> 4) + 8 * (x >> 2 & 3) + 4 * h + (x & 3);
-            const bool here = (nan >> x & 1) && e < a.dim;
-            float sum = 0.f;
-            if (here) {
+            const bool all = nan >> x & 1;
+            float more = 0.f;
+            if (e < a.dim && (odd || all)) {
                 auto value = [&](int j) { const float y = number<E>(vb_ + j * a.slot + e * 2); return odd32(y) ? y : 0.f; };
+                if (all)
 #pragma unroll 8
-                for (int j = k0; j < min(kend, L.n0); j++) sum += value(j);
+                    for (int j = k0; j < min(kend, L.n0); j++) more += value(j);
                 for (int j = max(k0, L.n0); j < kend; j++)
-                    if (sees(a, s, tok, j - L.n0)) sum += value(j);
+                    if (sees(a, s, tok, j - L.n0)) more += value(j);
             }
 #pragma unroll
             for (int m = 0; m < MD; m++)
 #pragma unroll
-                for (int i = 0; i < 16; i++) o[m][i] = here && sum != 0.f && x == 16 * m + i ? sum : o[m][i];
+                for (int i = 0; i < 16; i++) o[m][i] += x == 16 * m + i ? more : 0.f;
         }
+#pragma unroll
+        for (int m = 0; m < MD; m++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) o[m][i] = (nan >> (16 * m + i) & 1) && o[m][i] == 0.f ? NAN : o[m][i];
+    }
     const float ms = mx == -INFINITY ? 0.f : mx;
     if (a.parts > 1) {
         float *part = a.part + ((((long long)s * a.G + g) * a.tiles + row / 16) * a.parts + split) * (16 * (a.dim + 2));

@@ -107,3 +107,24 @@ def test_infinite_values_of_the_smallest_weights(ctx, hip, dtype, n_new):
                 v[i, j, 0, :, e] = np.inf if e % 2 else -np.inf
     s.q, s.kn, s.k, s.v = (ref.pack(x, dtype) for x in (q, kn, k, v))
     again(s, "q", "kn", "k", "v").run().check()
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("n_new,as_tree", [(9, False), (24, True), (150, False)])
+def test_many_rows_are_as_exact_as_few(ctx, hip, dtype, n_new, as_tree):
+    """A drafted token's result does not depend on how many are drafted with it: rounding a weight is 2^-16 of it at most, whatever the number of rows.  (Few slots, so that the values of a row do not even the roundings out.)"""
+    rng = np.random.default_rng(n_new)
+    H, G, D, S = 8, 2, 64, 6
+    tree = random_tree(rng, S, n_new) if as_tree else None
+    s = Step(ctx, hip, rng, dtype, H, G, D, 400, [0, 1, 2, 5, 3, 200], n_new, tree=tree, weights=False).run()
+    out, K, V, q, kn, vn = (ref.unpack(x, dtype) for x in (s.d["out"].numpy(), s.k, s.v, s.q, s.kn, s.vn))
+    for i in range(S):
+        n0 = int(s.n0[i])
+        K[i, n0:n0 + n_new, 0], V[i, n0:n0 + n_new, 0] = kn[i], vn[i]
+        want, _, size, far = ref.attend(q[i], K[i, :, 0], V[i, :, 0], n0, n_new, s.scale, None if tree is None else tree[i])
+        # as in Step.check; the weights as two numbers: 2^-16
+        rel = 2 * (D + 4) * 2.0**-24 * far + 2 * 2.0**-22 + (n0 + n_new + 64) * 2.0**-23 + 2.0**-16
+        bound = rel * size + ref.HALF_STEP[dtype] * (np.abs(want) + rel * size) + ref.TINY[dtype]
+        err = np.abs(out[i] - want)
+        assert (err <= bound).all(), (i, float((err / bound).max()))
+    s.free()
