@@ -526,9 +526,10 @@ int ps_hip_seq_bench_kernel(ps_hip_seq *m, int which, int T, int reps, double *u
 /* ------------------------------------------------------------------ a serving step of many sequences
  * Operators over device memory that the caller holds, for steps that serve several sequences at once: attention over their caches (ps_hip_cache_*), sampling from their logits
  * (ps_hip_sample) and low-rank adapters beside a shared projection (ps_hip_adapters_*).  Everything that changes from step to step -- lengths, counts, trees, settings, ids -- is read from
- * DEVICE arrays by the kernels, and scratch memory is the caller's (its size from the *_workspace function beside the call; 16-byte aligned; nothing is kept in it between calls), so that calls
- * on the ctx stream can be captured into a graph and replayed.  Two calls that may run at the same time (graphs, contexts) need a workspace each.  All calls only enqueue.  Buffers
- * lie on the ctx's device; memory last written on another stream is the caller's to order.  No two buffers of a call overlap unless it says so.  A refused call enqueues nothing. */
+ * DEVICE arrays by the kernels, and scratch memory is the caller's: its size from the *_workspace function beside the call, which serves every call of no more sequences, new tokens, logits, rows or
+ * tokens too (a server asks once, for its largest step); 16-byte aligned; nothing is kept in it between calls, so that calls on the ctx stream can be captured into a graph and replayed.  Two calls that
+ * may run at the same time (graphs, contexts) need a workspace each.  All calls only enqueue.  Buffers lie on the ctx's device; memory last written on another stream is the caller's to order, the
+ * workspace too.  No two buffers of a call overlap unless it says so.  A refused call enqueues nothing. */
 
 /* The keys and values of one attention layer for n_seqs sequences: number e of kv head g in slot j of sequence s is k[s * seq_stride + j * slot_stride + g * head_stride + e], the same for v; slots
  * of one layer may lie between those of others.  Rows are 16-byte aligned (pointers, and strides times the size of a number); dim is a multiple of 8, 8 to 128.  The slots 0 .. n_kv[s] - 1 are
@@ -562,6 +563,9 @@ typedef struct {
     const uint8_t *tree;
     float *weight_out;
 } ps_cache_attn_params;
+/* With weights the scratch memory holds a score per slot for up to 32 rows (new tokens times query heads of a kv head) whatever is held: n_seqs * kv_heads * n_ctx * min(rows, 32) fp32, of a 16-bit cache of dim 128
+ * at most a quarter of its size; beside them partial results, 16 * (dim + 2) fp32 for 16 rows and a part, of which a kv head has
+ * up to 64, and n_seqs * heads * n_new fp32. */
 size_t ps_hip_cache_attn_workspace(ps_hip_ctx *ctx, const ps_kv_cache *cache, const ps_cache_attn_params *p);
 int ps_hip_cache_attn(ps_hip_ctx *ctx, const ps_kv_cache *cache, const ps_cache_attn_params *p, void *workspace, size_t workspace_bytes);
 /* Takes new tokens into the cache: n_kv[s] += count[s].  take (NULL: the first count[s] tokens): [n_seqs][n_take] ascending indices of the tokens that stay, an accepted path of a tree -- token take[s][i]

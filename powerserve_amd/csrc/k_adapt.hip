@@ -300,20 +300,36 @@ __global__ __launch_bounds__(256) void adapt_up_kernel(const ad_args a) {
 }
 } // namespace
 
+// parts of K, for `most` tiles: so that the tiles of a batch of one adapter each fill the chip four times, 64 numbers of K a wave at least (64 adapters of rank 64, K 4096: 13 parts, 10.3 us; 7 parts, 13.8)
+static int parts_of(const ps_adapters &s, int64_t most) { return (int)std::max<int64_t>(1, std::min<int64_t>({(4 * s.n_cu + most - 1) / most, s.KP / 256, 16})); }
+static int64_t tiles_of(const ps_adapters &s, int64_t T, bool plan) { return !plan ? T : std::min<int64_t>(T, (int64_t)s.n_slots + 1 + T / TILE); } // there can be
+static void adapt_carve(const ps_adapters &s, ad_args &a, ps_carve &ws, int64_t T, int64_t tiles, int64_t in_parts, bool plan, int32_t **count) {
+    a.h = ws.take<float>((size_t)(in_parts * s.RP * TILE));
+    if (!plan) return;
+    a.order = ws.take<int32_t>((size_t)T);
+    a.tiles = ws.take<int32_t>(1 + 3 * (size_t)tiles);
+    *count = ws.take<int32_t>((size_t)s.n_slots + 1);
+}
+// The most that any call of up to T tokens takes.
+size_t psv_adapt_most(const ps_adapters &s, int T) {
+    const bool plan = !plans_itself(T, s.N);
+    const int64_t alone = std::min<int64_t>({(int64_t)T, 256, (1 << 19) / s.N}), tiles = std::max(alone, plan ? tiles_of(s, T, true) : 0);
+    int64_t in_parts = tiles; // of one part each, or of p > 1 parts: as many tiles as still have them
+    for (int p = 2; p <= std::min<int64_t>(s.KP / 256, 16); p++) in_parts = std::max(in_parts, p * std::min<int64_t>(tiles, (4 * s.n_cu - 1) / (p - 1)));
+    ad_args a{};
+    ps_carve ws{nullptr};
+    int32_t *count = nullptr;
+    adapt_carve(s, a, ws, T, tiles, in_parts, plan, &count);
+    return ws.at;
+}
 size_t psv_adapt_space(const ps_adapters &s, int x_dtype, const void *x, int64_t ldx, int T, const int32_t *ids, const float *base_out, float *out, int64_t ldo, void *base, bool launch, hipStream_t st) {
     ad_args a{};
     const bool plan = !plans_itself(T, s.N);
-    const int most = !plan ? T : std::min<int64_t>(T, (int64_t)s.n_slots + 1 + T / TILE); // tiles there can be
-    // parts of K so that the tiles of a batch of one adapter each fill the chip four times, 64 numbers of K a wave at least (64 adapters of rank 64, K 4096: 13 parts, 10.3 us; 7 parts, 13.8)
-    a.parts = (int)std::max<int64_t>(1, std::min<int64_t>({(4 * s.n_cu + most - 1) / most, s.KP / 256, 16}));
+    const int most = (int)tiles_of(s, T, plan);
+    a.parts = parts_of(s, most);
     ps_carve ws{(char *)base};
-    a.h = ws.take<float>((size_t)a.parts * most * s.RP * TILE);
     int32_t *count = nullptr;
-    if (plan) {
-        a.order = ws.take<int32_t>((size_t)T);
-        a.tiles = ws.take<int32_t>(1 + 3 * (size_t)most);
-        count = ws.take<int32_t>((size_t)s.n_slots + 1);
-    }
+    adapt_carve(s, a, ws, T, most, (int64_t)a.parts * most, plan, &count);
     if (!launch) return ws.at;
     a.down = s.down; a.up = s.up; a.rank = s.rank; a.ids = ids; a.scale = s.scale; a.x = (const char *)x; a.base = base_out; a.out = out;
     a.N = s.N; a.K = s.K; a.KP = s.KP; a.RP = s.RP; a.ldx = ldx; a.ldo = ldo; a.n_slots = s.n_slots; a.T = T;

@@ -1186,8 +1186,43 @@ void launch_attn(ca_args a, bool many, hipStream_t st) {
         if (a.wgroups) hipLaunchKernelGGL((cache_gather_kernel<64>), dim3((unsigned)((a.n_ctx + 255) / 256), (unsigned)a.G, (unsigned)a.n_seqs), dim3(256), 0, st, a);
     }
 }
+// work-groups of 256 threads that parts may make of a launch, whose grid has fewer than 2^32 threads
+constexpr long long MOST_PARTS = 64000 * 256;
 } // namespace
 
+// The most that any call of up to n_seqs sequences and n_new tokens takes, piece by piece: fewer rows have more parts, and up to 32 rows scores.
+size_t psv_attn_most(int n_cu, const ps_kv_cache &c, const ps_cache_attn_params &p) {
+    const long long R = p.heads / c.kv_heads, size = c.dtype == PS_F32 ? 4 : 2, T = p.n_new, few = size == 4 ? T : std::min(T, 32 / R), cap = std::min(64, (c.n_ctx + 127) / 128);
+    // work-groups times parts, of up to g work-groups that `fill` of them fill the chip, each in `x` parts at least; one part needs no place
+    auto in_parts = [&](long long g, long long fill, long long x) {
+        if (x == 1) g = std::min(g, fill - 1);
+        return cap == 1 ? 0 : std::min({std::max(fill + g - 1, x * g), cap * g, MOST_PARTS});
+    };
+    auto bytes = [&](long long n_seqs, bool chunks) {
+        const long long heads = n_seqs * c.kv_heads;
+        long long part = 0;
+        if (few) {
+            const long long tiles = (few * R + 15) / 16;
+            part = (tiles > 1 ? 2 : 1) * in_parts(heads * ((tiles + 1) / 2), 3 * n_cu, (c.n_ctx + 511) / 512);
+        }
+        if (T > few) {
+            part = std::max(part, std::min<long long>(ROWS / 16, (T * R + 15) / 16) * in_parts(heads, n_cu, n_seqs > 1 ? (c.n_ctx + 1023) / 1024 : 1));
+            part = std::max(part, ROWS / 16 * in_parts(heads * ((T * R + ROWS - 1) / ROWS), n_cu, 1));
+        }
+        ps_carve ws{nullptr};
+        ws.take<float>((size_t)(heads * T * R));
+        ws.take<float>((size_t)(part * 16 * (c.dim + 2)));
+        if (chunks) ws.take<int>((size_t)n_seqs);
+        if (!p.weight_out) return ws.at;
+        ws.take<float>((size_t)(heads * c.n_ctx * ((std::min(T, 32 / R) * R + 3) / 4 * 4)));
+        if (T * R > 32) {
+            const long long block = size == 2 ? 256 : 64, blocks = (c.n_ctx + block - 1) / block, shared = T * R > 4 * QT ? heads : std::min(heads, (2 * n_cu - 1) / blocks);
+            if (shared) ws.take<float>((size_t)((2 * n_cu + shared - 1 + shared * blocks) * block));
+        }
+        return ws.at;
+    };
+    return std::max(bytes(c.n_seqs, false), c.n_seqs > 1 && cap > 1 ? bytes(std::min(c.n_seqs, 256), true) : 0);
+}
 size_t psv_attn_space(int n_cu, const ps_kv_cache &c, const ps_cache_attn_params &p, void *base, bool launch, hipStream_t st) {
     const int R = p.heads / c.kv_heads, size = c.dtype == PS_F32 ? 4 : 2;
     const long long heads = (long long)c.n_seqs * c.kv_heads, rows = (long long)p.n_new * R;
@@ -1199,7 +1234,7 @@ size_t psv_attn_space(int n_cu, const ps_kv_cache &c, const ps_cache_attn_params
     const long long groups = heads * (many ? (rows + ROWS - 1) / ROWS : (a.tiles + 1) / 2);
     // parts of the keys: until the chip is full (few rows: three times, or 512 keys each); 1024 keys each where several sequences have one work-group's rows, so that the longest does not keep the others
     // waiting (32 sequences of up to 8100, 48 rows: 230 us in one part each, 110 so)
-    a.parts = (int)std::min<long long>({std::max<long long>(((many ? 1 : 3) * n_cu + groups - 1) / groups, !many ? (c.n_ctx + 511) / 512 : rows <= ROWS && c.n_seqs > 1 ? (c.n_ctx + 1023) / 1024 : 1), (c.n_ctx + 127) / 128, 64, std::max(1ll, ((1ll << 24) - 1) / groups)}); // (a launch's grid has fewer than 2^32 threads)
+    a.parts = (int)std::min<long long>({std::max<long long>(((many ? 1 : 3) * n_cu + groups - 1) / groups, !many ? (c.n_ctx + 511) / 512 : rows <= ROWS && c.n_seqs > 1 ? (c.n_ctx + 1023) / 1024 : 1), (c.n_ctx + 127) / 128, 64, std::max(1ll, MOST_PARTS / groups)});
     a.near = p.q_row_stride >= 0 && p.q_row_stride < (1 << 28) && (p.n_new + 1ll) * (p.q_row_stride + (long long)R * c.dim) < (1 << 29);
     a.plain = c.slot_stride >= 0 && c.slot_stride < (1 << 24);
     ps_carve ws{(char *)base};

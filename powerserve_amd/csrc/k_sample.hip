@@ -655,6 +655,26 @@ void launch(const smp_args &a, hipStream_t st) {
 }
 } // namespace
 
+// the pieces of the scratch memory of `rows` rows in `all` parts together
+static void sample_carve(smp_args &a, ps_carve &ws, size_t rows, size_t all) {
+    a.top = ws.take<float>(rows * 1024);
+    a.bound = ws.take<float>(rows * 2);
+    a.cnt = ws.take<unsigned>(all * (NB + 1));
+    a.sum = ws.take<u64>(all * (NB + 1));
+    a.head = ws.take<u64>(all * PART_HEAD);
+    a.held = ws.take<unsigned>(all);
+}
+// The most that any call of up to n logits and up to `rows` rows takes: the rows that have parts are up to half the CUs, and their parts up to two a CU.
+size_t psv_sample_most(int n_cu, int64_t n, int64_t rows) {
+    const int64_t least = 1024, r = std::min<int64_t>(rows, n_cu / 2);
+    if (r < 1 || n < 4 * least) return 0;
+    int parts = 4;
+    while (parts < 64 && parts * 2 * least <= n) parts *= 2;
+    smp_args a{};
+    ps_carve ws{nullptr};
+    sample_carve(a, ws, (size_t)r, (size_t)std::min<int64_t>(r * parts, 2 * n_cu));
+    return ws.at;
+}
 size_t psv_sample_space(int n_cu, int dtype, const void *logits, int64_t n, int64_t rows, int64_t stride, const ps_sample_params *p, int32_t *ids, float *prob, void *base, bool launch_, hipStream_t st) {
     smp_args a{};
     // a row alone where there is a row for half the CUs; else 4, 8 .. 64 parts (1024 groups of a row in all) of at least a piece of 16 bytes a thread, as many as the chip takes at once
@@ -663,14 +683,7 @@ size_t psv_sample_space(int n_cu, int dtype, const void *logits, int64_t n, int6
     if (rows * 2 <= n_cu && n >= 4 * least)
         for (a.parts = 4; a.parts < 64 && a.parts * 2 * rows <= 2 * n_cu && a.parts * 2 * least <= n;) a.parts *= 2;
     ps_carve ws{(char *)base};
-    if (a.parts > 1) {
-        a.top = ws.take<float>((size_t)rows * 1024);
-        a.bound = ws.take<float>((size_t)rows * 2);
-        a.cnt = ws.take<unsigned>((size_t)rows * a.parts * (NB + 1));
-        a.sum = ws.take<u64>((size_t)rows * a.parts * (NB + 1));
-        a.head = ws.take<u64>((size_t)rows * a.parts * PART_HEAD);
-        a.held = ws.take<unsigned>((size_t)rows * a.parts);
-    }
+    if (a.parts > 1) sample_carve(a, ws, (size_t)rows, (size_t)rows * a.parts);
     if (!launch_) return ws.at;
     a.logits = logits; a.n = (int)n; a.rows = rows; a.stride = stride;
     a.temperature = p->temperature; a.top_k = p->top_k; a.top_p = p->top_p; a.min_p = p->min_p; a.u = p->u;

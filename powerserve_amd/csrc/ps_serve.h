@@ -25,6 +25,9 @@ inline void ps_allow_lds(const void *kernel, size_t bytes, std::atomic<unsigned 
     if (hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) == hipSuccess) done.fetch_or(bit, std::memory_order_release);
 }
 
+// psv_*_space: the bytes that a call takes; psv_*_most: the most that any call takes of no more sequences, new tokens, logits, rows or tokens, which is what a server that keeps one workspace asks for
+size_t psv_attn_most(int n_cu, const ps_kv_cache &c, const ps_cache_attn_params &p);
+size_t psv_sample_most(int n_cu, int64_t n, int64_t rows);
 size_t psv_attn_space(int n_cu, const ps_kv_cache &c, const ps_cache_attn_params &p, void *base, bool launch, hipStream_t st); // the bytes it takes; launch: enqueues
 void psv_advance(hipStream_t st, const ps_kv_cache &c, const int32_t *count, const int32_t *take, int n_take);
 size_t psv_evict_space(const ps_kv_cache &c, const ps_cache_evict_params &p, void *base, bool launch, hipStream_t st);
@@ -39,6 +42,7 @@ struct ps_adapters {
     float *scale = nullptr;   // [n_slots]
     int device = 0, n_cu = 256;
 };
+size_t psv_adapt_most(const ps_adapters &a, int T);
 size_t psv_adapt_space(const ps_adapters &a, int x_dtype, const void *x, int64_t ldx, int T, const int32_t *ids, const float *base_out, float *out, int64_t ldo, void *base, bool launch, hipStream_t st);
 
 // a 16-byte piece of 16-bit numbers, and the wave's fp32 accumulators

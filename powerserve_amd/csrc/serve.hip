@@ -75,7 +75,7 @@ extern "C" {
 
 size_t ps_hip_cache_attn_workspace(ps_hip_ctx *c, const ps_kv_cache *k, const ps_cache_attn_params *p) {
     if (!c || wrong_attn(k, p) || !k->n_seqs || !p->n_new) return 0;
-    return psv_attn_space(c->n_cu, *k, *p, nullptr, false, c->stream);
+    return psv_attn_most(c->n_cu, *k, *p);
 }
 int ps_hip_cache_attn(ps_hip_ctx *c, const ps_kv_cache *k, const ps_cache_attn_params *p, void *ws, size_t bytes) {
     if (!c) return 2;
@@ -131,7 +131,7 @@ static const char *wrong_sample(int64_t n, int64_t rows) {
 }
 size_t ps_hip_sample_workspace(ps_hip_ctx *c, int64_t n, int64_t rows) {
     if (!c || wrong_sample(n, rows) || !rows) return 0;
-    return psv_sample_space(c->n_cu, PS_F32, nullptr, n, rows, n, nullptr, nullptr, nullptr, nullptr, false, c->stream);
+    return psv_sample_most(c->n_cu, n, rows);
 }
 int ps_hip_sample(ps_hip_ctx *c, int dtype, const void *logits, int64_t n, int64_t rows, int64_t stride, const ps_sample_params *p, int32_t *ids, float *prob, void *ws, size_t bytes) {
     if (!c) return 2;
@@ -215,7 +215,7 @@ int ps_hip_adapters_load(ps_hip_ctx *c, ps_adapters *a, int slot, const uint16_t
 }
 size_t ps_hip_adapters_workspace(const ps_adapters *a, int T) {
     if (!a || T < 1) return 0;
-    return psv_adapt_space(*a, PS_F32, nullptr, 0, T, nullptr, nullptr, nullptr, 0, nullptr, false, nullptr);
+    return psv_adapt_most(*a, T);
 }
 int ps_hip_adapters_apply(ps_hip_ctx *c, const ps_adapters *a, int x_dtype, const void *x, int64_t ldx, int T, const int32_t *ids, const float *base, float *out, int64_t ldo, void *ws, size_t bytes) {
     if (!c) return 2;
@@ -225,7 +225,7 @@ int ps_hip_adapters_apply(ps_hip_ctx *c, const ps_adapters *a, int x_dtype, cons
     if (!T) return 0;
     if (!x || !ids || !out || !aligned(x, number_size(x_dtype)) || (const void *)out == x) SV_FAIL(c, "adapters_apply", "x, ids or out are missing, not aligned or the same");
     if (T > 1 && (ldx < a->K || ldo < a->N)) SV_FAIL(c, "adapters_apply", "rows overlap");
-    if (!ws || !aligned(ws, 16) || bytes < ps_hip_adapters_workspace(a, T)) SV_FAIL(c, "adapters_apply", "the workspace is too small or not aligned");
+    if (!ws || !aligned(ws, 16) || bytes < psv_adapt_space(*a, x_dtype, nullptr, 0, T, nullptr, nullptr, nullptr, 0, nullptr, false, nullptr)) SV_FAIL(c, "adapters_apply", "the workspace is too small or not aligned");
     SV_DEVICE(c, "adapters_apply")
     psv_adapt_space(*a, x_dtype, x, ldx, T, ids, base, out, ldo, ws, true, c->stream);
     PS_CHECK(c, hipGetLastError());

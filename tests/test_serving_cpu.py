@@ -200,3 +200,37 @@ s.apply(a(), 500, a(), a(), space=space, space_bytes=1 << 20)
 assert count("hipLaunchKernel") > 10 and count("hipMemcpy") == count("hipMemset") == count("Synchronize") == count("hipEvent") == 0
 # (the lambdas allocate their buffers through the library: no other allocation)
 """)
+
+
+def test_a_workspace_serves_every_smaller_call(child):  # noqa: F811
+    """what the workspace functions say is enough for fewer sequences, new tokens, rows or tokens too: a server keeps one for its largest step"""
+    child(MADE + """
+import random
+rng = random.Random(1)
+huge = C.c_void_p(a())  # (nothing is enqueued for real: an address that is aligned will do)
+for n, rows in ((128256, 256), (128256, 129), (128256, 128), (151936, 33), (4096, 128), (50000, 7), (8192, 100)):
+    have = ctx.sample_workspace(n, rows)
+    for r in sorted({1, 2, 3, rows, *(rng.randint(1, rows) for _ in range(30)), *(x for x in (16, 31, 32, 33, 63, 64, 65, 127, 128) if x <= rows)}):
+        for m in (n, n // 2, n // 3, 5000, 4096, 100):
+            for dtype in (0, 1, 30):
+                if m <= n: ctx.sample(a(), m, r, hip.sample_params(a()), a(), dtype=dtype, space=huge.value, space_bytes=have)
+for N, K, slots, rank in ((64, 4096, 8, 64), (14336, 4096, 64, 64), (2048, 2048, 3, 16), (1 << 20, 300, 100, 4), (128, 64, 9000, 2)):
+    s = hip.Adapters(ctx, N, K, slots, rank)
+    for T in (1, 127, 128, 253, 300, 5000):
+        have = s.workspace(T)
+        for t in range(1, T + 1, 1 if T < 400 else 37): s.apply(a(), t, a(), a(), space=huge.value, space_bytes=have)
+    s.close()
+for i in range(400):
+    dtype, S, G, dim = rng.choice((0, 1, 30)), rng.choice((1, 2, 4, 16, 32, 255, 256, 257, 300, 600)), rng.choice((1, 2, 8)), rng.choice((8, 64, 128))
+    heads, n_ctx, new = G * rng.choice((1, 4, 7, 33, 150)), rng.choice((100, 129, 300, 600, 1100, 4096, 8192, 100000)), rng.choice((1, 2, 8, 9, 24, 33, 64, 70, 100))
+    weights = {"weight_out": a()} if rng.random() < 0.6 else {}
+    have = ctx.cache_attn_workspace(cache(dtype, S, n_ctx, G, dim), attn(heads, new, **weights))
+    assert have
+    for s in {1, min(2, S), S, *(rng.randint(1, S) for _ in range(8)), *(x for x in (255, 256, 257) if x < S)}:
+        for t in {1, new, *(rng.randint(1, new) for _ in range(8)), *(x for x in (4, 5, 8, 9, 16, 17, 32, 33) if x < new)}:
+            for w in {0, len(weights)}:
+                ctx.cache_attn(cache(dtype, s, n_ctx, G, dim), attn(heads, t, **(weights if w else {})), huge.value, have)
+    e = hip.cache_evict_args(rng.choice((1, 50, 99)))
+    have = ctx.cache_evict_workspace(cache(dtype, S, n_ctx, G, dim), e)
+    for s in {1, S, rng.randint(1, S)}: ctx.cache_evict(cache(dtype, s, n_ctx, G, dim), e, huge.value, have)
+""")
