@@ -606,7 +606,8 @@ int ps_hip_sample(ps_hip_ctx *ctx, int dtype, const void *logits, int64_t n, int
  * tokens whose id is no loaded slot get out = base.  Matrices are bfloat16, every product of them exact and every sum fp32 (x in fp32 is taken whole).  base: the shared projection's output, may be out; NULL: zeros. */
 typedef struct ps_adapters ps_adapters;
 int ps_hip_adapters_create(ps_hip_ctx *ctx, int64_t N, int64_t K, int n_slots, int max_rank, ps_adapters **out);
-/* host_down [rank][K], host_up [N][rank] bfloat16 bit patterns; rank 0 empties the slot.  Waits for the stream: what was enqueued before sees the old adapter, what follows the new one. */
+/* host_down [rank][K], host_up [N][rank] bfloat16 bit patterns, none of them infinite; rank 0 empties the slot.  Waits for the ctx's stream: what was enqueued there before sees the old adapter, what follows
+ * the new one.  Calls of other contexts on the same set, on streams of their own, are the caller's to order before a load and before the set is freed. */
 int ps_hip_adapters_load(ps_hip_ctx *ctx, ps_adapters *a, int slot, const uint16_t *host_down, const uint16_t *host_up, int rank, float scale);
 void ps_hip_adapters_free(ps_hip_ctx *ctx, ps_adapters *a);
 size_t ps_hip_adapters_workspace(const ps_adapters *a, int T);

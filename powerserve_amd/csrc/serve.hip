@@ -151,6 +151,12 @@ int ps_hip_sample(ps_hip_ctx *c, int dtype, const void *logits, int64_t n, int64
 }
 
 // ------------------------------------------------------------------ low-rank adapters
+// (The other factor goes in as three numbers that add up to it, of which the last ones are 0 where the first is exact: an infinite number in a matrix times those would be NaN instead of infinity.)
+static bool any_infinite(const uint16_t *m, int64_t n) {
+    bool any = false;
+    for (int64_t i = 0; i < n; i++) any |= (m[i] & 0x7fff) == 0x7f80;
+    return any;
+}
 int ps_hip_adapters_create(ps_hip_ctx *c, int64_t N, int64_t K, int n_slots, int max_rank, ps_adapters **out) {
     if (!c) return 2;
     if (!out) SV_FAIL(c, "adapters_create", "no place for the handle");
@@ -188,6 +194,7 @@ int ps_hip_adapters_load(ps_hip_ctx *c, ps_adapters *a, int slot, const uint16_t
     if (slot < 0 || slot >= a->n_slots) SV_FAIL(c, "adapters_load", "no such slot");
     if (rank < 0 || rank > a->max_rank) SV_FAIL(c, "adapters_load", "the rank is above the set's");
     if (rank && (!down || !up)) SV_FAIL(c, "adapters_load", "no matrices");
+    if (rank && (any_infinite(down, rank * a->K) || any_infinite(up, rank * a->N))) SV_FAIL(c, "adapters_load", "a matrix holds an infinite number");
     SV_DEVICE(c, "adapters_load")
     PS_CHECK(c, hipStreamSynchronize(c->stream));
     const int32_t none = 0;

@@ -234,3 +234,23 @@ for i in range(400):
     have = ctx.cache_evict_workspace(cache(dtype, S, n_ctx, G, dim), e)
     for s in {1, S, rng.randint(1, S)}: ctx.cache_evict(cache(dtype, s, n_ctx, G, dim), e, huge.value, have)
 """)
+
+
+def test_adapters_with_infinite_numbers_are_refused(child):  # noqa: F811
+    """in either matrix, of either sign, in the last place too; the slot keeps what it had, the largest number and NaN are taken"""
+    child(MADE + """
+s = hip.Adapters(ctx, 8, 12, 2, 4)
+ones = lambda *shape: np.full(shape, 0x3f80, dtype=np.uint16)
+s.load(1, ones(3, 12), ones(8, 3))
+for bits in (0x7f80, 0xff80):
+    for i, j in ((0, 0), (2, 11), (1, 5)):
+        down = ones(3, 12)
+        down[i, j] = bits
+        assert "infinite" in quiet(lambda: s.load(1, down, ones(8, 3)))
+    for i, j in ((0, 0), (7, 2)):
+        up = ones(8, 3)
+        up[i, j] = bits
+        assert "infinite" in quiet(lambda: s.load(1, ones(3, 12), up))
+for bits in (0x7f7f, 0xff7f, 0x7fc0, 0x7f81, 0x0001):
+    s.load(1, np.full((3, 12), bits, dtype=np.uint16), np.full((8, 3), bits, dtype=np.uint16))
+""")
