@@ -4,7 +4,8 @@ import pytest
 
 import serving_ref as ref
 from serving_ref import BF16, F16, F32
-from test_gpu_serving import NAN, Step, random_tree
+from test_gpu_serving import NAN, Step, random_tree, run_adapters
+from test_gpu_serving import test_eviction as evicts
 
 pytestmark = pytest.mark.gpu
 
@@ -128,3 +129,27 @@ def test_many_rows_are_as_exact_as_few(ctx, hip, dtype, n_new, as_tree):
         err = np.abs(out[i] - want)
         assert (err <= bound).all(), (i, float((err / bound).max()))
     s.free()
+
+
+# ---------------------------------------------------------------------------------------------------------------------------- paths that ordinary sizes do not take
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("S,G,n_ctx,n_new", [(64, 8, 256, 12), (32, 8, 500, 40), (128, 4, 200, 9)])
+def test_weights_of_portions_of_many_sequences(ctx, hip, dtype, S, G, n_ctx, n_new):
+    """33 to 256 rows a kv head, slots enough to fill the chip: a work-group has all rows of its slots, of which the causal mask leaves some out"""
+    rng = np.random.default_rng(S)
+    n_kv = rng.integers(0, n_ctx + 1, S)
+    Step(ctx, hip, rng, dtype, 4 * G, G, 32, n_ctx, n_kv, n_new, count=np.where(np.arange(S) % 7 == 6, 0, rng.integers(1, n_new + 1, S))).run().check()
+
+
+@pytest.mark.parametrize("dtype,dim", [(F32, 8), (BF16, 16)])
+@pytest.mark.parametrize("n_ctx,n_kv,keep,recent,first", [(32768, [32768, 16384, 16385, 20000], 2048, 300, 4), (20001, [20001, 17000], 16390, 16000, 0), (32767, [32767, 30000], 30001, 1, 1), (16400, [16399], 1, 0, 0)])
+@pytest.mark.parametrize("in_place", [False, True])
+def test_eviction_with_keys_in_lds_and_more_slots_than_are_loaded_at_once(ctx, hip, dtype, dim, n_ctx, n_kv, keep, recent, first, in_place):
+    evicts(ctx, hip, dtype, dim, n_ctx, n_kv, keep, recent, first, in_place)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("T,N,slots", [(3000, 1000, 2999), (3000, 997, 3500), (4200, 601, 4300)])
+def test_adapters_of_more_than_256_columns_a_work_group(ctx, hip, dtype, T, N, slots):
+    rng = np.random.default_rng(N)
+    run_adapters(ctx, hip, rng, dtype, T, N, 24, [2, 1] * (slots // 2), rng.integers(-1, slots + 2, T))

@@ -254,3 +254,51 @@ for bits in (0x7f80, 0xff80):
 for bits in (0x7f7f, 0xff7f, 0x7fc0, 0x7f81, 0x0001):
     s.load(1, np.full((3, 12), bits, dtype=np.uint16), np.full((8, 3), bits, dtype=np.uint16))
 """)
+
+
+def test_each_operator_of_a_step_is_its_launches_and_nothing_else(child):  # noqa: F811
+    """every operator, the sampler in parts among them, alone between two looks at the counts: so many launches, and no allocation, copy, memset, wait or event"""
+    child(MADE + """
+s = hip.Adapters(ctx, 8, 12, 2, 4)
+s.load(0, np.ones((3, 12), dtype=np.uint16), np.ones((8, 3), dtype=np.uint16))
+c, c16, tree = cache(), cache(dtype=30), a()
+one, two, many = attn(weight_out=a(), tree=tree), attn(new=3), attn(new=40, k_new=a(), v_new=a(), weight_out=a())
+long_one = cache(dtype=30, S=3, n_ctx=4096)
+evict, settings, x, y, z, e = hip.cache_evict_args(8), hip.sample_params(a()), a(), a(), a(), a()
+room = max(ctx.sample_workspace(100000, 2), ctx.cache_attn_workspace(long_one, many), s.workspace(500), 1 << 20)
+ws = a(room)
+for launches, call in (
+    (2, lambda: ctx.cache_attn(c, one, ws, room)),           # rows in one part, weights from the scores
+    (1, lambda: ctx.cache_attn(c, two, ws, room)),
+    (2, lambda: ctx.cache_attn(long_one, two, ws, room)),    # parts and their join
+    (5, lambda: ctx.cache_attn(long_one, many, ws, room)),   # new rows, rows, join, weights, their sums
+    (4, lambda: ctx.cache_attn(c16, many, ws, room)),        # one part
+    (1, lambda: ctx.cache_advance(c, x)), (2, lambda: ctx.cache_advance(c, x, y, 3)),
+    (2, lambda: ctx.cache_evict(c, evict, ws, room)),
+    (3, lambda: ctx.sample(x, 100000, 2, settings, y, prob=z, space=ws, space_bytes=room)), (1, lambda: ctx.sample(x, 100000, 200, settings, y, space=ws, space_bytes=room)),
+    (2, lambda: s.apply(x, 5, y, z, base=e, space=ws, space_bytes=room)), (3, lambda: s.apply(x, 500, y, z, space=ws, space_bytes=room)),
+):
+    fake.fake_reset()
+    call()
+    assert count("hipLaunchKernel") == launches, (launches, count("hipLaunchKernel"))
+    for name in ("hipMalloc", "hipHostMalloc", "hipFree", "hipMemcpyAsync", "hipMemsetAsync", "hipStreamSynchronize", "hipDeviceSynchronize", "hipEventRecord", "hipEventSynchronize", "put_kernel", "pin_copy_kernel"):
+        assert count(name) == 0, (launches, name)
+""")
+
+
+def test_adapters_launch_on_the_contexts_device_and_leave_the_callers_current(child):  # noqa: F811
+    child(MADE + """
+dev = C.c_int()
+s = hip.Adapters(ctx, 8, 12, 2, 4)
+other = hip.Ctx(1)
+def current():
+    fake.hipGetDevice(C.byref(dev))
+    return dev.value
+x, y, z = a(), a(), a()
+for f in (lambda: s.apply(x, 5, y, z, space=space, space_bytes=1 << 20), lambda: s.load(0, np.ones((3, 12), dtype=np.uint16), np.ones((8, 3), dtype=np.uint16)), lambda: hip.Adapters(ctx, 8, 12, 2, 4)):
+    for d in (1, 0):
+        fake.hipSetDevice(d)
+        fake.fake_reset()
+        f()
+        assert current() == d and count("hipSetDevice") == 2 * d, (d, count("hipSetDevice"))
+""")
