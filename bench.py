@@ -618,15 +618,21 @@ TRAFFIC_FILE = os.path.join("profiles", "pmc_traffic.json")  # the PMC record (t
 
 
 def kernel_sources_sha16():
-    """sha256[:16] over the kernel sources and the build recipe: what a PMC record must have been taken on to describe the library that runs"""
+    """sha256[:16] over the sources that the quantized path's kernels are built from, what those include, and the compiler's flags: what a PMC record must have been taken on to describe the kernels that run.
+    (The layer-list models' and the serving operators' sources are not in those kernels.)"""
     import hashlib
-    root = os.path.dirname(os.path.abspath(__file__))
+    import re
+    from powerserve_amd import build
     h = hashlib.sha256()
-    csrc = os.path.join(root, "powerserve_amd", "csrc")
-    for f in sorted(os.listdir(csrc)):
-        if f.endswith((".hip", ".h")):
-            h.update(f.encode()); h.update(open(os.path.join(csrc, f), "rb").read())
-    h.update(open(os.path.join(root, "powerserve_amd", "build.py"), "rb").read())
+    seen, todo = set(), [s for s in build.SOURCES if s == "ctx.hip" or s not in build.SEQ_SOURCES + build.SERVE_SOURCES]
+    while todo:
+        f = todo.pop()
+        if f not in seen:
+            seen.add(f)
+            todo += [i for i in re.findall(r'^#include "([^"/]+)"', open(os.path.join(build.CSRC, f)).read(), re.M)]
+    for f in sorted(seen):
+        h.update(f.encode()); h.update(open(os.path.join(build.CSRC, f), "rb").read())
+    h.update(repr([f for f in build.FLAGS if not f.startswith("-I")] + sorted(build.NOSLP & seen)).encode())
     return h.hexdigest()[:16]
 
 
