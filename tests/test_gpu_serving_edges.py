@@ -131,6 +131,28 @@ def test_many_rows_are_as_exact_as_few(ctx, hip, dtype, n_new, as_tree):
     s.free()
 
 
+@pytest.mark.parametrize("n_new", [1, 60])
+def test_small_products_of_a_score_are_not_all_lost_beside_a_large_one(ctx, hip, n_new):
+    """fp32: a score of 1 and 63 times 2^-26 is a sum of even and one of odd numbers, of which one has the 1: the other's 32 small products add up exactly and their sum does to the 1, so that 31 of them at most are
+    lost.  Times 2^20, beside a slot whose score is 1: the quotient of the two weights is e^(63/64), the exponent 31/64 too small at most."""
+    rng = np.random.default_rng(2)
+    s = Step(ctx, hip, rng, F32, 4, 2, 64, 80, [2], n_new, tree=np.zeros((1, n_new, n_new)))
+    s.q[...] = 1
+    s.k[0, :2] = 0
+    s.k[0, 0] = 2.0**-26
+    s.k[0, :2, 0, :, 0] = 1
+    s.weight[...] = 0
+    again(s, "q", "k")
+    s.d["weight"].free()
+    s.d["weight"] = ctx.to_device(s.weight)
+    s.cache.weight = s.d["weight"].ptr
+    s.args.scale = 2.0**20
+    w = s.run().d["weight_out"].numpy().astype(np.float64)[0, :, :2]
+    got = np.log(w[:, 0] / w[:, 1])
+    assert (got >= 32 / 64 - 1e-5).all() and (got <= 63 / 64 + 1e-5).all(), got  # (1e-5: e^x to 2^-22, sums of at most 120 weights)
+    s.free()
+
+
 # ---------------------------------------------------------------------------------------------------------------------------- paths that ordinary sizes do not take
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
 @pytest.mark.parametrize("S,G,n_ctx,n_new", [(64, 8, 256, 12), (32, 8, 500, 40), (128, 4, 200, 9)])
