@@ -229,31 +229,62 @@ def _ptr(a: np.ndarray):
     return a.ctypes.data_as(C.c_void_p)
 
 
-def _dev(a):
-    """Device address of a DevArray, of anything with a data_ptr(), or as given (None: none)."""
+_TYPE_NAMES = {}  # of element types, numpy's and torch's
+
+
+def _type_name(a) -> str:
+    t = getattr(a, "dtype", "")
+    n = _TYPE_NAMES.get(t)
+    if n is None:
+        n = _TYPE_NAMES[t] = str(t).split(".")[-1]
+    return n
+
+
+def _wrong(a, why: str):
+    return PSHipError(f"an array {tuple(getattr(a, 'shape', ()))} {_type_name(a)} {why}")
+
+
+def _dev(a, kind: str | None = None):
+    """Device address of a DevArray, of a tensor on the device (anything with a data_ptr()), or as given (None: none).  kind: the type of its elements, one behind the other (bytes may be anything's memory).
+    Host memory, a freed array and another type would be read as numbers that nobody wrote, or fault the device."""
     if a is None or isinstance(a, int):
         return a
-    return a.ptr if hasattr(a, "ptr") else a.data_ptr()
+    if isinstance(a, DevArray):
+        at = a.ptr
+        if not at:
+            raise _wrong(a, "that was freed")
+    elif hasattr(a, "data_ptr"):
+        if not getattr(a, "is_cuda", True):
+            raise _wrong(a, "in host memory: it has to be the device's")
+        if kind and not a.is_contiguous():
+            raise _wrong(a, "whose elements are not one behind the other")
+        at = a.data_ptr()
+    else:
+        raise PSHipError(f"{type(a).__name__} is not an array in device memory")
+    if kind and _type_name(a) not in (kind, "uint8", "int8"):
+        raise _wrong(a, f"has to be {kind}")
+    return at
 
 
 def kv_cache(dtype: int, k, v, n_kv, n_seqs: int, n_ctx: int, kv_heads: int, dim: int, pos=None, weight=None, strides=None) -> KVCache:
     """The caches of one attention layer (ps_kv_cache): by default numbers of [n_seqs][n_ctx][kv_heads][dim], or strides = (sequence, slot, head).  The buffers stay the caller's."""
     s = strides or (n_ctx * kv_heads * dim, kv_heads * dim, dim)
-    return KVCache(dtype, n_seqs, n_ctx, kv_heads, dim, 0, _dev(k), _dev(v), *s, _dev(n_kv), _dev(pos), _dev(weight))
+    return KVCache(dtype, n_seqs, n_ctx, kv_heads, dim, 0, _dev(k), _dev(v), *s, _dev(n_kv, "int32"), _dev(pos, "int32"), _dev(weight, "float32"))
 
 
 def cache_attn_args(q, out, heads: int, n_new: int, scale: float, k_new=None, v_new=None, count=None, pos_new=None, tree=None, weight_out=None, strides=(0, 0, 0, 0, 0, 0)) -> CacheAttnParams:
     """What Ctx.cache_attn takes beside the caches (ps_cache_attn_params): made once for a step's buffers, passed every step."""
-    return CacheAttnParams(heads, n_new, scale, 0, _dev(q), _dev(out), _dev(k_new), _dev(v_new), *strides, _dev(count), _dev(pos_new), _dev(tree), _dev(weight_out))
+    return CacheAttnParams(heads, n_new, scale, 0, _dev(q), _dev(out), _dev(k_new), _dev(v_new), *strides, _dev(count, "int32"), _dev(pos_new, "int32"), _dev(tree, "bool"),
+                           _dev(weight_out, "float32"))
 
 
 def cache_evict_args(keep: int, recent: int = 0, first: int = 0, weight_out=None, pos_out=None, n_kv_out=None) -> CacheEvictParams:
-    return CacheEvictParams(keep, recent, first, 0, _dev(weight_out), _dev(pos_out), _dev(n_kv_out))
+    return CacheEvictParams(keep, recent, first, 0, _dev(weight_out, "float32"), _dev(pos_out, "int32"), _dev(n_kv_out, "int32"))
 
 
 def sample_params(u, temperature=None, top_k=None, top_p=None, min_p=None) -> SampleParams:
     """Settings of a batch of requests, one number a row each (device arrays; None: off)."""
-    return SampleParams(_dev(temperature), _dev(top_k), _dev(top_p), _dev(min_p), _dev(u))
+    return SampleParams(_dev(temperature, "float32"), _dev(top_k, "int32"), _dev(top_p, "float32"), _dev(min_p, "float32"), _dev(u, "float32"))
 
 
 class Ctx:
@@ -316,7 +347,8 @@ class Ctx:
         self.check(self.L.ps_hip_event_elapsed_ms(self.h, a, b, C.byref(ms)))
         return ms.value
 
-    # ---- a serving step of many sequences (include/ps_hip.h; device buffers: addresses, DevArrays, or anything with a data_ptr())
+    # ---- a serving step of many sequences (include/ps_hip.h; device buffers: addresses, DevArrays, or tensors on the device.  Calls go to the
+    # context's own stream, ps_hip_stream: what another stream has written, the workspace's first filling too, is waited for by the caller)
     def cache_attn_workspace(self, cache: KVCache, args: CacheAttnParams) -> int:
         return self.L.ps_hip_cache_attn_workspace(self.h, cache, args)
 
@@ -326,7 +358,7 @@ class Ctx:
 
     def cache_advance(self, cache: KVCache, count, take=None, n_take: int = 0):
         """New tokens, or the accepted path of a tree, become part of the caches (ps_hip_cache_advance)."""
-        self.check(self.L.ps_hip_cache_advance(self.h, cache, _dev(count), _dev(take), n_take))
+        self.check(self.L.ps_hip_cache_advance(self.h, cache, _dev(count, "int32"), _dev(take, "int32"), n_take))
 
     def cache_evict_workspace(self, cache: KVCache, args: CacheEvictParams) -> int:
         return self.L.ps_hip_cache_evict_workspace(self.h, cache, args)
@@ -340,7 +372,7 @@ class Ctx:
 
     def sample(self, logits, n: int, rows: int, params: SampleParams, ids, prob=None, dtype: int = F32, stride: int | None = None, space=None, space_bytes: int = 0):
         """A token per row of logits (ps_hip_sample)."""
-        self.check(self.L.ps_hip_sample(self.h, dtype, _dev(logits), n, rows, n if stride is None else stride, params, _dev(ids), _dev(prob), _dev(space), space_bytes))
+        self.check(self.L.ps_hip_sample(self.h, dtype, _dev(logits), n, rows, n if stride is None else stride, params, _dev(ids, "int32"), _dev(prob, "float32"), _dev(space), space_bytes))
 
     # ---- weights
     def upload_weight(self, dtype: int, blocks: np.ndarray, K: int, N: int) -> "Weight":
@@ -424,7 +456,7 @@ class Adapters:
 
     def apply(self, x, T: int, ids, out, base=None, dtype: int = F32, ldx: int | None = None, ldo: int | None = None, space=None, space_bytes: int = 0):
         """out[t] = base[t] + scale * up (down x[t]) with the adapter ids[t] (ps_hip_adapters_apply)."""
-        self.ctx.check(self.ctx.L.ps_hip_adapters_apply(self.ctx.h, self.h, dtype, _dev(x), self.K if ldx is None else ldx, T, _dev(ids), _dev(base), _dev(out), self.N if ldo is None else ldo, _dev(space),
+        self.ctx.check(self.ctx.L.ps_hip_adapters_apply(self.ctx.h, self.h, dtype, _dev(x), self.K if ldx is None else ldx, T, _dev(ids, "int32"), _dev(base), _dev(out), self.N if ldo is None else ldo, _dev(space),
                                                         space_bytes))
 
     def close(self):

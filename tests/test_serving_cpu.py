@@ -302,3 +302,43 @@ for f in (lambda: s.apply(x, 5, y, z, space=space, space_bytes=1 << 20), lambda:
         f()
         assert current() == d and count("hipSetDevice") == 2 * d, (d, count("hipSetDevice"))
 """)
+
+
+def test_arrays_that_are_not_the_devices_or_not_of_the_type_are_refused(child):  # noqa: F811
+    """host tensors and numpy arrays, freed arrays, 64-bit lengths, views with gaps: refused where the address is taken, not read on the device"""
+    child(MADE + """
+import torch
+class On:  # a tensor as one on the device looks
+    def __init__(self, x): self.x, self.dtype, self.shape, self.device = x, x.dtype, x.shape, torch.device("cuda", 0)
+    def data_ptr(self): return self.x.data_ptr()
+    def is_contiguous(self): return self.x.is_contiguous()
+dev = lambda *s, dtype=torch.int32: On(torch.zeros(*s, dtype=dtype))
+k = a()
+def made(n_kv, **more): return lambda: hip.kv_cache(0, k, k + 64, n_kv, 2, 64, 2, 64, **more)
+freed = ctx.to_device(np.zeros(2, np.int32))
+made(freed)()
+made(dev(2))()
+assert "host" in refused(made(torch.zeros(2, dtype=torch.int32))) and "device memory" in refused(made(np.zeros(2, np.int32))) and "device memory" in refused(made([0, 0]))
+assert "int32" in refused(made(dev(2, dtype=torch.int64))) and "int32" in refused(made(dev(2, dtype=torch.float32))) and "int32" in refused(made(ctx.to_device(np.zeros(2, np.int64))))
+assert "behind the other" in refused(made(On(torch.zeros(1, dtype=torch.int32).expand(2)))) and "behind the other" in refused(made(On(torch.zeros(4, dtype=torch.int32)[::2])))
+freed.free()
+assert "freed" in refused(made(freed))
+assert "float32" in refused(made(dev(2), weight=dev(2, 2, 64, dtype=torch.float64))) and "int32" in refused(made(dev(2), pos=dev(2, 2, 64, dtype=torch.int64)))
+made(dev(2), weight=dev(2, 2, 64, dtype=torch.float32), pos=dev(2, 2, 64))()
+made(ctx.to_device(np.zeros(8, np.uint8)))()  # a piece of somebody's memory
+q = On(torch.zeros(2, 3, 4, 64).transpose(0, 1))  # rows have strides of their own
+hip.cache_attn_args(q, k, 4, 3, 0.1, tree=dev(2, 3, 3, dtype=torch.bool), count=dev(2))
+hip.cache_attn_args(q, k, 4, 3, 0.1, tree=dev(2, 3, 3, dtype=torch.uint8))
+for x in ({"tree": dev(2, 3, 3)}, {"count": dev(2, dtype=torch.int64)}, {"weight_out": dev(2)}, {"pos_new": dev(2, 3, dtype=torch.int64)}, {"k_new": torch.zeros(4)}):
+    refused(lambda: hip.cache_attn_args(q, k, 4, 3, 0.1, **x))
+for x in ({"u": dev(2, dtype=torch.float64)}, {"u": k, "top_k": dev(2, dtype=torch.int64)}, {"u": k, "temperature": torch.ones(2)}, {"u": k, "min_p": On(torch.zeros(1).expand(2))}): refused(lambda: hip.sample_params(**x))
+refused(lambda: hip.cache_evict_args(5, n_kv_out=dev(2, dtype=torch.int64)))
+p = hip.sample_params(k)
+fake.fake_reset()
+refused(lambda: ctx.sample(np.zeros((2, 9), np.float32), 9, 2, p, k))
+refused(lambda: ctx.sample(k, 9, 2, p, dev(2, dtype=torch.int64)))
+refused(lambda: ctx.cache_advance(cache(), dev(2, dtype=torch.int64)))
+s = hip.Adapters(ctx, 8, 12, 2, 4)
+refused(lambda: s.apply(k, 5, dev(5, dtype=torch.int64), k, space=space, space_bytes=1 << 20))
+assert count("hipLaunchKernel") == 0
+""")
