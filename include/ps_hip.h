@@ -586,8 +586,8 @@ typedef struct {
 size_t ps_hip_cache_evict_workspace(ps_hip_ctx *ctx, const ps_kv_cache *cache, const ps_cache_evict_params *p);
 int ps_hip_cache_evict(ps_hip_ctx *ctx, const ps_kv_cache *cache, const ps_cache_evict_params *p, void *workspace, size_t workspace_bytes);
 
-/* Sampling, the stages of the host's sampler chain in its order (top-k, temperature, soft-max, top-p, draw) with min-p beside top-p and the random number given: the candidates of a row of logits are
- * taken from the largest to the smallest, equal ones by index; NaN and minus infinity are none.  With w = exp((logit - largest) / temperature): the first top_k (<= 0: all); of those the shortest
+/* Sampling, the stages of the host's sampler chain behind its penalties and banned tokens (which are for the caller to put into the logits), in its order: top-k, temperature, soft-max, top-p, draw, with
+ * min-p behind top-p and the random number given.  The candidates of a row of logits are taken from the largest to the smallest, equal ones by index; NaN and minus infinity are none.  With w = exp((logit - largest) / temperature): the first top_k (<= 0: all); of those the shortest
  * beginning whose w add up to top_p of theirs (>= 1 or NaN: all; at least one); of those the ones with w >= min_p (<= 0 or NaN: all; the largest always stays); then the first whose w, added up to
  * and with it, exceed u times the sum of the ones left (u < 0 or NaN: 0; u >= 1: the last).  A temperature that is not above 0 takes the first candidate.  A row without candidates gives id -1 and
  * probability 0.  A weight is within 2^-27 of itself, and weights are added as whole multiples of 2^-38 (2^-45 for vocabularies of up to 2^17) or less of the largest one, so that no order of work

@@ -9,9 +9,10 @@
 // S^T = K Q^T, so that a lane has one row and maximum and sum run over its own registers and two lane moves; the second product O^T = V^T P^T takes its 32 keys in any order that both operands
 // share, so a lane's weights are its piece of the operand as they are.  16-bit values pass through LDS, a wave's own stretch, and come back transposed (ds_read_b64_tr_b16: 4 keys x 16 numbers).
 // Lengths are read on the device; a part is ceil(length / parts) keys, so that a fixed grid serves any length.
-// Measured, dim 128, 32 query heads of 8, bf16: one token of 32 sequences that hold 17 to 8191 slots, with weights, 51 + 10 us, 187 MB of keys and values at 3.7 TB/s (a plain read of 1 GiB: 4.0) -- memory
-// bounds it; 2048 tokens behind 2047, 138 + 88 us for 103 and 52 GFLOP, 750 and 590 TFLOP/s (the library's product of 8192^3: 1130) -- the vector units' soft-max beside the matrix units, which two
-// waves a SIMD overlap in part; one token behind 100 in fp32 (14 heads of 2, dim 64), 8 + 4 us: latency of lengths, keys, sums and two launches.
+// Measured, dim 128, 32 query heads of 8, bf16: one token of 32 sequences that hold 17 to 8191 slots, with weights, 54 + 10 us, 187 MB of keys and values at 3.5 TB/s (the library's sum over 1 GiB 4.0, this
+// repository's mat-vec 4.8) -- memory, and short work-groups whose plan and first block's loads nothing hides; 2048 tokens behind 2047, 175 + 90 us for 103 and 52 GFLOP, 590 and 580 TFLOP/s (the library's product of
+// 8192^3: 1130) -- the soft-max on the vector units and the products on the matrix units, busy 55 and 51 % of the CUs' time in the first and 47 and 30 % in the second: they hardly run at the same time; one
+// token behind 100 in fp32 (14 heads of 2, dim 64), 9 + 4 us: latency of lengths, keys, sums and two launches.
 #include "ps_serve.h"
 
 #include <algorithm>
@@ -210,7 +211,7 @@ __device__ __forceinline__ bool shared_part(const ca_args &a, int id, int blocks
     return true;
 }
 // The next block's keys and values are on their way while one is worked on; two work-groups a CU (three or four leave no registers for that: slower).  fp32 runs on v_mfma_f32_16x16x4: 1024 tokens behind
-// 1000, dim 64 57 TFLOP/s, dim 128, whose registers leave one work-group a CU, 52 (the library's product: 153).
+// 1000, dim 64 55 TFLOP/s, dim 128, whose registers leave one work-group a CU, 50 (the library's product: 153).
 template <class E, int DP, int RT>
 __global__ __launch_bounds__(256, E::SIZE == 4 && DP == 128 ? 1 : 2) void cache_attn_kernel(const ca_args a) {
     constexpr int NS = STEPS<E, DP>, ND = DP / 16, OP = DP + 4, VR = DP + VPAD;
@@ -725,11 +726,12 @@ __global__ __launch_bounds__(256) void cache_append_kernel(const ca_args a, int 
 // Many rows of a 16-bit cache: 128 of a kv head against a part of its keys, a wave 32 of them against all, 64 keys at a time through two LDS stages that the four waves fill.  The products are
 // v_mfma_f32_32x32x16: S^T = K Q^T with the queries in registers (a lane: one row, 16 keys a tile), O^T = V^T P^T with the weights as they come, values transposed on their way out of LDS.
 // The weights go into the second product as two 16-bit numbers each, as in cache_attn_kernel, so that a token's result is as exact among many new tokens as among few; one number each, 2^-9 of a weight off
-// (bf16), would take a third fewer matrix instructions (2048 tokens behind 2047, all launches: 214 us instead of 248).  Their sum is taken before they are rounded.
-// What bounds it: a wave and 64 keys take 48 matrix instructions of 32 clocks, 32 KB of operands from LDS and some 300 vector instructions; two waves a SIMD overlap them in part, at the 2.0 GHz that the card holds
-// under it (2048 tokens behind 2047: 138 us, 750 TFLOP/s).  Work-groups of eight waves read a tile for twice the rows, and their sizes even out worse (168 us there; 8192 tokens 5 % faster).
+// (bf16), would take a third fewer matrix instructions (2048 tokens behind 2047: 138 us instead of 175).  Their sum is taken before they are rounded.
+// What bounds it: a wave and 64 keys take 48 matrix instructions of 32 clocks, 32 KB of operands from LDS and some 300 vector instructions, which two waves a SIMD hardly run at the same time: matrix units 51 % and
+// vector units 55 % of the CUs' time (2048 tokens behind 2047: 175 us, 590 TFLOP/s, 880 with the weights' second numbers).  Work-groups of eight waves read a tile for twice the rows, and their sizes even out
+// worse (with one number a weight 168 us there instead of 138; 8192 tokens 5 % faster).
 constexpr int ROWS = 128, KEYS = 64;
-// the same for a lane's 16 keys of a tile of 32, x + 8 (i / 4) + i % 4
+// which of new tokens x + 8 (i / 4) + i % 4, a lane's 16 keys of a tile of 32, token tok sees, as sees4
 __device__ __forceinline__ unsigned sees16(const ca_args &a, const ca_lens &L, int s, int tok, int x) {
     unsigned bits = 0;
 #pragma unroll
@@ -832,7 +834,7 @@ __global__ __launch_bounds__(256, 2) void cache_rows_kernel(const ca_args a) {
         for (int st = 0; st < KS; st++)
 #pragma unroll
             for (int u = 0; u < 2; u++) z[u] = mfma32<E>(*(const pv_u4 *)(kl[cur] + (32 * u + c) * KR + 16 * st + 8 * h), qf[st], z[u]);
-        // keys are loaded six products ahead, not two as the compiler has them (2048 tokens behind 2047: 152 us, 149 so)
+        // keys are loaded six products ahead, not two as the compiler has them (4 sequences of 1801 to 4001, trees of 24 tokens: 25.0 us, 26.2 without; a portion the same)
         __builtin_amdgcn_sched_group_barrier(0x100, 6, 0);
 #pragma unroll
         for (int i = 0; i < 2 * KS - 6; i++) {
@@ -1234,8 +1236,8 @@ size_t psv_attn_space(int n_cu, const ps_kv_cache &c, const ps_cache_attn_params
     const long long heads = (long long)c.n_seqs * c.kv_heads, rows = (long long)p.n_new * R;
     ca_args a{};
     a.tiles = (int)((rows + 15) / 16);
-    // more than 32 rows of a 16-bit cache: 128 rows a work-group (one side and the other, with weights, bf16, 32 heads of 8, dim 128: 4 sequences of 1801 to 4001, 20 rows 40 and 43 us, 32 rows 44 and 44; 32 sequences
-    // of up to 8100, 20 rows 90 and 102, 32 rows 104 and 102)
+    // more than 32 rows of a 16-bit cache: 128 rows a work-group (one side and the other, bf16, 32 heads of 8, dim 128, with weights: 4 sequences of 1801 to 4001, 20 rows 42 and 40 us, 32 rows 36 and 40; 32 sequences
+    // of up to 8100, 20 rows 76 and 95, 32 rows 91 and 96; without: 40 and 30, 32 and 31; 63 and 58, 65 and 59)
     const bool many = size == 2 && rows > 32;
     const long long groups = heads * (many ? (rows + ROWS - 1) / ROWS : (a.tiles + 1) / 2);
     // parts of the keys: until the chip is full (few rows: three times, or 512 keys each); 1024 keys each where several sequences have one work-group's rows, so that the longest does not keep the others

@@ -9,8 +9,9 @@
 //   high temperature) every digit is a pass over the row.
 //   Weights e^-z -- of z in 64 bits, e^-(bin / 32) from a table times a polynomial of what is left, below 1/32 -- are added as whole multiples of 2^-scale of the largest one: any order of
 //   work gives the same sums, and what a weight is off by, 2^-28 of it to either side alike, moves one draw in millions to a neighbour, where 32-bit sums would move one in some thousands.
-// Measured: one row of 128256 in fp32, 3 + 7 + 10 us, the latency of the passes and of a stage's steps; 33 rows of 151936 in bf16, 5 + 21 + 17, the second pass's 64-bit arithmetic and its additions to the LDS; 256
-// such rows of fp32 in one launch, 116 us: 15 the first pass (131 MB), 30 the second where the head alone counts and 55 where all do, 14 for each place that lies behind the head, 1 for one in it.
+// Measured: one row of 128256 in fp32, 3 + 7 + 10 us, the latency of the passes and of a stage's steps; 33 rows of 151936 in bf16, 4 + 21 + 17, the second pass's 64-bit arithmetic and its additions to the LDS; 256
+// such rows of fp32 in one launch, 116 us: 15 the first pass (131 MB), 30 the second where the head alone counts and 55 where all do, 14 for each place that lies behind the head, 1 for one in it (vector units 49 % busy; waves wait 64 % of
+// their time, for the row, for LDS and for each other).
 //   sample_top_kernel   the first pass over a part of a row
 //   sample_head_kernel  the second pass over a part
 //   sample_pick_kernel  the stages; with few parts of a row (many rows) it makes both passes itself
@@ -21,7 +22,7 @@
 
 namespace {
 typedef unsigned long long u64;
-constexpr int NB = 1280, LIST = 2048, HEAD = 8192, PICK = 1024; // bins below z = 40; candidates of a sorted list, of the head; threads of a pick
+constexpr int NB = 1280, LIST = 2048, HEAD = 8192, PICK = 1024; // bins below z = 40; candidates of a bin's list, of the head; threads of a pick
 constexpr int PART_HEAD = 2048; // of a part
 constexpr int QUANTILE = 1014; // of the 1024 groups' largest logits: the head's bound where no count gives one
 constexpr double WIDTH = 1.0 / 32;
