@@ -244,6 +244,24 @@ def _wrong(a, why: str):
     return PSHipError(f"an array {tuple(getattr(a, 'shape', ()))} {_type_name(a)} {why}")
 
 
+BYTES = ("uint8", "int8")  # anything's memory
+NUMBERS = {F32: ("float32", *BYTES), F16: ("float16", "uint16", "int16", *BYTES), BF16: ("bfloat16", "uint16", "int16", *BYTES)}  # the element types that an array of each may have
+
+
+def _rows(a, dense: bool):
+    """_dev of an array of numbers whose rows have strides of their own; dense: they are not given, so that the rows have to be one behind the other"""
+    if dense and hasattr(a, "is_contiguous") and not a.is_contiguous():
+        raise _wrong(a, "whose rows are not one behind the other, without strides")
+    return _dev(a)
+
+
+def _numbers(a, dtype: int, dense: bool):
+    """_rows of numbers of dtype"""
+    if not (a is None or isinstance(a, int)) and _type_name(a) not in NUMBERS.get(dtype, ()):
+        raise _wrong(a, f"is not one of type {dtype}")
+    return _rows(a, dense)
+
+
 def _dev(a, kind: str | None = None):
     """Device address of a DevArray, of a tensor on the device (anything with a data_ptr()), or as given (None: none).  kind: the type of its elements, one behind the other (bytes may be anything's memory).
     Host memory, a freed array and another type would be read as numbers that nobody wrote, or fault the device."""
@@ -261,7 +279,7 @@ def _dev(a, kind: str | None = None):
         at = a.data_ptr()
     else:
         raise PSHipError(f"{type(a).__name__} is not an array in device memory")
-    if kind and _type_name(a) not in (kind, "uint8", "int8"):
+    if kind and _type_name(a) not in (kind, *BYTES):
         raise _wrong(a, f"has to be {kind}")
     return at
 
@@ -269,13 +287,14 @@ def _dev(a, kind: str | None = None):
 def kv_cache(dtype: int, k, v, n_kv, n_seqs: int, n_ctx: int, kv_heads: int, dim: int, pos=None, weight=None, strides=None) -> KVCache:
     """The caches of one attention layer (ps_kv_cache): by default numbers of [n_seqs][n_ctx][kv_heads][dim], or strides = (sequence, slot, head).  The buffers stay the caller's."""
     s = strides or (n_ctx * kv_heads * dim, kv_heads * dim, dim)
-    return KVCache(dtype, n_seqs, n_ctx, kv_heads, dim, 0, _dev(k), _dev(v), *s, _dev(n_kv, "int32"), _dev(pos, "int32"), _dev(weight, "float32"))
+    return KVCache(dtype, n_seqs, n_ctx, kv_heads, dim, 0, _numbers(k, dtype, not strides), _numbers(v, dtype, not strides), *s, _dev(n_kv, "int32"), _dev(pos, "int32"), _dev(weight, "float32"))
 
 
 def cache_attn_args(q, out, heads: int, n_new: int, scale: float, k_new=None, v_new=None, count=None, pos_new=None, tree=None, weight_out=None, strides=(0, 0, 0, 0, 0, 0)) -> CacheAttnParams:
     """What Ctx.cache_attn takes beside the caches (ps_cache_attn_params): made once for a step's buffers, passed every step."""
-    return CacheAttnParams(heads, n_new, scale, 0, _dev(q), _dev(out), _dev(k_new), _dev(v_new), *strides, _dev(count, "int32"), _dev(pos_new, "int32"), _dev(tree, "bool"),
-                           _dev(weight_out, "float32"))
+    p = CacheAttnParams(heads, n_new, scale, 0, _rows(q, not any(strides[:2])), _rows(out, not any(strides[2:4])), _rows(k_new, not any(strides[4:])), _rows(v_new, not any(strides[4:])), *strides, _dev(count, "int32"), _dev(pos_new, "int32"), _dev(tree, "bool"), _dev(weight_out, "float32"))
+    p.types = {_type_name(a) for a in (q, out, k_new, v_new) if not (a is None or isinstance(a, int))}  # (Ctx.cache_attn looks whether they are the cache's)
+    return p
 
 
 def cache_evict_args(keep: int, recent: int = 0, first: int = 0, weight_out=None, pos_out=None, n_kv_out=None) -> CacheEvictParams:
@@ -354,6 +373,9 @@ class Ctx:
 
     def cache_attn(self, cache: KVCache, args: CacheAttnParams, space, space_bytes: int):
         """The newest tokens into the caches and their attention (ps_hip_cache_attn)."""
+        types = getattr(args, "types", None)
+        if types and not types.issubset(NUMBERS.get(cache.dtype, types)):
+            raise PSHipError(f"cache_attn: q, out, k_new and v_new {sorted(types)} are not of the cache's type {cache.dtype}")
         self.check(self.L.ps_hip_cache_attn(self.h, cache, args, _dev(space), space_bytes))
 
     def cache_advance(self, cache: KVCache, count, take=None, n_take: int = 0):
@@ -372,7 +394,7 @@ class Ctx:
 
     def sample(self, logits, n: int, rows: int, params: SampleParams, ids, prob=None, dtype: int = F32, stride: int | None = None, space=None, space_bytes: int = 0):
         """A token per row of logits (ps_hip_sample)."""
-        self.check(self.L.ps_hip_sample(self.h, dtype, _dev(logits), n, rows, n if stride is None else stride, params, _dev(ids, "int32"), _dev(prob, "float32"), _dev(space), space_bytes))
+        self.check(self.L.ps_hip_sample(self.h, dtype, _numbers(logits, dtype, stride is None), n, rows, n if stride is None else stride, params, _dev(ids, "int32"), _dev(prob, "float32"), _dev(space), space_bytes))
 
     # ---- weights
     def upload_weight(self, dtype: int, blocks: np.ndarray, K: int, N: int) -> "Weight":
@@ -456,7 +478,8 @@ class Adapters:
 
     def apply(self, x, T: int, ids, out, base=None, dtype: int = F32, ldx: int | None = None, ldo: int | None = None, space=None, space_bytes: int = 0):
         """out[t] = base[t] + scale * up (down x[t]) with the adapter ids[t] (ps_hip_adapters_apply)."""
-        self.ctx.check(self.ctx.L.ps_hip_adapters_apply(self.ctx.h, self.h, dtype, _dev(x), self.K if ldx is None else ldx, T, _dev(ids, "int32"), _dev(base), _dev(out), self.N if ldo is None else ldo, _dev(space),
+        self.ctx.check(self.ctx.L.ps_hip_adapters_apply(self.ctx.h, self.h, dtype, _numbers(x, dtype, ldx is None), self.K if ldx is None else ldx, T, _dev(ids, "int32"),
+                                                        _numbers(base, F32, ldo is None), _numbers(out, F32, ldo is None), self.N if ldo is None else ldo, _dev(space),
                                                         space_bytes))
 
     def close(self):

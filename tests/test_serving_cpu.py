@@ -326,7 +326,7 @@ assert "freed" in refused(made(freed))
 assert "float32" in refused(made(dev(2), weight=dev(2, 2, 64, dtype=torch.float64))) and "int32" in refused(made(dev(2), pos=dev(2, 2, 64, dtype=torch.int64)))
 made(dev(2), weight=dev(2, 2, 64, dtype=torch.float32), pos=dev(2, 2, 64))()
 made(ctx.to_device(np.zeros(8, np.uint8)))()  # a piece of somebody's memory
-q = On(torch.zeros(2, 3, 4, 64).transpose(0, 1))  # rows have strides of their own
+q = On(torch.zeros(2, 3, 4, 64))
 hip.cache_attn_args(q, k, 4, 3, 0.1, tree=dev(2, 3, 3, dtype=torch.bool), count=dev(2))
 hip.cache_attn_args(q, k, 4, 3, 0.1, tree=dev(2, 3, 3, dtype=torch.uint8))
 for x in ({"tree": dev(2, 3, 3)}, {"count": dev(2, dtype=torch.int64)}, {"weight_out": dev(2)}, {"pos_new": dev(2, 3, dtype=torch.int64)}, {"k_new": torch.zeros(4)}):
@@ -341,4 +341,70 @@ refused(lambda: ctx.cache_advance(cache(), dev(2, dtype=torch.int64)))
 s = hip.Adapters(ctx, 8, 12, 2, 4)
 refused(lambda: s.apply(k, 5, dev(5, dtype=torch.int64), k, space=space, space_bytes=1 << 20))
 assert count("hipLaunchKernel") == 0
+""")
+
+
+def test_arrays_of_other_numbers_than_the_call_says_are_refused(child):  # noqa: F811
+    """16-bit logits read as fp32 would be read past their end: an array that knows its type has to have the call's"""
+    child(MADE + """
+import torch
+class On:
+    def __init__(self, *s, dtype): self.x = torch.zeros(*s, dtype=dtype); self.dtype, self.shape = dtype, self.x.shape
+    def data_ptr(self): return (self.x.data_ptr() + 15) // 16 * 16
+    def is_contiguous(self): return True
+f32, f16, b16 = torch.float32, torch.float16, torch.bfloat16
+u, ids = a(), a()
+p = hip.sample_params(u)
+fake.fake_reset()
+for dtype, good, bad in ((hip.F32, (f32,), (f16, b16, torch.float64, torch.int16)), (hip.F16, (f16, torch.int16), (f32, b16)), (hip.BF16, (b16, torch.int16, torch.uint8), (f32, f16, torch.float64))):
+    for t in bad:
+        x = On(999, dtype=t)
+        for f in (lambda: ctx.sample(x, 100, 3, p, ids, dtype=dtype), lambda: hip.kv_cache(dtype, x, u, u, 2, 64, 2, 64), lambda: hip.kv_cache(dtype, u, x, u, 2, 64, 2, 64)): assert "type" in refused(f)
+    for t in good:
+        x = On(999, dtype=t)
+        ctx.sample(x, 100, 3, p, ids, dtype=dtype)
+        hip.kv_cache(dtype, x, u, u, 2, 64, 2, 64)
+assert count("hipLaunchKernel") == 6
+s = hip.Adapters(ctx, 8, 12, 2, 4)
+for x, dtype, base, out in ((On(60, dtype=b16), hip.F32, None, u), (On(60, dtype=f32), hip.BF16, None, u), (On(60, dtype=f32), hip.F32, On(40, dtype=b16), u), (On(60, dtype=f32), hip.F32, None, On(40, dtype=f16))):
+    assert "type" in quiet(lambda: s.apply(x, 5, ids, out, base=base, dtype=dtype, space=space, space_bytes=1 << 20))
+s.apply(On(60, dtype=b16), 5, ids, On(40, dtype=f32), dtype=hip.BF16, space=space, space_bytes=1 << 20)
+for dtype, good, bad in ((hip.F32, f32, b16), (hip.BF16, b16, f32), (hip.F16, f16, b16)):
+    c = cache(dtype=dtype)
+    for i in range(4):
+        for t in (good, bad):
+            x = [On(2, 3, 4, 64, dtype=t if i == j else good) for j in range(4)]
+            q = hip.cache_attn_args(x[0], x[1], 4, 3, 0.1, k_new=x[2], v_new=x[3])
+            if t is good: ctx.cache_attn(c, q, space, 1 << 20)
+            else: assert "type" in quiet(lambda: ctx.cache_attn(c, q, space, 1 << 20))
+""")
+
+
+def test_views_whose_rows_have_strides_come_with_them(child):  # noqa: F811
+    child(MADE + """
+import torch
+class On:
+    def __init__(self, x): self.x, self.dtype, self.shape = x, x.dtype, x.shape
+    def data_ptr(self): return (self.x.data_ptr() + 15) // 16 * 16
+    def is_contiguous(self): return self.x.is_contiguous()
+u, ids = a(), a()
+p = hip.sample_params(u)
+part = lambda *s: On(torch.zeros(*s, dtype=torch.float32)[..., :8])  # the first columns of wider rows
+s = hip.Adapters(ctx, 8, 8, 2, 4)
+w = {"space": space, "space_bytes": 1 << 20}
+wide = part(2, 3, 4, 64)
+for view, told in (
+    (lambda: hip.kv_cache(0, wide, u, u, 2, 3, 4, 8), lambda: hip.kv_cache(0, wide, u, u, 2, 3, 4, 8, strides=(768, 256, 64))),
+    (lambda: hip.kv_cache(0, u, wide, u, 2, 3, 4, 8), lambda: hip.kv_cache(0, u, wide, u, 2, 3, 4, 8, strides=(768, 256, 64))),
+    (lambda: hip.cache_attn_args(wide, u, 1, 3, 0.1), lambda: hip.cache_attn_args(wide, u, 1, 3, 0.1, strides=(192, 64, 0, 0, 0, 0))),
+    (lambda: hip.cache_attn_args(u, wide, 1, 3, 0.1), lambda: hip.cache_attn_args(u, wide, 1, 3, 0.1, strides=(0, 0, 192, 64, 0, 0))),
+    (lambda: hip.cache_attn_args(u, u, 1, 3, 0.1, k_new=wide), lambda: hip.cache_attn_args(u, u, 1, 3, 0.1, k_new=wide, v_new=wide, strides=(0, 0, 0, 0, 192, 64))),
+    (lambda: hip.cache_attn_args(u, u, 1, 3, 0.1, v_new=wide), lambda: None),
+    (lambda: ctx.sample(part(3, 20), 8, 3, p, ids), lambda: ctx.sample(part(3, 20), 8, 3, p, ids, stride=20)),
+    (lambda: s.apply(part(3, 20), 3, ids, u, **w), lambda: s.apply(part(3, 20), 3, ids, u, ldx=20, **w)),
+    (lambda: s.apply(u, 3, ids, part(3, 20), **w), lambda: s.apply(u, 3, ids, part(3, 20), ldo=20, **w)),
+    (lambda: s.apply(u, 3, ids, ids, base=part(3, 20), **w), lambda: s.apply(u, 3, ids, ids, base=part(3, 20), ldo=20, **w)),
+):
+    assert "without strides" in quiet(view)
+    told()
 """)
