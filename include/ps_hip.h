@@ -546,10 +546,11 @@ typedef struct {
 
 /* Attention of the newest tokens: token t < count[s] of sequence s goes into slot n_kv[s] + t (written here where k_new / v_new are given; they are there already where both are NULL; n_kv is not
  * changed: a step may be repeated) and attends to the slots before n_kv[s] and to the new tokens u with tree[s][t][u] != 0, or u <= t where tree is NULL.  Query head h reads kv head
- * h / (heads / kv_heads).  out = soft-max(scale * q . k) . v, zero for a token that sees nothing; sums, maxima and soft-max in fp32, what multiplies the values of 16-bit
- * caches as two 16-bit numbers (2^-17 of a weight off).  weight_out (NULL: not wanted; may be cache->weight): a slot's soft-max weights, summed over all tokens of the call and the query heads of its kv head, added
- * to cache->weight (NULL: to nothing) for the slots before n_kv[s] and set for the new ones; other slots are left as they were.  Tokens that do not fit behind n_kv[s] are left out,
- * as if count[s] were smaller; rows of out behind count[s] are left as they were.  A number that a token does not see does not reach its result, whatever it is. */
+ * h / (heads / kv_heads).  out = soft-max(scale * q . k) . v, zero for a token that sees nothing; sums, maxima and soft-max in fp32, what multiplies the values of 16-bit caches as two 16-bit numbers
+ * (2^-17 of a weight off).  The sums are of values times weights of up to 1, before they are divided: values near 3.4e38 over the number of slots pass what fp32 holds.  A number that a token does not see
+ * does not reach its result, whatever it is; infinite values that it sees are infinite there, those of both signs and NaN are NaN.  weight_out (NULL: not wanted; may be cache->weight): a slot's soft-max
+ * weights, summed over all tokens of the call and the query heads of its kv head, added to cache->weight (NULL: to nothing) for the slots before n_kv[s] and set for the new ones; other slots are left as
+ * they were.  Tokens that do not fit behind n_kv[s] are left out, as if count[s] were smaller; rows of out behind count[s] are left as they were. */
 typedef struct {
     int32_t heads, n_new; /* query heads; rows per sequence of q, out, k_new, v_new, tree (n_new x n_new bytes), pos_new */
     float scale;
